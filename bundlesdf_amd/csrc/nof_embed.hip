@@ -1,0 +1,466 @@
+// Row lookup with scaling and its gradient by sorted ids (nof_embed_fwd / nof_embed_bwd, include/nof_hip.h).
+//
+//   out[i, :]  = scale * table[ids[i], :]                    an id outside [0, V): a row of zeros
+//   grad[v, :] = scale * sum over {i : ids[i] = v} dout[i, :]  an id outside [0, V): no contribution; a row nobody names: zeros
+//
+// Both are bound by memory: the rows read and written once each.  The gradient adds in a fixed order, so equal inputs give equal
+// bits (the hash table's scatter beside it, nof_hash.hip, adds with atomics):
+//   1. a stable radix sort of (id, position): k_embed_hist + one k_embed_scatter per digit, or k_embed_sort_small as one workgroup;
+//   2. k_embed_reduce: a group of lanes owns a run of C sorted positions and one slice of the columns, reads the rows of dout behind
+//      them and writes the sum of every id that lies within the run; an id cut by the run's ends leaves a partial sum.  Further
+//      workgroups of the same launch write the zeros of the rows that no id names -- most of the bytes of a large table;
+//   3. k_embed_join: the partial sums of a cut id, in the order of their runs.
+#include "nof_learn_dev.h"
+
+#define EMB_T 256                       // threads of the streaming kernels
+#define EMB_ZROWS 32                    // table rows per workgroup of the zero role
+#define EMB_SMALL 4096                  // positions that the one-workgroup sort holds in LDS
+#define EMB_SORT_T 512
+#define EMB_SORT_W (EMB_SORT_T / 64)
+#define EMB_BITS 10                     // widest digit of the many-workgroup sort
+#define EMB_MAX_BLOCKS 128
+
+// ---- lookup -----------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int64_t emb_id(const void* __restrict__ ids, int ids64, int64_t i) {
+  return ids64 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
+}
+
+// 2^ls lanes a row, further columns by blockIdx.y
+template <typename T, int V>
+__global__ __launch_bounds__(EMB_T) void k_embed_fwd(const T* __restrict__ table, int64_t stride, const void* __restrict__ ids, int ids64,
+                                                     float scale, T* __restrict__ out, int64_t N, int64_t rows, int D, int ls) {
+  const int lane = threadIdx.x & ((1 << ls) - 1);
+  const int col = (((int)blockIdx.y << ls) + lane) * V;
+  const int64_t step = (int64_t)gridDim.x * (EMB_T >> ls);
+  if (col >= D) return;
+  for (int64_t i = (int64_t)blockIdx.x * (EMB_T >> ls) + (threadIdx.x >> ls); i < N; i += step) {
+    const int64_t id = emb_id(ids, ids64, i);
+    float f[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = 0.0f;
+    if (id >= 0 && id < rows) {
+      lload<T, V>(table + id * stride + col, f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] *= scale;
+    }
+    lstore<T, V>(out + i * D + col, f);
+  }
+}
+
+// ---- stable radix sort of (id, position) ------------------------------------------------------------------------------------------
+// An absent id sorts behind every row as the key V.
+__device__ __forceinline__ uint32_t emb_key(const void* __restrict__ ids, int ids64, int64_t i, int64_t rows) {
+  const int64_t id = emb_id(ids, ids64, i);
+  return id >= 0 && id < rows ? (uint32_t)id : (uint32_t)rows;
+}
+
+// the lanes of this wave that are `in` and hold the same digit as this lane
+__device__ __forceinline__ uint64_t emb_match(uint32_t digit, int bits, bool in) {
+  uint64_t m = __ballot(in);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1u;
+    const uint64_t bal = __ballot(in && one);
+    m &= one ? bal : ~bal;
+  }
+  return m;
+}
+
+struct EmbSort {
+  const void* ids; int ids64; int64_t rows;
+  uint32_t N, per;                      // positions; positions per workgroup (a multiple of EMB_SORT_T)
+  int n_blocks, passes, bits;
+};
+
+// hist[block][digit] of the first pass; clears the histograms of the later ones, which the scatter before each fills
+__global__ __launch_bounds__(EMB_SORT_T) void k_embed_hist(EmbSort s, uint32_t* __restrict__ hist) {
+  __shared__ uint32_t cnt[1 << EMB_BITS];
+  const int bins = 1 << s.bits;
+  for (int d = threadIdx.x; d < bins; d += EMB_SORT_T) cnt[d] = 0;
+  __syncthreads();
+  const uint32_t lo = blockIdx.x * s.per, hi = lo + s.per < s.N ? lo + s.per : s.N;
+  for (uint32_t i = lo + threadIdx.x; i < hi; i += EMB_SORT_T) atomicAdd(&cnt[emb_key(s.ids, s.ids64, i, s.rows) & (bins - 1)], 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < bins; d += EMB_SORT_T) {
+    hist[blockIdx.x * bins + d] = cnt[d];
+    for (int p = 1; p < s.passes; ++p) hist[((size_t)p * s.n_blocks + blockIdx.x) * bins + d] = 0;
+  }
+}
+
+// One digit: a workgroup knows where its keys go from the histogram of all workgroups (at most EMB_MAX_BLOCKS * 4 KiB, from L2), a
+// wave from the counts of the waves before it, a lane from its rank among the equal digits of its wave: no order is left to chance.
+__global__ __launch_bounds__(EMB_SORT_T) void k_embed_scatter(EmbSort s, int pass, const uint32_t* __restrict__ key_in,
+                                                              const uint32_t* __restrict__ pos_in, uint32_t* __restrict__ key_out,
+                                                              uint32_t* __restrict__ pos_out, uint32_t* __restrict__ hist) {
+  __shared__ uint32_t cnt[EMB_SORT_W][1 << EMB_BITS];
+  __shared__ uint32_t wsum[EMB_SORT_W];
+  const int bins = 1 << s.bits, shift = pass * s.bits, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t lo = blockIdx.x * s.per, hi = lo + s.per < s.N ? lo + s.per : s.N, per_wave = s.per / EMB_SORT_W;
+  const uint32_t wlo = lo + w * per_wave < hi ? lo + w * per_wave : hi, whi = wlo + per_wave < hi ? wlo + per_wave : hi;
+  for (int d = threadIdx.x; d < bins * EMB_SORT_W; d += EMB_SORT_T) cnt[d / bins][d % bins] = 0;
+  __syncthreads();
+  for (uint32_t i = wlo + lane; i < whi; i += 64) {
+    const uint32_t k = pass == 0 ? emb_key(s.ids, s.ids64, i, s.rows) : key_in[i];
+    atomicAdd(&cnt[w][(k >> shift) & (bins - 1)], 1u);
+  }
+  // digits 2t and 2t + 1 are thread t's (bins <= 2 * EMB_SORT_T): totals over all workgroups, and over those before this one
+  const uint32_t* h = hist + (size_t)pass * s.n_blocks * bins;
+  uint32_t tot[2] = {0, 0}, before[2] = {0, 0};
+  const int d0 = 2 * threadIdx.x;
+  if (d0 < bins)
+    for (int b = 0; b < s.n_blocks; ++b) {
+      const uint2 x = *reinterpret_cast<const uint2*>(h + (size_t)b * bins + d0);
+      tot[0] += x.x; tot[1] += x.y;
+      if (b < (int)blockIdx.x) { before[0] += x.x; before[1] += x.y; }
+    }
+  uint32_t run = tot[0] + tot[1];
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(run, o);
+    if (lane >= o) run += y;
+  }
+  if (lane == 63) wsum[w] = run;
+  __syncthreads();
+  uint32_t at = run - tot[0] - tot[1];
+  for (int k = 0; k < w; ++k) at += wsum[k];
+  if (d0 < bins) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint32_t next = at + before[q];
+      for (int k = 0; k < EMB_SORT_W; ++k) {
+        const uint32_t c = cnt[k][d0 + q];
+        cnt[k][d0 + q] = next;
+        next += c;
+      }
+      at += tot[q];
+    }
+  }
+  __syncthreads();
+  for (uint32_t base = wlo; base < whi; base += 64) {
+    const uint32_t i = base + lane;
+    const bool in = i < whi;
+    uint32_t k = 0, p = 0;
+    if (in) {
+      k = pass == 0 ? emb_key(s.ids, s.ids64, i, s.rows) : key_in[i];
+      p = pass == 0 ? i : pos_in[i];
+    }
+    const uint32_t digit = (k >> shift) & (bins - 1);
+    const uint64_t same = emb_match(digit, s.bits, in);
+    const int leader = in ? __ffsll((unsigned long long)same) - 1 : lane;
+    uint32_t old = 0;
+    if (in && lane == leader) old = atomicAdd(&cnt[w][digit], (uint32_t)__popcll(same));
+    old = __shfl(old, leader);
+    if (in) {
+      const uint32_t to = old + (uint32_t)__popcll(same & (((uint64_t)1 << lane) - 1));
+      key_out[to] = k;
+      pos_out[to] = p;
+      if (pass + 1 < s.passes) atomicAdd(&hist[((size_t)(pass + 1) * s.n_blocks + to / s.per) * bins + ((k >> (shift + s.bits)) & (bins - 1))], 1u);
+    }
+  }
+}
+
+// The whole sort as one workgroup of sixteen waves, 8 bits a digit, keys and positions in LDS (56 KiB).
+__global__ __launch_bounds__(1024) void k_embed_sort_small(const void* __restrict__ ids, int ids64, int64_t rows, int N, int passes,
+                                                           uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out) {
+  __shared__ uint32_t key[2][EMB_SMALL];
+  __shared__ uint16_t pos[2][EMB_SMALL];
+  __shared__ uint32_t cnt[16][128];                                  // two digits a word: counts stay below 2^16
+  __shared__ uint32_t wsum[2];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int per_wave = ((N + 1023) / 1024) * 64, wlo = w * per_wave < N ? w * per_wave : N, whi = wlo + per_wave < N ? wlo + per_wave : N;
+  for (int i = threadIdx.x; i < N; i += 1024) { key[0][i] = emb_key(ids, ids64, i, rows); pos[0][i] = (uint16_t)i; }
+  int cur = 0;
+  for (int pass = 0; pass < passes; ++pass, cur ^= 1) {
+    for (int d = threadIdx.x; d < 16 * 128; d += 1024) cnt[d >> 7][d & 127] = 0;
+    __syncthreads();
+    for (int i = wlo + lane; i < whi; i += 64) {
+      const uint32_t g = (key[cur][i] >> (8 * pass)) & 255u;
+      atomicAdd(&cnt[w][g >> 1], 1u << (16 * (g & 1)));
+    }
+    __syncthreads();
+    // thread t < 128 owns digits 2t and 2t + 1
+    uint32_t tot = 0, tot2 = 0, run = 0;
+    const int d = threadIdx.x;
+    if (d < 128) {
+      for (int k = 0; k < 16; ++k) { tot += cnt[k][d] & 0xffffu; tot2 += cnt[k][d] >> 16; }
+      run = tot + tot2;
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(run, o);
+        if (lane >= o) run += y;
+      }
+      if (lane == 63) wsum[w] = run;
+    }
+    __syncthreads();
+    if (d < 128) {
+      uint32_t next = run - tot - tot2 + (w == 1 ? wsum[0] : 0u), next2 = next + tot;
+      for (int k = 0; k < 16; ++k) {
+        const uint32_t c = cnt[k][d];
+        cnt[k][d] = next | (next2 << 16);
+        next += c & 0xffffu;
+        next2 += c >> 16;
+      }
+    }
+    __syncthreads();
+    for (int base = wlo; base < whi; base += 64) {
+      const int i = base + lane;
+      const bool in = i < whi;
+      const uint32_t k = in ? key[cur][i] : 0u, g = (k >> (8 * pass)) & 255u;
+      const uint64_t same = emb_match(g, 8, in);
+      const int leader = in ? __ffsll((unsigned long long)same) - 1 : lane;
+      uint32_t old = 0;
+      if (in && lane == leader) old = atomicAdd(&cnt[w][g >> 1], (uint32_t)__popcll(same) << (16 * (g & 1)));
+      old = (__shfl(old, leader) >> (16 * (g & 1))) & 0xffffu;
+      if (in) {
+        const int to = (int)old + __popcll(same & (((uint64_t)1 << lane) - 1));
+        key[cur ^ 1][to] = k;
+        pos[cur ^ 1][to] = pos[cur][i];
+      }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < N; i += 1024) { key_out[i] = key[cur][i]; pos_out[i] = pos[cur][i]; }
+}
+
+// ---- sums over the sorted positions -----------------------------------------------------------------------------------------------
+// first position whose key is >= v
+__device__ __forceinline__ uint32_t emb_lower(const uint32_t* __restrict__ key, uint32_t n, uint32_t v) {
+  uint32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const uint32_t mid = lo + ((hi - lo) >> 1);
+    if (key[mid] < v) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void emb_put(T* __restrict__ grad, int64_t row, int D, int col, float scale, const float (&acc)[V]) {
+  float f[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) f[k] = acc[k] * scale;
+  lstore<T, V>(grad + row * D + col, f);
+}
+
+// part [chunk][2][D]: the sum of the id that a run inherits from the run before it, and of the one that it starts and hands on
+template <typename T, int V>
+__global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ dout, int64_t stride, const uint32_t* __restrict__ key,
+                                                        const uint32_t* __restrict__ pos, uint32_t N, uint32_t rows, int D, float scale,
+                                                        T* __restrict__ grad, float* __restrict__ part, int ls, int C, uint32_t n_red) {
+  const int lane = threadIdx.x & ((1 << ls) - 1);
+  const int col = (((int)blockIdx.y << ls) + lane) * V;
+  if (blockIdx.x >= n_red) {                                          // the zero role
+    __shared__ uint8_t named[EMB_ZROWS];
+    const uint32_t v0 = (blockIdx.x - n_red) * EMB_ZROWS;
+    if (threadIdx.x < EMB_ZROWS) {
+      const uint32_t v = v0 + threadIdx.x;
+      const uint32_t at = v < rows ? emb_lower(key, N, v) : 0;
+      named[threadIdx.x] = v >= rows || (at < N && key[at] == v);
+    }
+    __syncthreads();
+    float z[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) z[k] = 0.0f;
+    if (col < D)
+      for (int r = threadIdx.x >> ls; r < EMB_ZROWS; r += EMB_T >> ls)
+        if (!named[r]) lstore<T, V>(grad + (int64_t)(v0 + r) * D + col, z);
+    return;
+  }
+  const uint32_t chunk = blockIdx.x * (EMB_T >> ls) + (threadIdx.x >> ls);
+  const uint64_t first = (uint64_t)chunk * C;
+  if (first >= N || col >= D) return;
+  const uint32_t lo = (uint32_t)first, hi = N - lo > (uint32_t)C ? lo + C : N;
+  uint32_t cur = key[lo];
+  if (cur >= rows) return;                                            // absent ids are last
+  bool inherited = lo > 0 && key[lo - 1] == cur;
+  float acc[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+  constexpr int U = 4;
+  for (uint32_t i = lo; i < hi; i += U) {
+    uint32_t kk[U];
+    float x[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      kk[u] = i + u < hi ? key[i + u] : rows;
+      if (kk[u] < rows) lload<T, V>(dout + (int64_t)pos[i + u] * stride + col, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (kk[u] != cur) {                                             // an id ends here (or the run does: `rows`)
+        if (cur < rows && i + u < hi) {
+          if (inherited) lstore<float, V>(part + ((size_t)chunk * 2) * D + col, acc);
+          else emb_put<T, V>(grad, cur, D, col, scale, acc);
+          inherited = false;
+          cur = kk[u];
+#pragma unroll
+          for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+        }
+      }
+      if (kk[u] < rows) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += x[u][k];
+      }
+    }
+  }
+  if (cur >= rows) return;
+  const bool on = hi < N && key[hi] == cur;
+  if (inherited) lstore<float, V>(part + ((size_t)chunk * 2) * D + col, acc);
+  else if (on) lstore<float, V>(part + ((size_t)chunk * 2 + 1) * D + col, acc);
+  else emb_put<T, V>(grad, cur, D, col, scale, acc);
+}
+
+// the run in which a cut id starts adds what the runs behind it inherited
+template <typename T, int V>
+__global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict__ key, uint32_t N, uint32_t rows, int D, float scale,
+                                                      T* __restrict__ grad, const float* __restrict__ part, int ls, int C) {
+  const int lane = threadIdx.x & ((1 << ls) - 1);
+  const int col = (((int)blockIdx.y << ls) + lane) * V;
+  const uint32_t chunk = blockIdx.x * (EMB_T >> ls) + (threadIdx.x >> ls);
+  const uint64_t first = (uint64_t)chunk * C, end = first + C;
+  if (end >= N || col >= D) return;
+  const uint32_t lo = (uint32_t)first, id = key[end - 1];
+  if (id >= rows || key[end] != id) return;                           // nothing handed on
+  if (key[lo] == id && lo > 0 && key[lo - 1] == id) return;           // nor started here
+  const uint32_t last = (emb_lower(key + end, (uint32_t)(N - end), id + 1) + (uint32_t)end - 1) / C;    // the run that it ends in
+  float acc[V], x[V];
+  lload<float, V>(part + ((size_t)chunk * 2 + 1) * D + col, acc);
+#pragma unroll 4
+  for (uint32_t c = chunk + 1; c <= last; ++c) {
+    lload<float, V>(part + ((size_t)c * 2) * D + col, x);
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] += x[k];
+  }
+  emb_put<T, V>(grad, id, D, col, scale, acc);
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------------
+// sorted positions per run: long where there is work for every compute unit anyway, short where a run is the critical path
+static int emb_chunk(int64_t N, int32_t D) {
+  const int64_t e = N * D;
+  return e >= (int64_t)1 << 26 ? 64 : e >= (int64_t)1 << 24 ? 32 : e >= (int64_t)1 << 22 ? 16 : 8;
+}
+
+struct EmbPlan { EmbSort s; bool small; int64_t key[2], pos[2], hist, part, bytes; int C; uint32_t chunks; };
+
+static EmbPlan emb_plan(int64_t N, int64_t rows, int32_t D) {
+  EmbPlan p = {};
+  const int bits = learn_log2_up(rows + 1) > 0 ? learn_log2_up(rows + 1) : 1;
+  p.small = N <= EMB_SMALL;
+  p.s.N = (uint32_t)N;
+  p.s.rows = rows;
+  if (p.small) {
+    p.s.passes = (bits + 7) / 8;
+  } else {
+    p.s.passes = (bits + EMB_BITS - 1) / EMB_BITS;
+    p.s.bits = (bits + p.s.passes - 1) / p.s.passes;
+    const int64_t want = nof_div_up(N, 1024);
+    const int64_t per = nof_div_up(N, want < EMB_MAX_BLOCKS ? want : EMB_MAX_BLOCKS);
+    p.s.per = (uint32_t)(nof_div_up(per, EMB_SORT_T) * EMB_SORT_T);
+    p.s.n_blocks = (int)nof_div_up(N, p.s.per);
+  }
+  p.C = emb_chunk(N, D);
+  p.chunks = (uint32_t)nof_div_up(N, p.C);
+  int64_t at = 0;
+  for (int k = 0; k < 2; ++k) {
+    p.key[k] = at; at += learn_align(4 * N);
+    p.pos[k] = at; at += learn_align(4 * N);
+  }
+  p.hist = at; at += learn_align(p.small ? 0 : (int64_t)4 * p.s.passes * p.s.n_blocks << p.s.bits);
+  p.part = at; at += learn_align((int64_t)p.chunks * 2 * D * 4);
+  p.bytes = at;
+  return p;
+}
+
+static bool emb_sizes_ok(int64_t N, int64_t V, int32_t D) {
+  return N >= 0 && N < ((int64_t)1 << 31) - 65536 && V >= 0 && V < (int64_t)1 << 30 && D >= 0 && D <= 1 << 20;
+}
+
+// elements per access: 16 bytes where every row starts on a 16-byte border, else 4, else one element
+static int emb_vec(int32_t type, int32_t D, int64_t stride, const void* a, const void* b) {
+  const int size = (int)learn_type_size(type);
+  for (int v = 16 / size; v > 1; v = v * size == 16 ? 4 / size : 1)
+    if (D % v == 0 && stride % v == 0 && (((uintptr_t)a | (uintptr_t)b) % (uintptr_t)(v * size)) == 0) return v;
+  return 1;
+}
+
+#define EMB_PICK(NAME, ...)                                                                                                    \
+  do {                                                                                                                         \
+    if (type == NOF_TYPE_F32) { if (v == 4) NAME<float, 4>(__VA_ARGS__); else NAME<float, 1>(__VA_ARGS__); }                   \
+    else if (type == NOF_TYPE_BF16) { if (v == 8) NAME<__bf16, 8>(__VA_ARGS__); else if (v == 2) NAME<__bf16, 2>(__VA_ARGS__); \
+                                      else NAME<__bf16, 1>(__VA_ARGS__); }                                                     \
+    else { if (v == 8) NAME<_Float16, 8>(__VA_ARGS__); else if (v == 2) NAME<_Float16, 2>(__VA_ARGS__);                        \
+           else NAME<_Float16, 1>(__VA_ARGS__); }                                                                              \
+  } while (0)
+
+template <typename T, int V>
+static void emb_launch_fwd(const void* table, int64_t stride, const void* ids, int ids64, float scale, void* out, int64_t N, int64_t rows,
+                           int32_t D, hipStream_t st) {
+  const int64_t nv = D / V;
+  const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
+  const int64_t want = nof_div_up(N, EMB_T >> ls), most = (int64_t)1 << 20;
+  hipLaunchKernelGGL((k_embed_fwd<T, V>), dim3((unsigned)(want < most ? want : most), (unsigned)nof_div_up(nv, (int64_t)1 << ls)), dim3(EMB_T), 0, st,
+                     (const T*)table, stride, ids, ids64, scale, (T*)out, N, rows, D, ls);
+}
+
+template <typename T, int V>
+static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* key, const uint32_t* pos, float scale, void* grad, float* part,
+                            const EmbPlan& p, int32_t D, hipStream_t st) {
+  const int64_t nv = D / V;
+  const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
+  const unsigned cols = (unsigned)nof_div_up(nv, (int64_t)1 << ls), n_red = (unsigned)nof_div_up(p.chunks, EMB_T >> ls);
+  const unsigned n_zero = (unsigned)nof_div_up(p.s.rows, EMB_ZROWS);
+  hipLaunchKernelGGL((k_embed_reduce<T, V>), dim3(n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N,
+                     (uint32_t)p.s.rows, D, scale, (T*)grad, part, ls, p.C, n_red);
+  if (p.chunks > 1)
+    hipLaunchKernelGGL((k_embed_join<T, V>), dim3(n_red, cols), dim3(EMB_T), 0, st, key, p.s.N, (uint32_t)p.s.rows, D, scale, (T*)grad,
+                       (const float*)part, ls, p.C);
+}
+
+extern "C" int nof_embed_fwd(const void* table, int64_t table_stride, int32_t type, const void* ids, int32_t ids64, float scale, void* out,
+                             int64_t N, int64_t V, int32_t D, void* stream) {
+  NOF_ARG(learn_type_ok(type) && (ids64 == 0 || ids64 == 1));
+  NOF_ARG(emb_sizes_ok(N, V, D) && table_stride >= 0);
+  if (N == 0 || D == 0) return 0;
+  NOF_ARG(ids && out && (table || V == 0));
+  const int v = emb_vec(type, D, table_stride, table, out);
+  EMB_PICK(emb_launch_fwd, table, table_stride, ids, ids64, scale, out, N, V, D, (hipStream_t)stream);
+  NOF_LAUNCH_OK();
+  return 0;
+}
+
+extern "C" int64_t nof_embed_bwd_workspace_bytes(int64_t N, int64_t V, int32_t D) {
+  return emb_sizes_ok(N, V, D) ? emb_plan(N, V, D).bytes : -1;
+}
+
+extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type, const void* ids, int32_t ids64, float scale,
+                             void* grad_table, void* workspace, int64_t workspace_bytes, int64_t N, int64_t V, int32_t D, void* stream) {
+  NOF_ARG(learn_type_ok(type) && (ids64 == 0 || ids64 == 1));
+  NOF_ARG(emb_sizes_ok(N, V, D) && dout_stride >= 0);
+  if (V == 0 || D == 0) return 0;
+  NOF_ARG(grad_table && (N == 0 || (dout && ids && workspace)));
+  EmbPlan p = emb_plan(N, V, D);
+  NOF_ARG(N == 0 || workspace_bytes >= p.bytes);
+  NOF_ARG(N == 0 || ((uintptr_t)workspace & 255) == 0);
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  uint32_t *key[2] = {nullptr, nullptr}, *pos[2] = {nullptr, nullptr};
+  float* part = nullptr;
+  int cur = 0;
+  if (N > 0) {
+    for (int k = 0; k < 2; ++k) { key[k] = (uint32_t*)(ws + p.key[k]); pos[k] = (uint32_t*)(ws + p.pos[k]); }
+    part = (float*)(ws + p.part);
+    uint32_t* hist = (uint32_t*)(ws + p.hist);
+    p.s.ids = ids;
+    p.s.ids64 = ids64;
+    if (p.small) {
+      hipLaunchKernelGGL(k_embed_sort_small, dim3(1), dim3(1024), 0, st, ids, (int)ids64, V, (int)N, p.s.passes, key[0], pos[0]);
+    } else {
+      hipLaunchKernelGGL(k_embed_hist, dim3(p.s.n_blocks), dim3(EMB_SORT_T), 0, st, p.s, hist);
+      for (int pass = 0; pass < p.s.passes; ++pass, cur ^= 1)
+        hipLaunchKernelGGL(k_embed_scatter, dim3(p.s.n_blocks), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur],
+                           (const uint32_t*)pos[cur], key[cur ^ 1], pos[cur ^ 1], hist);
+    }
+    NOF_LAUNCH_OK();
+  }
+  const int v = emb_vec(type, D, dout_stride, dout, grad_table);
+  EMB_PICK(emb_launch_sums, dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
+  NOF_LAUNCH_OK();
+  return 0;
+}

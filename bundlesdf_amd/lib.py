@@ -173,9 +173,12 @@ _SIGNATURES = {
     'nof_encode_mlp_wide_fwd': ([C.POINTER(NofHashGrid), C.POINTER(NofMlpDesc), _P, _P, _P, _P, _I32, _P, _P, _P, _I64, _P], C.c_int),
     'nof_mlp_wide_bwd_parts': ([C.POINTER(NofMlpDesc), _P, _P, _P, _I32, _P, _I32, _P, _P, _P, _P, _P, _P, _I32, _I64, _P], C.c_int),
     'nof_texture_bake_frame': ([_P, _P, _I32, _I32, _P, _P, _I64, _P, _P, _P, _F, _I32, _P, _P, _P, _P, _P], C.c_int),
+    'nof_embed_fwd': ([_P, _I64, _I32, _P, _I32, _F, _P, _I64, _I64, _I32, _P], C.c_int),
+    'nof_embed_bwd_workspace_bytes': ([_I64, _I64, _I32], C.c_int64),
+    'nof_embed_bwd': ([_P, _I64, _I32, _P, _I32, _F, _P, _P, _I64, _I64, _I64, _I32, _P], C.c_int),
 }
 OPTIONAL = set()
-ABI_VERSION = 122           # include/nof_hip.h: NOF_ABI_VERSION
+ABI_VERSION = 123           # include/nof_hip.h: NOF_ABI_VERSION
 
 _lib = None
 

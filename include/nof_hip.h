@@ -39,8 +39,9 @@ const char* nof_last_error(void);
  *   110  round 5: nof_batch_trace gained `marcher` (in the middle of its argument list); NofSampleCfg gained `marcher` (trailing)
  *   120  round 6: nof_mlp_wide_bwd_parts gained `featq`; the wide networks' workspace holds the sigma head's hand-off only
  *   121  round 6: new entry points nof_encode_mlp_wide_fwd, nof_mcl_count_blocks, nof_mcl_emit_blocks (nothing existing changed);
- *        the wide entry points refuse precisions 3 / 4 instead of running them as 2 / 1 */
-#define NOF_ABI_VERSION 122
+ *        the wide entry points refuse precisions 3 / 4 instead of running them as 2 / 1
+ *   123  new entry points: the learning operators at the end (nothing existing changed) */
+#define NOF_ABI_VERSION 123
 int nof_version(void);
 
 /* ---- multires hash grid (replaces gridencoder.*) --------------------------------------------- */
@@ -548,6 +549,25 @@ int nof_adam_step_tail_dyn(float* params, float* grads, float* exp_avg, float* e
 /* flags[0] |= 4 when any of grad[0, n) is not finite (the check of nof_reduce_partials, for a gradient that was summed over the
  * data-parallel ranks afterwards: every rank must skip the same step). */
 int nof_grad_check(const float* grad, int64_t n, int32_t* flags, void* stream);
+
+/* ---- learning operators: row lookup with a sorted gradient, gated scan, orthogonalised update ------------------------------------
+ * Operators that the reference leaves to its tensor library (the per-frame codes of FeatureArray nerf_helpers.py:119, the blend of
+ * samples along a ray nerf_runner.py:1132-1169, the optimiser's update :492-504), for any element type below, on caller-owned buffers.
+ * They live beside nof_hash_encode_*, nof_composite_loss and nof_adam_step and share this header's conventions; `workspace` is
+ * 256-byte aligned, its content is undefined before and after a call, and two calls that may run at the same time need two of them. */
+#define NOF_TYPE_F32 0
+#define NOF_TYPE_BF16 1
+#define NOF_TYPE_F16 2
+/* out [N,D] = scale * table[ids[i]]; table [V,D] with `table_stride` elements between rows; ids [N] int32 (ids64 = 0) or int64 (1).
+ * An id outside [0, V) gives a row of zeros (as nof_hash_encode_fwd does for a point outside its box).  N < 2^31 - 65536, V < 2^30,
+ * D <= 2^20. */
+int nof_embed_fwd(const void* table, int64_t table_stride, int32_t type, const void* ids, int32_t ids64, float scale, void* out,
+                  int64_t N, int64_t V, int32_t D, void* stream);
+/* grad_table [V,D], overwritten, = scale * the sum of the rows of dout [N,D] (row stride `dout_stride`) whose id names the row; ids
+ * outside [0, V) contribute nothing.  Sums in binary32, in the order of the positions: equal inputs give equal bits. */
+int64_t nof_embed_bwd_workspace_bytes(int64_t N, int64_t V, int32_t D);
+int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type, const void* ids, int32_t ids64, float scale, void* grad_table,
+                  void* workspace, int64_t workspace_bytes, int64_t N, int64_t V, int32_t D, void* stream);
 
 #ifdef __cplusplus
 }
