@@ -93,3 +93,129 @@ def embed_lookup_grad(dout, ids, n_rows, scale=1.0):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call(dev, 'nof_embed_bwd', dout.data_ptr(), stride, _TYPE[dout.dtype], ids, _INT64[ids.dtype], float(scale), grad, ws, nbytes, N, n_rows, D)
     return grad
+
+
+# ---- gated recurrence along time ------------------------------------------------------------------------------------------------------
+def _scan_even(dtype, D, G):
+    """whether the kernels take two channels per lane (csrc/nof_scan.hip: scan_vec)"""
+    return dtype != torch.float32 and (D if G == D else D // G) % 2 == 0
+
+
+def _scan_strided(x, even):
+    """x [B, T, C] (or [B, C]) as the kernels take it: channels side by side, two-channel loads on their border"""
+    if x.shape[-1] > 1 and x.stride(-1) != 1:
+        x = x.contiguous()
+    if even and (x.data_ptr() % (2 * x.element_size()) or any(s % 2 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1)):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _scan_strides(x):
+    return tuple(s if n > 1 else 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]))
+
+
+def _state_ok(what, name, x, B, D):
+    _need(x is None or (x.dtype == torch.float32 and x.shape == (B, D)), f'{what}: {name} must be [B, D] float32')
+
+
+def _scan_args(what, gate, value, lengths, dims):
+    _need(value.dim() == dims and value.dtype in _TYPE, f'{what}: value must be [{"B, T, D" if dims == 3 else "B, D"}] float32, bfloat16 or float16')
+    _need(gate.dim() == dims and gate.shape[:-1] == value.shape[:-1], f"{what}: gate must have value's shape but for the channels")
+    _need(gate.dtype in (value.dtype, torch.float32), f"{what}: gate must be float32 or of value's type")
+    D, G = value.shape[-1], gate.shape[-1]
+    _need(D == 0 or (G > 0 and D % G == 0), f'{what}: the number of gates per position must divide the number of channels')
+    _need(D <= 1 << 20 and value.shape[0] < 1 << 24 and (dims == 2 or value.shape[1] < 1 << 31), f'{what}: sizes out of range')
+    if lengths is not None:
+        _need(lengths.dtype == torch.int32 and lengths.shape == value.shape[:1], f'{what}: lengths must be [B] int32')
+    return D, G
+
+
+def _scan_bytes(kind, B, T, D, G, dtype):
+    n = getattr(lib.load(), f'nof_gated_scan_{kind}_bytes')(B, T, D, G, _TYPE[dtype])
+    _need(n >= 0, f'gated_scan: sizes out of range (B = {B}, T = {T}, D = {D}, G = {G})')
+    return n
+
+
+def gated_scan(gate, value, state=None, lengths=None, reverse=False, want_marks=False):
+    """h[:, t] = gate[:, t] * h[:, t-1] + value[:, t] with h[:, -1] = state (None: zeros) -> (h [B, T, D] in value's type, the last h
+    [B, D] float32), and with want_marks the float32 states that gated_scan_grad starts from.
+
+    gate [B, T, G] (value's type or float32), value [B, T, D]; G divides D: channel d uses gate d // (D // G) -- G = D is a gate per
+    channel, G = 1 one for all.  lengths [B] int32: rows from lengths[b] on do not exist (not read; zeros in h).  reverse: from the last
+    existing row to the first -- with gate = 1 - opacity and value = opacity * feature, h[:, 0] is the ray's blend, back to front.
+    Gates compose over positions in float32: their products must stay in its range (|gate| <= 1 always does)."""
+    D, G = _scan_args('gated_scan', gate, value, lengths, 3)
+    B, T = value.shape[:2]
+    _state_ok('gated_scan', 'state', state, B, D)
+    dev = _on_device('gated_scan', gate, value, state, lengths)
+    return _scan_forward(dev, gate, value, state, lengths, reverse, want_marks, True)
+
+
+def _scan_forward(dev, gate, value, state, lengths, reverse, want_marks, want_h):
+    B, T, D = value.shape
+    G = gate.shape[-1]
+    dt = value.dtype
+    even = _scan_even(dt, D, G)
+    value, gate = _scan_strided(value, even), _scan_strided(gate, even and G == D)
+    state = _scan_strided(state.contiguous(), even) if state is not None else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    h = torch.empty((B, T, D), dtype=dt, device=dev) if want_h else None
+    last = torch.empty((B, D), dtype=torch.float32, device=dev) if want_h else None
+    marks = torch.empty(_scan_bytes('marks', B, T, D, G, dt) // 4, dtype=torch.float32, device=dev) if want_marks else None
+    nbytes = _scan_bytes('workspace', B, T, D, G, dt)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call(dev, 'nof_gated_scan_fwd', gate.data_ptr(), *_scan_strides(gate), _TYPE[gate.dtype], value.data_ptr(), *_scan_strides(value), _TYPE[dt],
+          state, lengths, int(bool(reverse)), h, last, marks, ws, nbytes, B, T, D, G)
+    return (h, last, marks) if want_marks else (h, last)
+
+
+def gated_scan_grad(gate, value, dh, dlast=None, state=None, marks=None, lengths=None, reverse=False):
+    """The gradients of gated_scan: dh [B, T, D] and dlast [B, D] float32 (None: zeros) are the loss's gradients of its two results; the
+    other arguments are the forward's.  -> (dgate in gate's type, summed over the channels that share it, dvalue, dstate [B, D] float32).
+    marks: what gated_scan(..., want_marks=True) gave for the same gate, value, state, lengths and reverse; None recomputes them."""
+    D, G = _scan_args('gated_scan_grad', gate, value, lengths, 3)
+    B, T = value.shape[:2]
+    dt = value.dtype
+    _need(dh.shape == value.shape and dh.dtype == dt, "gated_scan_grad: dh must have value's shape and type")
+    _state_ok('gated_scan_grad', 'state', state, B, D)
+    _state_ok('gated_scan_grad', 'dlast', dlast, B, D)
+    if marks is not None:
+        _need(marks.dtype == torch.float32 and marks.dim() == 1 and marks.numel() * 4 == _scan_bytes('marks', B, T, D, G, dt),
+              'gated_scan_grad: marks are not those of a forward pass of these sizes')
+    dev = _on_device('gated_scan_grad', gate, value, dh, dlast, state, marks, lengths)
+    if marks is None:
+        marks = _scan_forward(dev, gate, value, state, lengths, reverse, True, False)[2]
+    even = _scan_even(dt, D, G)
+    value, gate, dh = _scan_strided(value, even), _scan_strided(gate, even and G == D), _scan_strided(dh, even)
+    dlast = _scan_strided(dlast.contiguous(), even) if dlast is not None else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    dgate = torch.empty((B, T, G), dtype=gate.dtype, device=dev)
+    dvalue = torch.empty((B, T, D), dtype=dt, device=dev)
+    dstate = torch.empty((B, D), dtype=torch.float32, device=dev)
+    nbytes = _scan_bytes('workspace', B, T, D, G, dt)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call(dev, 'nof_gated_scan_bwd', gate.data_ptr(), *_scan_strides(gate), _TYPE[gate.dtype], value.data_ptr(), *_scan_strides(value), _TYPE[dt],
+          dh.data_ptr(), *_scan_strides(dh), dlast, marks.contiguous(), lengths, int(bool(reverse)), dgate, dvalue, dstate, ws, nbytes, B, T, D, G)
+    return dgate, dvalue, dstate
+
+
+def gated_scan_step(gate, value, state, new_state=None):
+    """One position of gated_scan: gate [B, G], value [B, D], state [B, D] float32 -> (h [B, D] in value's type, the new state).
+    new_state: where the new state goes (`state` itself for an update in place); None allocates it."""
+    D, G = _scan_args('gated_scan_step', gate, value, None, 2)
+    B = value.shape[0]
+    _need(state is not None, 'gated_scan_step: state must be [B, D] float32')
+    _state_ok('gated_scan_step', 'state', state, B, D)
+    _state_ok('gated_scan_step', 'new_state', new_state, B, D)
+    dev = _on_device('gated_scan_step', gate, value, state, new_state)
+    _need(new_state is None or new_state.is_contiguous(), 'gated_scan_step: new_state must be contiguous')
+    even = _scan_even(value.dtype, D, G)
+    value, gate = _scan_strided(value, even), _scan_strided(gate, even and G == D)
+    state = _scan_strided(state.contiguous(), even)
+    _need(new_state is None or not even or new_state.data_ptr() % 8 == 0, 'gated_scan_step: new_state must start on an 8-byte border')
+    if new_state is None:
+        new_state = torch.empty((B, D), dtype=torch.float32, device=dev)
+    h = torch.empty((B, D), dtype=value.dtype, device=dev)
+    _call(dev, 'nof_gated_scan_step', gate.data_ptr(), *_scan_strides(gate), _TYPE[gate.dtype], value.data_ptr(), *_scan_strides(value),
+          _TYPE[value.dtype], state, new_state, h, B, D, G)
+    return h, new_state

@@ -175,6 +175,12 @@ _SIGNATURES = {
     'nof_texture_bake_frame': ([_P, _P, _I32, _I32, _P, _P, _I64, _P, _P, _P, _F, _I32, _P, _P, _P, _P, _P], C.c_int),
     'nof_embed_fwd': ([_P, _I64, _I32, _P, _I32, _F, _P, _I64, _I64, _I32, _P], C.c_int),
     'nof_embed_bwd_workspace_bytes': ([_I64, _I64, _I32], C.c_int64),
+    'nof_gated_scan_marks_bytes': ([_I64, _I64, _I32, _I32, _I32], C.c_int64),
+    'nof_gated_scan_workspace_bytes': ([_I64, _I64, _I32, _I32, _I32], C.c_int64),
+    'nof_gated_scan_fwd': ([_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _P, _I32, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _P], C.c_int),
+    'nof_gated_scan_bwd': ([_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _P, _I32, _P, _P, _P, _P, _I64, _I64, _I64, _I32,
+                            _I32, _P], C.c_int),
+    'nof_gated_scan_step': ([_P, _I64, _I32, _P, _I64, _I32, _P, _P, _P, _I64, _I32, _I32, _P], C.c_int),
     'nof_embed_bwd': ([_P, _I64, _I32, _P, _I32, _F, _P, _P, _I64, _I64, _I64, _I32, _P], C.c_int),
 }
 OPTIONAL = set()

@@ -568,6 +568,29 @@ int nof_embed_fwd(const void* table, int64_t table_stride, int32_t type, const v
 int64_t nof_embed_bwd_workspace_bytes(int64_t N, int64_t V, int32_t D);
 int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type, const void* ids, int32_t ids64, float scale, void* grad_table,
                   void* workspace, int64_t workspace_bytes, int64_t N, int64_t V, int32_t D, void* stream);
+/* Gated linear recurrence along time: h[t] = gate[t] h[t-1] + value[t], h[-1] = state.  gate [B,T,G] (type, or float32 beside a 16-bit
+ * type), value and h [B,T,D], G divides D: channel d uses gate d / (D / G), so G = D is a gate per channel and G = 1 one for all.  *_sb /
+ * *_st: elements between batches / positions (channels are side by side); h, dgate, dvalue are contiguous.  state, last [B,D] float32
+ * (state NULL: zeros; last, h and marks may be NULL).  lengths [B] int32 or NULL: only the first lengths[b] rows (clamped to [0, T]) exist;
+ * the others are not read, their rows of h, dgate, dvalue are zeros.  reverse = 1: the recurrence runs from row lengths[b] - 1 down to 0.
+ * Positions compose in parallel, so products of gates over a run of positions must stay within binary32 (|gate| <= 1 always does).
+ * 16-bit types with an even number of channels per group: pointers and strides are multiples of two elements.
+ * B < 2^24, T < 2^31, D <= 2^20. */
+int64_t nof_gated_scan_marks_bytes(int64_t B, int64_t T, int32_t D, int32_t G, int32_t type);
+int64_t nof_gated_scan_workspace_bytes(int64_t B, int64_t T, int32_t D, int32_t G, int32_t type);
+int nof_gated_scan_fwd(const void* gate, int64_t gate_sb, int64_t gate_st, int32_t gate_type, const void* value, int64_t value_sb,
+                       int64_t value_st, int32_t type, const float* state, const int32_t* lengths, int32_t reverse, void* h,
+                       float* last, float* marks, void* workspace, int64_t workspace_bytes, int64_t B, int64_t T, int32_t D,
+                       int32_t G, void* stream);
+/* dh [B,T,D] and dlast [B,D] (NULL: zeros) = the loss's gradients of h and last; marks as the forward of the same inputs wrote them ->
+ * dgate (gate_type; summed over a shared gate's channels), dvalue (type), dstate [B,D] float32 (may be NULL). */
+int nof_gated_scan_bwd(const void* gate, int64_t gate_sb, int64_t gate_st, int32_t gate_type, const void* value, int64_t value_sb,
+                       int64_t value_st, int32_t type, const void* dh, int64_t dh_sb, int64_t dh_st, const float* dlast,
+                       const float* marks, const int32_t* lengths, int32_t reverse, void* dgate, void* dvalue, float* dstate,
+                       void* workspace, int64_t workspace_bytes, int64_t B, int64_t T, int32_t D, int32_t G, void* stream);
+/* one position: gate [B,G], value [B,D], state [B,D] -> new_state [B,D] (may be `state`), h [B,D] = new_state in `type` */
+int nof_gated_scan_step(const void* gate, int64_t gate_sb, int32_t gate_type, const void* value, int64_t value_sb, int32_t type,
+                        const float* state, float* new_state, void* h, int64_t B, int32_t D, int32_t G, void* stream);
 
 #ifdef __cplusplus
 }

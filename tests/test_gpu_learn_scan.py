@@ -1,0 +1,232 @@
+"""The gated recurrence along time (bundlesdf_amd/learn_ops.py: gated_scan, its gradients, its step) against the recurrence itself in
+64 bits, position by position.
+
+Tolerances, with u = 2^-24.  m[t] = |gate| m[t-1] + |value| bounds every partial sum of h[t].  A term value[s] prod(gate) reaches h[t] through
+at most one rounded product per position (whichever way they are composed) and one rounded addition per position, slot, wave, chunk and
+segment: e[t] = |gate| e[t-1] + 3 u m[t] carries those per position, and 64 u m[t] covers the levels of the composition (8 + 6 + 16 + 16 + the
+chunks' own, which are per position again).  r, the gradient of the values, likewise from the other end.  A gate's gradient is a sum of P
+products r h: |r| e_h + |h| e_r + (P + 2) u |r| |h| per term, summed.  Results are rounded once to their type: eps/2 of the value."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+TYPES = [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16), (torch.bfloat16, torch.float32),
+         (torch.float16, torch.float32)]
+U = 2.0 ** -24
+
+
+def recurrence(gate, value, state, lengths, reverse, dh=None, dlast=None):
+    """everything in 64 bits on the CPU: dict of (value, tolerance before the rounding to the type)"""
+    g, x = gate.double().cpu(), value.double().cpu()
+    B, T, D = x.shape
+    G = g.shape[2]
+    P = D // G if G else 1
+    g = g.repeat_interleave(P, 2)
+    n = torch.full((B,), T) if lengths is None else lengths.long().cpu().clamp(0, T)
+    s = torch.zeros(B, D, dtype=torch.float64) if state is None else state.double().cpu()
+    order = [(torch.where(t < n, n - 1 - t, t) if reverse else torch.full((B,), t)) for t in range(T)]
+    rows = torch.arange(B)
+    h, eh, before, ebefore = (torch.zeros(B, T, D, dtype=torch.float64) for _ in range(4))
+    m, e = s.abs(), torch.zeros_like(s)
+    for t in range(T):
+        at, on = order[t], (t < n)[:, None]
+        a, v = g[rows, at], x[rows, at]
+        before[rows, at], ebefore[rows, at] = torch.where(on, s, 0 * s), torch.where(on, e + 64 * U * m, 0 * s)
+        s2 = a * s + v
+        m2 = a.abs() * m + v.abs()
+        e2 = a.abs() * e + 3 * U * m2
+        s, m, e = torch.where(on, s2, s), torch.where(on, m2, m), torch.where(on, e2, e)
+        h[rows, at], eh[rows, at] = torch.where(on, s, 0 * s), torch.where(on, e + 64 * U * m, 0 * s)
+    res = {'h': (h, eh), 'last': (s, e + 64 * U * m)}
+    if dh is None:
+        return res
+    d = dh.double().cpu()
+    c = torch.zeros(B, D, dtype=torch.float64) if dlast is None else dlast.double().cpu()
+    r, er = torch.zeros_like(h), torch.zeros_like(h)
+    m, e = c.abs(), torch.zeros_like(c)
+    for t in reversed(range(T)):
+        at, on = order[t], (t < n)[:, None]
+        a, v = g[rows, at], d[rows, at]
+        q, mq, eq = c + v, m + v.abs(), e + 3 * U * (m + v.abs())
+        r[rows, at], er[rows, at] = torch.where(on, q, 0 * q), torch.where(on, eq + 64 * U * mq, 0 * q)
+        c, m, e = torch.where(on, a * q, c), torch.where(on, a.abs() * mq, m), torch.where(on, a.abs() * eq + 2 * U * mq, e)
+    res['dvalue'] = (r, er)
+    res['dstate'] = (c, e + 64 * U * m)
+    term = r.abs() * ebefore + before.abs() * er + er * ebefore + (P + 2) * U * r.abs() * before.abs()
+    res['dgate'] = ((r * before).reshape(B, T, G, P).sum(3), term.reshape(B, T, G, P).sum(3))
+    return res
+
+
+def check(got, want, name):
+    ref, tol = want
+    eps = torch.finfo(got.dtype).eps
+    tol = tol * (1 + 1e-6) + (eps / 2) * (ref.abs() + tol) + (2.0 ** -25 if got.dtype == torch.float16 else 1e-42)
+    bad = ~((got.double().cpu() - ref).abs() <= tol)
+    assert got.shape == ref.shape and not bad.any(), (name, int(bad.sum()), bad.nonzero()[:3].tolist())
+
+
+def make(B, T, D, G, dtype, gdtype, seed, signed=False):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    gate = torch.sigmoid(torch.randn(B, T, G, device='cuda', generator=gen) * 2 + 1.5)
+    if signed:
+        gate = gate * torch.randn(B, T, G, device='cuda', generator=gen).sign()
+    return (gate.to(gdtype), torch.randn(B, T, D, device='cuda', generator=gen).to(dtype), torch.randn(B, D, device='cuda', generator=gen),
+            torch.randn(B, T, D, device='cuda', generator=gen).to(dtype), torch.randn(B, D, device='cuda', generator=gen))
+
+
+SIZES = [(1, 1, 1, 1), (2, 0, 3, 3), (3, 7, 5, 5), (2, 65, 64, 64), (5, 193, 16, 1), (1, 1025, 33, 3), (2, 600, 130, 2), (1, 5000, 8, 8), (40, 100, 6, 2),
+         (1, 4097, 256, 1), (2, 700, 200, 200), (1, 9001, 3, 1), (2, 130, 1, 1), (3, 64, 24, 3), (1, 3000, 390, 1), (600, 9, 64, 4)]
+
+
+@pytest.mark.parametrize('B,T,D,G', SIZES)
+@pytest.mark.parametrize('kind', range(5))
+def test_forward_and_gradients(nof, B, T, D, G, kind):
+    from bundlesdf_amd import learn_ops as L
+    seed = SIZES.index((B, T, D, G)) + kind
+    dtype, gdtype = TYPES[kind]
+    reverse, ragged, with_state = bool(seed & 1), seed % 3 == 0, seed % 4 != 1
+    gate, value, state, dh, dlast = make(B, T, D, G, dtype, gdtype, seed, signed=seed % 5 == 2)
+    state = state if with_state else None
+    lengths = None
+    if ragged:
+        lengths = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+        lengths[0] = T + 5                                            # clamped
+        if B > 2:
+            lengths[1], lengths[2] = 0, -3                            # nothing there
+        for b in range(B):                                            # what does not exist is not read
+            k = min(max(int(lengths[b]), 0), T)
+            gate[b, k:], value[b, k:], dh[b, k:] = float('nan'), float('inf'), float('nan')
+        lengths = lengths.cuda()
+    clean = lambda x: torch.nan_to_num(x, nan=0.0, posinf=0.0)        # noqa: E731
+    want = recurrence(clean(gate), clean(value), state, lengths, reverse, clean(dh), dlast)
+    h, last, marks = L.gated_scan(gate, value, state, lengths, reverse, want_marks=True)
+    check(h, want['h'], 'h')
+    check(last, want['last'], 'last')
+    assert h.dtype == dtype and last.dtype == torch.float32
+    got = L.gated_scan_grad(gate, value, dh, dlast, state, marks, lengths, reverse)
+    for name, x in zip(('dgate', 'dvalue', 'dstate'), got):
+        check(x, want[name], name)
+    assert got[0].dtype == gdtype and got[1].dtype == dtype
+    again = L.gated_scan_grad(gate, value, dh, dlast, state, None, lengths, reverse)      # marks recomputed; the same bits
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+    h2, last2 = L.gated_scan(gate, value, state, lengths, reverse)
+    assert torch.equal(h, h2) and torch.equal(last, last2)
+
+
+def test_gradients_against_differences(nof):
+    from bundlesdf_amd import learn_ops as L
+    gate, value, state, dh, dlast = make(2, 5, 4, 2, torch.float32, torch.float32, 3)
+    lengths = torch.tensor([5, 3], dtype=torch.int32, device='cuda')
+
+    def loss(g, v, s):
+        h, last = L.gated_scan(g, v, s, lengths, True)
+        return float((h.double() * dh).sum() + (last.double() * dlast).sum())
+
+    grads = L.gated_scan_grad(gate, value, dh, dlast, state, None, lengths, True)
+    for which, (x, g) in enumerate(zip((gate, value, state), grads)):
+        for at in np.ndindex(*x.shape):
+            up, down = x.clone(), x.clone()
+            up[at] += 0.0625
+            down[at] -= 0.0625
+            args = [[gate, value, state][:which] + [y] + [gate, value, state][which + 1:] for y in (up, down)]
+            diff = (loss(*args[0]) - loss(*args[1])) / 0.125          # h is linear in each single input: no error of order step^2
+            assert abs(diff - float(g[at])) < 2e-4, (which, at)       # 40 terms of size <= 10, 2^-24 each, over 0.125
+
+
+def test_blends_a_ray(nof):
+    """gate = 1 - opacity, value = opacity * colour, reversed: the front-to-back compositing sum of transmittance * opacity * colour"""
+    from bundlesdf_amd import learn_ops as L
+    gen = torch.Generator(device='cuda').manual_seed(0)
+    alpha = torch.rand(50, 192, 1, device='cuda', generator=gen) * 0.1
+    colour = torch.rand(50, 192, 3, device='cuda', generator=gen)
+    h, last = L.gated_scan(1 - alpha, alpha * colour, reverse=True)
+    a = alpha.double()
+    T = torch.cumprod(torch.cat((torch.ones_like(a[:, :1]), 1 - a[:, :-1]), 1), 1)
+    want = (T * a * colour.double()).sum(1)
+    assert torch.equal(h[:, 0], last) and (last.double() - want).abs().max() < 1e-5
+
+
+@pytest.mark.parametrize('kind', range(5))
+@pytest.mark.parametrize('B,D,G', [(1, 1, 1), (3, 6, 2), (7, 130, 130), (2, 65, 5), (96, 2048, 2048), (4, 600, 1)])
+def test_step(nof, kind, B, D, G):
+    from bundlesdf_amd import learn_ops as L
+    dtype, gdtype = TYPES[kind]
+    gate, value, state, _, _ = make(B, 1, D, G, dtype, gdtype, kind)
+    want = recurrence(gate, value, state, None, False)
+    h, new = L.gated_scan_step(gate[:, 0], value[:, 0], state)
+    check(new, want['last'], 'state')
+    check(h, (want['h'][0][:, 0], want['h'][1][:, 0]), 'h')
+    h1, last = L.gated_scan(gate, value, state)
+    assert torch.equal(last, new) and torch.equal(h1[:, 0], h)           # one position of the scan is the step
+    h2, same = L.gated_scan_step(gate[:, 0], value[:, 0], state, new_state=state)
+    assert same.data_ptr() == state.data_ptr() and torch.equal(state, new) and torch.equal(h2, h)
+
+
+def test_step_by_step_is_the_scan(nof):
+    from bundlesdf_amd import learn_ops as L
+    gate, value, state, _, _ = make(3, 40, 10, 5, torch.bfloat16, torch.float32, 9)
+    want = recurrence(gate, value, state, None, False)
+    s = state.clone()
+    for t in range(40):
+        h, s = L.gated_scan_step(gate[:, t], value[:, t], s, s)
+        check(h, (want['h'][0][:, t], want['h'][1][:, t]), t)
+
+
+@pytest.mark.parametrize('kind', range(5))
+def test_strides(nof, kind):
+    """slices of wider tensors, starts off the two-channel border, time-major inputs, broadcast gates and gradients"""
+    from bundlesdf_amd import learn_ops as L
+    dtype, gdtype = TYPES[kind]
+    gate, value, state, dh, dlast = make(3, 50, 21, 21, dtype, gdtype, 1)
+    for lo, hi in ((0, 20), (1, 21), (2, 9)):
+        g, v, d = gate[..., lo:hi], value[..., lo:hi], dh[..., lo:hi]
+        s, dl = state[:, lo:hi], dlast[:, lo:hi]
+        for f in (lambda x: x, lambda x: x.transpose(0, 1).contiguous().transpose(0, 1), lambda x: x[:1].expand_as(x), lambda x: x[:, :1].expand_as(x)):
+            a, b, c = f(g), f(v), f(d)
+            want = recurrence(a, b, s, None, True, c, dl)
+            h, last = L.gated_scan(a, b, s, reverse=True)
+            check(h, want['h'], 'h')
+            check(last, want['last'], 'last')
+            for name, x in zip(('dgate', 'dvalue', 'dstate'), L.gated_scan_grad(a, b, c, dl, s, reverse=True)):
+                check(x, want[name], name)
+
+
+def test_what_is_not_finite_stays_in_its_sequence_and_behind(nof):
+    from bundlesdf_amd import learn_ops as L
+    gate, value, state, dh, dlast = make(2, 600, 4, 4, torch.float32, torch.float32, 2)
+    want, _ = L.gated_scan(gate, value, state)
+    bad = value.clone()
+    bad[0, 300, 1] = float('nan')
+    h, last = L.gated_scan(gate, bad, state)
+    assert torch.equal(h[1], want[1]) and torch.equal(h[0, :300], want[0, :300]) and torch.equal(h[0, :, [0, 2, 3]], want[0, :, [0, 2, 3]])
+    assert h[0, 300:, 1].isnan().all() and last[0, 1].isnan()
+
+
+def test_stream_and_graph(nof):
+    from bundlesdf_amd import learn_ops as L
+    gate, value, state, dh, dlast = make(2, 3000, 12, 3, torch.float16, torch.float32, 5)
+    lengths = torch.tensor([3000, 17], dtype=torch.int32, device='cuda')
+
+    def both():
+        h, last, marks = L.gated_scan(gate, value, state, lengths, want_marks=True)
+        return (h, last, *L.gated_scan_grad(gate, value, dh, dlast, state, marks, lengths))
+
+    want = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = both()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = both()
+    gen = torch.Generator(device='cuda').manual_seed(1)
+    for k in range(4):
+        value.normal_(generator=gen)
+        dh.normal_(generator=gen)
+        lengths.copy_(torch.tensor([k * 900, 3000 - k], dtype=torch.int32))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, both()))

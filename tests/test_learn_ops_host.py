@@ -48,3 +48,60 @@ def test_embed_entry_points_refuse():
     assert fwd(N=0) == 0 and fwd(D=0) == 0 and bwd(V=0) == 0 and bwd(D=0) == 0           # nothing to do, nothing touched
     assert so.nof_embed_bwd_workspace_bytes(-1, 4, 4) == -1 and so.nof_embed_bwd_workspace_bytes(0, 4, 4) == 0
     assert so.nof_embed_bwd_workspace_bytes(70001, 1 << 20, 2) > 16 * 70001
+
+
+def test_scan_refusals():
+    g, v, s = torch.zeros(2, 5, 3), torch.zeros(2, 5, 6), torch.zeros(2, 6)
+    n = torch.zeros(2, dtype=torch.int32)
+    assert 'GPU' in refused(L.gated_scan, g, v)
+    assert 'B, T, D' in refused(L.gated_scan, g, v[0])
+    assert 'B, T, D' in refused(L.gated_scan, g, v.double())
+    assert 'but for the channels' in refused(L.gated_scan, g[:, :4], v)
+    assert "float32 or of value's type" in refused(L.gated_scan, g.half(), v)
+    assert "float32 or of value's type" in refused(L.gated_scan, g.half(), v.bfloat16())
+    assert 'divide' in refused(L.gated_scan, torch.zeros(2, 5, 4), v)
+    assert 'divide' in refused(L.gated_scan, torch.zeros(2, 5, 0), v)
+    assert 'divide' in refused(L.gated_scan, torch.zeros(2, 5, 12), v)
+    assert 'state' in refused(L.gated_scan, g, v, s[:1])
+    assert 'state' in refused(L.gated_scan, g, v, s.half())
+    assert 'lengths' in refused(L.gated_scan, g, v, s, n.long())
+    assert 'lengths' in refused(L.gated_scan, g, v, s, n[:1])
+    assert 'dh' in refused(L.gated_scan_grad, g, v, v[:, :4])
+    assert 'dh' in refused(L.gated_scan_grad, g, v, v.half())
+    assert 'dlast' in refused(L.gated_scan_grad, g, v, v, s[:, :2])
+    assert 'marks' in refused(L.gated_scan_grad, g, v, v, s, s, torch.zeros(3))
+    assert 'GPU' in refused(L.gated_scan_grad, g, v, v, s, s)
+    assert 'state' in refused(L.gated_scan_step, g[:, 0], v[:, 0], None)
+    assert 'B, D' in refused(L.gated_scan_step, g, v, s)
+    assert 'new_state' in refused(L.gated_scan_step, g[:, 0], v[:, 0], s, s[:1])
+    assert 'GPU' in refused(L.gated_scan_step, g[:, 0], v[:, 0], s)
+
+
+def test_scan_entry_points_refuse():
+    so = lib.load()
+    null = C.c_void_p(None)
+
+    def fwd(gt=0, t=0, rev=0, B=2, T=5, D=4, G=4, sb=20, st=4, gate=PTR, value=PTR, ws=null, size=0):
+        return so.nof_gated_scan_fwd(gate, sb, st, gt, value, sb, st, t, null, null, rev, PTR, PTR, null, ws, size, B, T, D, G, None)
+
+    def bwd(gt=0, t=0, rev=0, B=2, T=5, D=4, G=4, sb=20, st=4, gate=PTR, value=PTR, dh=PTR, marks=PTR, dgate=PTR, dvalue=PTR, ws=null, size=0):
+        return so.nof_gated_scan_bwd(gate, sb, st, gt, value, sb, st, t, dh, sb, st, null, marks, null, rev, dgate, dvalue, PTR, ws, size, B, T, D, G, None)
+
+    def step(gt=0, t=0, B=2, D=4, G=4, sb=4, gate=PTR, value=PTR, state=PTR, h=PTR):
+        return so.nof_gated_scan_step(gate, sb, gt, value, sb, t, state, PTR, h, B, D, G, None)
+
+    common = [{'t': 3}, {'gt': 1}, {'gt': 2, 't': 1}, {'B': -1}, {'B': 1 << 24}, {'D': -1}, {'D': (1 << 20) + 1}, {'G': 3}, {'G': 0}, {'G': 8}, {'sb': -1},
+              {'gate': None}, {'value': None}, {'t': 1, 'gt': 1, 'value': C.c_void_p(258)}, {'t': 1, 'gt': 1, 'sb': 21}]
+    for f in (fwd, bwd, step):
+        for bad in common:
+            assert f(**bad) < 0 and b'argument check' in so.nof_last_error(), (f.__name__, bad)
+        assert f(B=0) == 0 and f(D=0) == 0
+    for f in (fwd, bwd):
+        for bad in ({'rev': 2}, {'T': -1}, {'T': 1 << 31}, {'st': -1}, {'T': 100000}):          # the last needs a workspace
+            assert f(**bad) < 0 and b'argument check' in so.nof_last_error(), (f.__name__, bad)
+    for bad in ({'dh': None}, {'marks': None}, {'dgate': None}, {'dvalue': None}):
+        assert bwd(**bad) < 0
+    assert step(state=None) < 0 and step(h=None) < 0
+    assert so.nof_gated_scan_marks_bytes(2, 5, 4, 3, 0) == -1 and so.nof_gated_scan_workspace_bytes(2, 5, 4, 4, 7) == -1
+    assert so.nof_gated_scan_marks_bytes(0, 5, 4, 4, 0) == 0 and so.nof_gated_scan_marks_bytes(2, 0, 4, 4, 0) == 0
+    assert so.nof_gated_scan_marks_bytes(2, 5, 4, 4, 0) == 2 * 4 * 4
