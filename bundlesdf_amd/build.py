@@ -14,7 +14,7 @@ CSRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(CSRC, 'build')
 LIB = os.path.join(HERE, 'libnof_hip.so')
 SOURCES = ['nof_capi.hip', 'nof_hash.hip', 'nof_trace.hip', 'nof_loss.hip', 'nof_adam_tail.hip', 'nof_pose.hip', 'nof_mlp.hip', 'nof_mlp_wide.hip', 'nof_mesh.hip', 'nof_texture.hip',
-           'nof_embed.hip', 'nof_scan.hip']
+           'nof_embed.hip', 'nof_scan.hip', 'nof_ortho.hip']
 HEADERS = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.h')) + [os.path.join(HERE, '..', 'include', 'nof_hip.h')]
 FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=off', '-munsafe-fp-atomics',
          '-Wno-unused-result', '-Wno-pass-failed', '-fno-slp-vectorize']
@@ -31,7 +31,8 @@ FLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-ffp-contract=o
 # first); the file has no NaN-dependent logic.
 # The learning operators are built without packed-fp32 instructions altogether (hipcc's host pass warns that it does not know the feature).
 NO_PACKED = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
-EXTRA = {'nof_mlp.hip': ['-fno-honor-nans'], 'nof_mlp_wide.hip': ['-fno-honor-nans'], 'nof_embed.hip': NO_PACKED, 'nof_scan.hip': NO_PACKED}
+EXTRA = {'nof_mlp.hip': ['-fno-honor-nans'], 'nof_mlp_wide.hip': ['-fno-honor-nans'], 'nof_embed.hip': NO_PACKED, 'nof_scan.hip': NO_PACKED,
+         'nof_ortho.hip': NO_PACKED}
 
 
 def hipcc():

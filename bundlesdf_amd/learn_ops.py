@@ -11,6 +11,9 @@ device, without a host synchronisation: every one can be captured into a graph. 
 and norms are float32 or wider and a result is rounded to its type once.  They record no autograd history -- a tensor that would need it
 is refused -- and they raise lib.NofError on anything they do not take; there is no fallback.
 """
+import ctypes as C
+import functools
+
 import torch
 
 from . import lib
@@ -219,3 +222,38 @@ def gated_scan_step(gate, value, state, new_state=None):
     _call(dev, 'nof_gated_scan_step', gate.data_ptr(), *_scan_strides(gate), _TYPE[gate.dtype], value.data_ptr(), *_scan_strides(value),
           _TYPE[value.dtype], state, new_state, h, B, D, G)
     return h, new_state
+
+
+# ---- the orthogonalised update --------------------------------------------------------------------------------------------------------
+QUINTIC = (3.4445, -4.7750, 2.0315)     # steep at 0 (a small singular value grows 3.4 times a step), within about [0.7, 1.2] from there on
+
+
+@functools.lru_cache(maxsize=64)
+def _coefficients(steps, coefficients):
+    flat = coefficients if isinstance(coefficients[0], (tuple, list)) else (coefficients,) * steps
+    _need(1 <= steps <= 32, 'orthogonalize: steps must be in [1, 32]')
+    _need(len(flat) == steps and all(len(c) == 3 for c in flat), 'orthogonalize: coefficients must be (a, b, c) or one such triple per step')
+    return (C.c_float * (3 * steps))(*[float(x) for c in flat for x in c])
+
+
+def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-30, out=None):
+    """The orthogonalised form of weight updates [..., m, n]: X = update / max(|update|_F, eps), then `steps` times
+    X <- (a + b A + c A A) X, A = X X^T (over the shorter side), with coefficients (a, b, c) -- one triple, or a tuple of `steps` of them.
+    The singular vectors stay, the singular values go to the quintic's fixed band around 1.  Result in the update's type, in `out` (which
+    may be `update`) where given.  Coefficients that let a singular value leave [0, 2] are refused."""
+    _need(update.dim() >= 2 and update.dtype in _TYPE, 'orthogonalize: update must be [..., m, n] float32, bfloat16 or float16')
+    m, n = update.shape[-2:]
+    _need(m <= 16384 and n <= 16384, 'orthogonalize: m and n must be at most 16384')
+    batch = update.shape[:-2].numel()
+    _need(batch < 65536, 'orthogonalize: at most 65535 matrices')
+    coef = _coefficients(int(steps), tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients))
+    _need(out is None or (out.shape == update.shape and out.dtype == update.dtype and out.is_contiguous()),
+          "orthogonalize: out must be contiguous, of update's shape and type")
+    dev = _on_device('orthogonalize', update, out)
+    update = update.contiguous()
+    if out is None:
+        out = torch.empty(update.shape, dtype=update.dtype, device=dev)
+    nbytes = lib.load().nof_orthogonalize_workspace_bytes(batch, m, n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _call(dev, 'nof_orthogonalize', update, out, _TYPE[update.dtype], int(steps), coef, float(eps), ws, nbytes, batch, m, n)
+    return out

@@ -181,6 +181,8 @@ _SIGNATURES = {
     'nof_gated_scan_bwd': ([_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _P, _I32, _P, _P, _P, _P, _I64, _I64, _I64, _I32,
                             _I32, _P], C.c_int),
     'nof_gated_scan_step': ([_P, _I64, _I32, _P, _I64, _I32, _P, _P, _P, _I64, _I32, _I32, _P], C.c_int),
+    'nof_orthogonalize_workspace_bytes': ([_I64, _I64, _I64], C.c_int64),
+    'nof_orthogonalize': ([_P, _P, _I32, _I32, C.POINTER(C.c_float), _F, _P, _I64, _I64, _I64, _I64, _P], C.c_int),
     'nof_embed_bwd': ([_P, _I64, _I32, _P, _I32, _F, _P, _P, _I64, _I64, _I64, _I32, _P], C.c_int),
 }
 OPTIONAL = set()

@@ -591,6 +591,14 @@ int nof_gated_scan_bwd(const void* gate, int64_t gate_sb, int64_t gate_st, int32
 /* one position: gate [B,G], value [B,D], state [B,D] -> new_state [B,D] (may be `state`), h [B,D] = new_state in `type` */
 int nof_gated_scan_step(const void* gate, int64_t gate_sb, int32_t gate_type, const void* value, int64_t value_sb, int32_t type,
                         const float* state, float* new_state, void* h, int64_t B, int32_t D, int32_t G, void* stream);
+/* The orthogonalised update of `batch` weight matrices [m,n]: X = update / max(|update|_F, eps) (a zero matrix: zeros), then for each of
+ * `steps` <= 32 triples (a, b, c) of h_coef: X <- (a I + b A + c A A) X with A = X X^T (X^T X for m > n) -> out [batch,m,n] in the update's
+ * type (may be `update` itself).  A singular value s becomes a s + b s^3 + c s^5; triples that take a start in [0, 1] beyond 2, or the
+ * bracket beyond 15, are refused.  Products are as exact as binary32's (fp16 operand pairs, binary32 sums), the norm is summed in 64
+ * bits; a result is accurate relative to max(|update|_F, eps) / |update|_F.  m, n <= 16384, batch < 65536. */
+int64_t nof_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n);
+int nof_orthogonalize(const void* update, void* out, int32_t type, int32_t steps, const float* h_coef, float eps, void* workspace,
+                      int64_t workspace_bytes, int64_t batch, int64_t m, int64_t n, void* stream);
 
 #ifdef __cplusplus
 }

@@ -105,3 +105,35 @@ def test_scan_entry_points_refuse():
     assert so.nof_gated_scan_marks_bytes(2, 5, 4, 3, 0) == -1 and so.nof_gated_scan_workspace_bytes(2, 5, 4, 4, 7) == -1
     assert so.nof_gated_scan_marks_bytes(0, 5, 4, 4, 0) == 0 and so.nof_gated_scan_marks_bytes(2, 0, 4, 4, 0) == 0
     assert so.nof_gated_scan_marks_bytes(2, 5, 4, 4, 0) == 2 * 4 * 4
+
+
+def test_orthogonalize_refusals():
+    u = torch.zeros(4, 6)
+    assert 'GPU' in refused(L.orthogonalize, u)
+    assert 'm, n' in refused(L.orthogonalize, u[0])
+    assert 'm, n' in refused(L.orthogonalize, u.double())
+    assert '16384' in refused(L.orthogonalize, torch.zeros(1, 1).expand(16385, 1))
+    assert '65535' in refused(L.orthogonalize, torch.zeros(1, 1, 1).expand(65536, 1, 1))
+    assert 'steps' in refused(L.orthogonalize, u, steps=0)
+    assert 'steps' in refused(L.orthogonalize, u, steps=33)
+    assert 'triple' in refused(L.orthogonalize, u, coefficients=(1.0, 2.0))
+    assert 'triple' in refused(L.orthogonalize, u, steps=3, coefficients=((1.5, -0.5, 0.0),) * 2)
+    assert 'out' in refused(L.orthogonalize, u, out=torch.zeros(6, 4))
+    assert 'out' in refused(L.orthogonalize, u, out=torch.zeros(6, 4).t())
+
+
+def test_orthogonalize_entry_point_refuses():
+    so = lib.load()
+    quintic = (C.c_float * 15)(*L.QUINTIC * 5)
+
+    def call(type=0, steps=5, coef=quintic, eps=1e-30, ws=None, size=0, batch=2, m=4, n=6, u=PTR, out=PTR):
+        return so.nof_orthogonalize(u, out, type, steps, coef, eps, ws, size, batch, m, n, None)
+
+    for bad in ({'type': 3}, {'steps': 0}, {'steps': 33}, {'coef': None}, {'eps': -1.0}, {'eps': float('nan')}, {'batch': -1}, {'batch': 65536},
+                {'m': 16385}, {'n': -1}, {'u': None}, {'out': None}, {'m': 200}, {'m': 200, 'ws': PTR, 'size': 8}, {'m': 200, 'ws': C.c_void_p(8), 'size': 1 << 30},
+                {'steps': 1, 'coef': (C.c_float * 3)(2.5, 0.0, 0.0)}, {'steps': 1, 'coef': (C.c_float * 3)(float('nan'), 0.0, 0.0)},
+                {'steps': 2, 'coef': (C.c_float * 6)(1.9, 0.0, 0.0, 1.9, 0.0, 0.0)}, {'steps': 1, 'coef': (C.c_float * 3)(-16.0, 0.0, 15.0)}):
+        assert call(**bad) < 0 and b'argument check' in so.nof_last_error(), bad
+    assert call(batch=0) == 0 and call(m=0) == 0 and call(n=0) == 0
+    assert so.nof_orthogonalize_workspace_bytes(1, 16385, 4) == -1 and so.nof_orthogonalize_workspace_bytes(1, 128, 128) == 0
+    assert so.nof_orthogonalize_workspace_bytes(3, 129, 20) > 3 * 4 * 256 * 256
