@@ -16,12 +16,11 @@
 // rows along the summed index, so X is stored in both orientations.
 #include "nof_learn_dev.h"
 #include "nof_mfma_dev.h"
+#include <type_traits>
 
 #define ORT_SCALE 4096.0f               // operands hold 4096 times their value: |P| <= 15, |X| <= 2 stay below 65504
-#define ORT_TILE 128
-#define ORT_KSTEP 32
 #define ORT_SMALL 128
-#define ORT_NORM_BLOCKS 64
+#define ORT_NORM_BLOCKS 512             // at most
 #define ORT_MAX_STEPS 32
 
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -160,61 +159,75 @@ __global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restric
 
 // ---- larger matrices --------------------------------------------------------------------------------------------------------------
 // images of one matrix, in halves: X [rp][kp], X^T [kp][rp] twice (the last product reads one while it writes the other), A and P
-// [rp][rp]; each image is a hi plane followed by its lo plane.  rp, kp: r and k up to whole tiles, zeros in between.
+// [rp][rp].  32 hi of a row lie next to their 32 lo, a cache line that one stage of a product reads whole (as planes, lines of which a
+// stage read half, L2 held the products at 10 TB/s of useful and as much useless traffic); an image that is read for hi alone is a hi plane.
+// rp, kp: r and k up to whole tiles, zeros in between.
 struct OrtArgs {
   _Float16* ws; size_t per;             // halves per matrix
-  int r, k, rp, kp, m, n, tall, nt;     // nt = rp / ORT_TILE
+  int r, k, rp, kp, m, n, tall;
   float ca, cb, cc;
   int cur;                              // which X^T holds X
+  int tiles;                            // of a matrix in this launch
+  int flat;                             // this launch's P or X^T is read for hi alone
 };
 __device__ __forceinline__ _Float16* ort_x(const OrtArgs& p, int b) { return p.ws + b * p.per; }
 __device__ __forceinline__ _Float16* ort_xt(const OrtArgs& p, int b, int which) { return p.ws + b * p.per + (size_t)(1 + which) * 2 * p.rp * p.kp; }
 __device__ __forceinline__ _Float16* ort_a(const OrtArgs& p, int b) { return p.ws + b * p.per + (size_t)6 * p.rp * p.kp; }
 __device__ __forceinline__ _Float16* ort_p(const OrtArgs& p, int b) { return p.ws + b * p.per + (size_t)6 * p.rp * p.kp + (size_t)2 * p.rp * p.rp; }
 
-template <typename T>
+// partial sums of squares, one per workgroup; V elements (16 bytes) per access where every matrix starts on a 16-byte border
+template <typename T, int V>
 __global__ __launch_bounds__(256) void k_ortho_norm(const T* __restrict__ g, int64_t count, double* __restrict__ part) {
   __shared__ double red[4];
   g += (size_t)blockIdx.y * count;
-  double s = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)ORT_NORM_BLOCKS * 256) {
-    const double x = (double)lf(g[i]);
-    s += x * x;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  const int64_t step = (int64_t)gridDim.x * 256 * V;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < count; i += step) {
+    float f[V];
+    lload<T, V>(g + i, f);
+#pragma unroll
+    for (int q = 0; q < V; ++q) s[q & 3] += (double)f[q] * (double)f[q];
   }
-  s = ort_block_sum(s, red);
-  if (threadIdx.x == 0) part[blockIdx.y * ORT_NORM_BLOCKS + blockIdx.x] = s;
+  const double t = ort_block_sum((s[0] + s[1]) + (s[2] + s[3]), red);
+  if (threadIdx.x == 0) part[blockIdx.y * gridDim.x + blockIdx.x] = t;
 }
+
+// where column `col` (of `ld`) of row `row` has its hi; its lo is 32 halves on
+__device__ __forceinline__ size_t ort_at(int row, int col, int ld) { return (size_t)row * 2 * ld + (col >> 5) * 64 + (col & 31); }
 
 // X and X^T of 4096 G / norm, tiles of 64 x 64 turned through LDS
 template <typename T>
-__global__ __launch_bounds__(256) void k_ortho_split(const T* __restrict__ g, const double* __restrict__ part, OrtArgs p, float eps) {
+__global__ __launch_bounds__(256) void k_ortho_split(const T* __restrict__ g, const double* __restrict__ part, int n_part, OrtArgs p, float eps) {
+  __shared__ double red[4];
   __shared__ float tile[64][65];
   const int b = blockIdx.z;
   double s = 0.0;
-  for (int q = 0; q < ORT_NORM_BLOCKS; ++q) s += part[b * ORT_NORM_BLOCKS + q];
-  const double f = ort_factor(s, eps);
+  for (int q = threadIdx.x; q < n_part; q += 256) s += part[b * n_part + q];
+  const double f = ort_factor(ort_block_sum(s, red), eps);
   g += (size_t)b * p.m * p.n;
   const int rows = p.tall ? p.kp : p.rp, cols = p.tall ? p.rp : p.kp;  // of G's own orientation, padded
   const int y0 = blockIdx.y * 64, x0 = blockIdx.x * 64;
   _Float16* along = p.tall ? ort_xt(p, b, p.cur) : ort_x(p, b);        // [rows][cols]
   _Float16* turned = p.tall ? ort_x(p, b) : ort_xt(p, b, p.cur);       // [cols][rows]
-  const size_t plane = (size_t)p.rp * p.kp;
   const int c = threadIdx.x & 63;
+  const bool flat_a = p.flat && p.tall, flat_t = p.flat && !p.tall;   // X^T for a single step of hi alone
   for (int y = threadIdx.x >> 6; y < 64; y += 4) {
     const int gy = y0 + y, gx = x0 + c;
     const float v = gy < p.m && gx < p.n ? (float)((double)lf(g[(size_t)gy * p.n + gx]) * f) : 0.0f;
     tile[y][c] = v;
     _Float16 h, l;
     ort_split(v, h, l);
-    along[(size_t)gy * cols + gx] = h;
-    along[plane + (size_t)gy * cols + gx] = l;
+    const size_t at = flat_a ? (size_t)gy * cols + gx : ort_at(gy, gx, cols);
+    along[at] = h;
+    if (!flat_a) along[at + 32] = l;
   }
   __syncthreads();
   for (int y = threadIdx.x >> 6; y < 64; y += 4) {
     _Float16 h, l;
     ort_split(tile[c][y], h, l);
-    turned[(size_t)(x0 + y) * rows + y0 + c] = h;
-    turned[plane + (size_t)(x0 + y) * rows + y0 + c] = l;
+    const size_t at = flat_t ? (size_t)(x0 + y) * rows + y0 + c : ort_at(x0 + y, y0 + c, rows);
+    turned[at] = h;
+    if (!flat_t) turned[at + 32] = l;
   }
 }
 
@@ -223,122 +236,266 @@ __global__ __launch_bounds__(256) void k_ortho_split(const T* __restrict__ g, co
 #define ORT_APPLY 2
 #define ORT_LAST 3
 
-// 16-byte piece c of row `row` of a staged tile sits at piece c ^ ort_swizzle(row): a fragment's reads (one piece of 32 consecutive rows)
-// then touch every bank equally
-__device__ __forceinline__ int ort_swizzle(int row) { return ((row >> 1) & 3) ^ ((row >> 3) & 1); }
+// A stage is 64 halves of every row: 32 of the summed index as hi and lo, or 64 of it as hi alone.  16-byte piece c of row `row`
+// sits at piece c ^ ort_swizzle(row): a fragment's reads (one piece of 32 consecutive rows) then touch every bank equally, for eight lanes
+// of 128 bytes and for sixteen of 256
+__device__ __forceinline__ int ort_swizzle(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
-// C = L R^T in tiles of 128 x 128, four waves of 64 x 64, ORT_KSTEP of the summed index per stage, two stages in LDS filled by direct loads
-template <int MODE, typename T>
-__global__ __launch_bounds__(256, 2) void k_ortho_gemm(OrtArgs p, T* __restrict__ out) {
-  __shared__ __attribute__((aligned(16))) _Float16 lds[2][4][ORT_TILE * ORT_KSTEP];
-  const int b = blockIdx.z, lane = threadIdx.x & 63, w = threadIdx.x >> 6, hi = lane >> 5, l31 = lane & 31;
-  int bi, bj;
+// C = L R^T.  A workgroup is WM x WN waves of TI x TJ tiles of 32 x 32; a stage is 64 halves of every row, NS stages a ring in
+// LDS that direct loads fill NS - 1 stages ahead, one barrier a stage.  PAIRS: operands are hi + lo (three products), else hi alone: what the last
+// product of a bfloat16 result takes, off by at most 2^-10 of it beside the rounding's 2^-8 (in any other product, an error of hi alone would
+// be amplified by the steps that follow: up to 1 % for a multiple of the identity).
+// KG groups of such waves take the stages in turn, so that few tiles still give every SIMD several waves; their sums meet in LDS.
+template <int WM, int WN, int TI, int TJ, int NS, int KG> struct OrtShape {
+  static constexpr int wm = WM, wn = WN, ti = TI, tj = TJ, ns = NS, kg = KG, M = WM * TI * 32, N = WN * TJ * 32, group = WM * WN * 64, threads = group * KG;
+  static constexpr int stage = 64 * (M + N), loads = stage / 8 / group;                            // halves of a stage; 16-byte pieces of it per thread
+};
+// counted wait for this thread's direct loads, its LDS reads done
+template <int N> __device__ __forceinline__ void ort_wait() { __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070); }
+
+// a wave's LDS writes are seen by its other lanes' reads behind this (LDS operations of a wave complete in order; this holds the compiler)
+__device__ __forceinline__ void ort_wave_sync() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_wave_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int MODE, typename T, typename S, bool PAIRS>
+__global__ __launch_bounds__(S::threads, S::ns * S::kg * S::stage <= 40960 ? 2 * S::kg : S::kg) void k_ortho_gemm(OrtArgs p, T* __restrict__ out) {
+  __shared__ __attribute__((aligned(16))) _Float16 lds[S::ns * S::kg * S::stage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, l31 = lane & 31;
+  const int w = wave % (S::group / 64), kg = wave / (S::group / 64), tid = threadIdx.x % S::group;
+  // Workgroups go round the eight XCDs: each takes a stretch of neighbouring tiles, whose operands its L2 then holds once
+  const int total = gridDim.x, each = total / 8, more = total % 8, xcd = blockIdx.x % 8;
+  int t = xcd * each + (xcd < more ? xcd : more) + blockIdx.x / 8, bi, bj;
+  const int b = t / p.tiles;
+  t -= b * p.tiles;
+  // within it, blocks of 8 x 8 tiles
+  const int nt = p.rp / S::M;
   if (MODE == ORT_GRAM || MODE == ORT_POLY) {                         // tiles on and above the diagonal
-    int t = blockIdx.x;
-    bi = 0;
-    while (t >= p.nt - bi) { t -= p.nt - bi; ++bi; }
-    bj = bi + t;
+    int bI = 0, bJ = 0;
+    for (;;) {
+      const int h = nt - 8 * bI < 8 ? nt - 8 * bI : 8, v = nt - 8 * bJ < 8 ? nt - 8 * bJ : 8, n = bI == bJ ? h * (h + 1) / 2 : h * v;
+      if (t < n) {
+        if (bI == bJ) {
+          bi = 0;
+          while (t >= h - bi) { t -= h - bi; ++bi; }
+          bj = 8 * bJ + bi + t;
+          bi += 8 * bI;
+        } else {
+          bi = 8 * bI + t % h;
+          bj = 8 * bJ + t / h;
+        }
+        break;
+      }
+      t -= n;
+      if (8 * ++bJ >= nt) bJ = ++bI;
+    }
   } else {
-    bi = blockIdx.x % p.nt;
-    bj = blockIdx.x / p.nt;
+    const int mt = p.kp / S::N, panel = t / (8 * mt), h = nt - 8 * panel < 8 ? nt - 8 * panel : 8;
+    t -= panel * 8 * mt;
+    bi = 8 * panel + t % h;
+    bj = t / h;
   }
   const _Float16 *L, *R;
-  size_t planeL, planeR;
   int K;
-  if (MODE == ORT_GRAM) { L = R = ort_x(p, b); planeL = planeR = (size_t)p.rp * p.kp; K = p.kp; }
-  else if (MODE == ORT_POLY) { L = R = ort_a(p, b); planeL = planeR = (size_t)p.rp * p.rp; K = p.rp; }
-  else { L = ort_p(p, b); planeL = (size_t)p.rp * p.rp; R = ort_xt(p, b, p.cur); planeR = (size_t)p.rp * p.kp; K = p.rp; }
-  L += (size_t)bi * ORT_TILE * K;
-  R += (size_t)bj * ORT_TILE * K;
-  auto load = [&](int stage, int k0) {
+  if (MODE == ORT_GRAM) { L = R = ort_x(p, b); K = p.kp; }
+  else if (MODE == ORT_POLY) { L = R = ort_a(p, b); K = p.rp; }
+  else { L = ort_p(p, b); R = ort_xt(p, b, p.cur); K = p.rp; }
+  constexpr int kstep = PAIRS ? 32 : 64;
+  const size_t pitch = PAIRS ? 2 * (size_t)K : (size_t)K;
+  // where this thread's pieces of a stage come from: L's rows, then R's
+  const _Float16* src[S::loads];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {                                     // 2048 pieces of 16 bytes, 256 a turn
-      const int plane = q >> 1, base = (q & 1) * 256 + w * 64, piece = base + lane, row = piece >> 2, c = (piece & 3) ^ ort_swizzle(row);
-      const _Float16* src = (plane < 2 ? L + (plane & 1) * planeL : R + (plane & 1) * planeR) + (size_t)row * K + k0 + c * 8;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                       (__attribute__((address_space(3))) void*)(&lds[stage][plane][base * 8]), 16, 0, 0);
+  for (int q = 0; q < S::loads; ++q) {
+    const bool left = q * S::group < 8 * S::M;                        // (a turn of the group lies within one of the two)
+    const int piece = q * S::group + tid - (left ? 0 : 8 * S::M), row = piece / 8, c = (piece % 8) ^ ort_swizzle(row);
+    src[q] = (left ? L + (size_t)(bi * S::M + row) * pitch : R + (size_t)(bj * S::N + row) * pitch) + kg * 64 + c * 8;
+  }
+  auto load = [&](int slot) {
+#pragma unroll
+    for (int q = 0; q < S::loads; ++q) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[q],
+                                       (__attribute__((address_space(3))) void*)(lds + (slot * S::kg + kg) * S::stage + (q * S::group + w * 64) * 8), 16, 0, 0);
+      src[q] += S::kg * 64;
     }
   };
-  f32x16 acc[2][2] = {};
-  const int wi = (w >> 1) * 64, wj = (w & 1) * 64;
-  load(0, 0);
-  __builtin_amdgcn_s_waitcnt(0x0f70);                                 // vmcnt(0): the stage is in LDS
-  __syncthreads();
-  for (int k0 = 0, s = 0; k0 < K; k0 += ORT_KSTEP, s ^= 1) {
-    if (k0 + ORT_KSTEP < K) load(s ^ 1, k0 + ORT_KSTEP);
+  f32x16 acc[S::ti][S::tj] = {};
+  const int wi = (w / S::wn) * S::ti * 32, wj = (w % S::wn) * S::tj * 32, rounds = (K / kstep + S::kg - 1) / S::kg, stages = (K / kstep - kg + S::kg - 1) / S::kg;      // this group's stages
 #pragma unroll
-    for (int kk = 0; kk < ORT_KSTEP / 16; ++kk) {
-      f16x8 f[4][2];
+  for (int q = 0; q < S::ns - 1; ++q)
+    if (q < stages) load(q);
+  int slot = 0, fill = S::ns - 1;
+  for (int it = 0; it < rounds; ++it) {
+    if (it + S::ns - 2 < stages) ort_wait<(S::ns - 2) * S::loads>(); else ort_wait<0>();      // stage `it` has landed (this wave's part)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();                                     // ... everybody's; and everybody has read the stage before
+    asm volatile("" ::: "memory");
+    if (it + S::ns - 1 < stages) load(fill);
+    const _Float16* st = lds + (slot * S::kg + kg) * S::stage;
+    if (it < stages) {
+    f16x8 lh[kstep / 16][S::ti], ll[kstep / 16][S::ti], rh[kstep / 16][S::tj], rl[kstep / 16][S::tj];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int ra = wi + 32 * t + l31, rb = wj + 32 * t + l31, c = 2 * kk + hi;
-        const int oa = ra * ORT_KSTEP + (c ^ ort_swizzle(ra)) * 8, ob = rb * ORT_KSTEP + (c ^ ort_swizzle(rb)) * 8;
-        f[0][t] = *(const f16x8*)(&lds[s][0][oa]);
-        f[1][t] = *(const f16x8*)(&lds[s][1][oa]);
-        f[2][t] = *(const f16x8*)(&lds[s][2][ob]);
-        f[3][t] = *(const f16x8*)(&lds[s][3][ob]);
+    for (int kk = 0; kk < kstep / 16; ++kk) {
+      const int c = 2 * kk + hi;
+#pragma unroll
+      for (int t = 0; t < S::ti; ++t) {
+        const int row = wi + 32 * t + l31, o = row * 64, z = ort_swizzle(row);
+        lh[kk][t] = *(const f16x8*)(st + o + (c ^ z) * 8);
+        if (PAIRS) ll[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = ort_mma3(f[0][i], f[1][i], f[2][j], f[3][j], acc[i][j]);
+      for (int t = 0; t < S::tj; ++t) {
+        const int row = wj + 32 * t + l31, o = (S::M + row) * 64, z = ort_swizzle(row);
+        rh[kk][t] = *(const f16x8*)(st + o + (c ^ z) * 8);
+        if (PAIRS) rl[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
+      }
     }
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < kstep / 16; ++kk)
+#pragma unroll
+      for (int i = 0; i < S::ti; ++i)
+#pragma unroll
+        for (int j = 0; j < S::tj; ++j)
+          acc[i][j] = PAIRS ? ort_mma3(lh[kk][i], ll[kk][i], rh[kk][j], rl[kk][j], acc[i][j]) : PrecF16::mma(lh[kk][i], rh[kk][j], acc[i][j]);
+    }
+    slot = slot + 1 == S::ns ? 0 : slot + 1;
+    fill = fill + 1 == S::ns ? 0 : fill + 1;
   }
-  const size_t planeX = (size_t)p.rp * p.kp, planeA = (size_t)p.rp * p.rp;
+  // Results leave through LDS, a band of 32 rows of the wave's tile at a time, so that global stores are 16 bytes a lane and whole rows of
+  // the tile: stored from the accumulators they were 2 bytes a lane, and 8 in the other orientation.
+  constexpr int wmax = 32 * (S::ti > S::tj ? S::ti : S::tj) + 8;
+  static_assert(S::ns * S::stage >= S::wm * S::wn * 32 * wmax && S::ns * S::stage >= S::wm * S::wn * 64 * 33, "the bands fit the ring");
+  ort_wait<0>();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();                                       // the ring is free
+  asm volatile("" ::: "memory");
+  if (S::kg > 1) {                                                    // the first group adds the others' sums, in order, and goes on alone
+    static_assert(S::ns * S::stage * S::kg >= 2 * (S::kg - 1) * S::M * S::N, "the sums fit the ring");
+    float* sums = (float*)lds;
+    if (kg > 0) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < S::ti; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int i0 = bi * ORT_TILE + wi + 32 * i, col = bj * ORT_TILE + wj + 32 * j + l31;
+        for (int j = 0; j < S::tj; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sums[(((kg - 1) * S::group / 64 + w) * S::ti * S::tj * 16 + (i * S::tj + j) * 16 + e) * 64 + lane] = acc[i][j][e];
+    }
+    __syncthreads();
+    if (kg == 0) {
+#pragma unroll
+      for (int g = 1; g < S::kg; ++g)
+#pragma unroll
+        for (int i = 0; i < S::ti; ++i)
+#pragma unroll
+          for (int j = 0; j < S::tj; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] += sums[(((g - 1) * S::group / 64 + w) * S::ti * S::tj * 16 + (i * S::tj + j) * 16 + e) * 64 + lane];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+  }
+  const int i0 = bi * S::M + wi, j0 = bj * S::N + wj;
+  if (MODE == ORT_LAST) {
+    T* o = out + (size_t)b * p.m * p.n;
+    float* band = (float*)lds + w * 32 * 33;
+#pragma unroll
+    for (int i = 0; i < S::ti; ++i)
+#pragma unroll
+      for (int j = 0; j < S::tj; ++j) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float v = acc[i][j][e] * (1.0f / (ORT_SCALE * ORT_SCALE));
+          if (p.tall) band[l31 * 33 + nloc(hi, e)] = v;
+          else if (i0 + 32 * i + nloc(hi, e) < p.r && j0 + 32 * j + l31 < p.k) o[(size_t)(i0 + 32 * i + nloc(hi, e)) * p.n + j0 + 32 * j + l31] = lt<T>(v);
+        }
+        if (p.tall) {
+          ort_wave_sync();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int y = 2 * e + hi;
+            if (j0 + 32 * j + y < p.k && i0 + 32 * i + l31 < p.r) o[(size_t)(j0 + 32 * j + y) * p.n + i0 + 32 * i + l31] = lt<T>(band[y * 33 + l31]);
+          }
+          ort_wave_sync();
+        }
+      }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < S::ti; ++i)
+#pragma unroll
+    for (int j = 0; j < S::tj; ++j) {
       f32x16& v = acc[i][j];
       if (MODE == ORT_POLY) {                                         // A is symmetric: its column piece is read along a row
-        const _Float16* a = ort_a(p, b) + (size_t)col * p.rp + i0 + 4 * hi;
+        const int col = j0 + 32 * j + l31, row0 = i0 + 32 * i + 4 * hi;
+        const _Float16* a = ort_a(p, b) + ort_at(col, i0 + 32 * i, p.rp) + 4 * hi;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const f16x4 h4 = *(const f16x4*)(a + 8 * q), l4 = *(const f16x4*)(a + planeA + 8 * q);
+          const f16x4 h4 = *(const f16x4*)(a + 8 * q), l4 = *(const f16x4*)(a + 32 + 8 * q);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            v[4 * q + e] = (i0 + 8 * q + 4 * hi + e == col ? p.ca * ORT_SCALE : 0.0f) + p.cb * ((float)h4[e] + (float)l4[e]) +
+            v[4 * q + e] = (row0 + 8 * q + e == col ? p.ca * ORT_SCALE : 0.0f) + p.cb * ((float)h4[e] + (float)l4[e]) +
                            p.cc * (v[4 * q + e] * (1.0f / ORT_SCALE));
         }
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] *= 1.0f / ORT_SCALE;
       }
-      if (MODE == ORT_LAST) {
-        T* o = out + (size_t)b * p.m * p.n;
+    }
+  _Float16* c = MODE == ORT_GRAM ? ort_a(p, b) : MODE == ORT_POLY ? ort_p(p, b) : ort_x(p, b);
+  _Float16* ct = MODE == ORT_APPLY ? ort_xt(p, b, p.cur ^ 1) : c;
+  const int ld = MODE == ORT_APPLY ? p.kp : p.rp;
+  _Float16* band = lds + w * 32 * wmax;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int row = i0 + nloc(hi, e);
-          if (row < p.r && col < p.k) o[p.tall ? (size_t)col * p.n + row : (size_t)row * p.n + col] = lt<T>(v[e] * (1.0f / ORT_SCALE));
+  for (int half = 0; half < 2; ++half) {
+    if (MODE == ORT_POLY && p.flat && half) break;
+    if (MODE == ORT_APPLY || bi != bj) {                              // as computed; a tile on the diagonal is its own mirror image
+#pragma unroll
+      for (int i = 0; i < S::ti; ++i) {
+#pragma unroll
+        for (int j = 0; j < S::tj; ++j)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            _Float16 h, l;
+            ort_split(acc[i][j][e], h, l);
+            band[nloc(hi, e) * wmax + 32 * j + l31] = half ? l : h;
+          }
+        ort_wave_sync();
+#pragma unroll
+        for (int q = 0; q < 2 * S::tj; ++q) {
+          const int piece = q * 64 + lane, row = piece / (4 * S::tj), at = piece % (4 * S::tj) * 8;
+          const size_t to = MODE == ORT_POLY && p.flat ? (size_t)(i0 + 32 * i + row) * ld + j0 + at : ort_at(i0 + 32 * i + row, j0 + at, ld) + 32 * half;
+          *(f16x8*)(c + to) = *(const f16x8*)(band + row * wmax + at);
         }
-      } else {
-        _Float16* c = MODE == ORT_GRAM ? ort_a(p, b) : MODE == ORT_POLY ? ort_p(p, b) : ort_x(p, b);
-        _Float16* ct = MODE == ORT_APPLY ? ort_xt(p, b, p.cur ^ 1) : c;
-        const size_t plane = MODE == ORT_APPLY ? planeX : planeA;
-        const int ld = MODE == ORT_APPLY ? p.kp : p.rp;
+        ort_wave_sync();
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < S::tj; ++j) {                                 // and turned
+      if (p.flat && half) break;
+#pragma unroll
+      for (int i = 0; i < S::ti; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          f16x4 h4, l4;
+          f16x4 x;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             _Float16 h, l;
-            ort_split(v[4 * q + e], h, l);
-            h4[e] = h; l4[e] = l;
-            if (MODE == ORT_APPLY || bi != bj) {
-              const size_t at = (size_t)(i0 + 8 * q + 4 * hi + e) * ld + col;
-              c[at] = h;
-              c[plane + at] = l;
-            }
+            ort_split(acc[i][j][4 * q + e], h, l);
+            x[e] = half ? l : h;
           }
-          const size_t at = (size_t)col * p.rp + i0 + 8 * q + 4 * hi;
-          *(f16x4*)(ct + at) = h4;
-          *(f16x4*)(ct + plane + at) = l4;
+          *(f16x4*)(band + l31 * wmax + 32 * i + 8 * q + 4 * hi) = x;
         }
+      ort_wave_sync();
+#pragma unroll
+      for (int q = 0; q < 2 * S::ti; ++q) {
+        const int piece = q * 64 + lane, row = piece / (4 * S::ti), at = piece % (4 * S::ti) * 8;
+        const size_t to = p.flat ? (size_t)(j0 + 32 * j + row) * p.rp + i0 + at : ort_at(j0 + 32 * j + row, i0 + at, p.rp) + 32 * half;
+        *(f16x8*)(ct + to) = *(const f16x8*)(band + row * wmax + at);
       }
+      ort_wave_sync();
     }
+  }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
@@ -346,12 +503,28 @@ static bool ort_sizes_ok(int64_t batch, int64_t m, int64_t n) {
   return batch >= 0 && batch < 65536 && m >= 0 && m <= 16384 && n >= 0 && n <= 16384;
 }
 static bool ort_is_small(int64_t m, int64_t n) { return m <= ORT_SMALL && n <= ORT_SMALL; }
-static int64_t ort_up(int64_t x) { return nof_div_up(x, ORT_TILE) * ORT_TILE; }
+// The tile of a product: 128 x 128 where that gives a workgroup per compute unit, else 64 x 64.  Images are padded to whole tiles.
+#ifndef ORT_ND
+#define ORT_ND 2, 4
+#endif
+#ifndef ORT_N
+#define ORT_N 2, 2
+#endif
+#ifndef ORT_WD
+#define ORT_WD 2, 2
+#endif
+typedef OrtShape<2, 2, 2, 2, 2, 1> OrtWide;
+typedef OrtShape<2, 2, 2, 2, ORT_WD> OrtWideDeep;                      // one workgroup per compute unit at most: all of LDS is its ring
+typedef OrtShape<2, 2, 1, 1, ORT_N> OrtNarrow;
+typedef OrtShape<2, 2, 1, 1, ORT_ND> OrtNarrowDeep;
+static bool ort_wide(int64_t tiles_of_128) { return tiles_of_128 >= 256; }
+static int64_t ort_up(int64_t x, int64_t unit) { return nof_div_up(x, unit) * unit; }
+static int64_t ort_unit(int64_t batch, int64_t r, int64_t k) { return ort_wide(batch * nof_div_up(r, 128) * nof_div_up(k, 128)) ? 128 : 64; }
 
 extern "C" int64_t nof_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n) {
   if (!ort_sizes_ok(batch, m, n)) return -1;
   if (batch == 0 || m == 0 || n == 0 || ort_is_small(m, n)) return 0;
-  const int64_t rp = ort_up(m < n ? m : n), kp = ort_up(m < n ? n : m);
+  const int64_t r = m < n ? m : n, k = m < n ? n : m, unit = ort_unit(batch, r, k), rp = ort_up(r, unit), kp = ort_up(k, unit);
   return learn_align(batch * ORT_NORM_BLOCKS * 8) + batch * (6 * rp * kp + 4 * rp * rp) * 2;
 }
 
@@ -363,6 +536,24 @@ static void ort_launch_small(const void* g, void* out, int64_t batch, int64_t m,
   constexpr size_t lds = (size_t)4 * 2 * 32 * KT * (32 * KT + 8);    // 136 KiB for KT = 4
   if (lds > 64 << 10) (void)hipFuncSetAttribute((const void*)&k_ortho_small<T, KT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   hipLaunchKernelGGL((k_ortho_small<T, KT>), dim3((unsigned)batch), dim3(64 * rt * KT), lds, st, (const T*)g, (T*)out, (int)m, (int)n, steps, c, eps);
+}
+
+template <int MODE, typename S> static int64_t ort_tiles(const OrtArgs& p) {
+  const int64_t ni = p.rp / S::M, nj = p.kp / S::N;
+  return MODE == ORT_GRAM || MODE == ORT_POLY ? ni * (ni + 1) / 2 : ni * nj;
+}
+template <int MODE, typename T, typename S, bool PAIRS>
+static void ort_gemm(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
+  p.tiles = (int)ort_tiles<MODE, S>(p);
+  hipLaunchKernelGGL((k_ortho_gemm<MODE, T, S, PAIRS>), dim3((unsigned)(p.tiles * batch)), dim3(S::threads), 0, st, p, out);
+}
+template <int MODE, typename T, bool PAIRS>
+static void ort_product(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
+  const int64_t wide = p.rp % 128 == 0 && p.kp % 128 == 0 ? batch * ort_tiles<MODE, OrtWide>(p) : 0;
+  if (wide > 256) ort_gemm<MODE, T, OrtWide, PAIRS>(p, out, batch, st);
+  else if (ort_wide(wide)) ort_gemm<MODE, T, OrtWideDeep, PAIRS>(p, out, batch, st);
+  else if (batch * ort_tiles<MODE, OrtNarrow>(p) > 256) ort_gemm<MODE, T, OrtNarrow, PAIRS>(p, out, batch, st);
+  else ort_gemm<MODE, T, OrtNarrowDeep, PAIRS>(p, out, batch, st);
 }
 
 template <typename T>
@@ -377,23 +568,33 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
     else ort_launch_small<T, 4>(g, out, batch, m, n, steps, coef, eps, st);
     return;
   }
+  const int64_t unit = ort_unit(batch, r, k);
   OrtArgs p = {};
-  p.r = (int)r; p.k = (int)k; p.rp = (int)ort_up(r); p.kp = (int)ort_up(k);
+  p.r = (int)r; p.k = (int)k; p.rp = (int)ort_up(r, unit); p.kp = (int)ort_up(k, unit);
   p.m = (int)m; p.n = (int)n; p.tall = m > n;
-  p.nt = p.rp / ORT_TILE;
   p.per = (size_t)6 * p.rp * p.kp + (size_t)4 * p.rp * p.rp;
+  constexpr bool light = std::is_same<T, __bf16>::value;             // the last product of hi alone (k_ortho_gemm)
+  p.flat = light && steps == 1;
   double* part = (double*)workspace;
   p.ws = (_Float16*)((char*)workspace + learn_align(batch * ORT_NORM_BLOCKS * 8));
-  const unsigned nb = (unsigned)batch, sym = (unsigned)(p.nt * (p.nt + 1) / 2), full = (unsigned)(p.nt * (p.kp / ORT_TILE));
-  hipLaunchKernelGGL(k_ortho_norm<T>, dim3(ORT_NORM_BLOCKS, nb), dim3(256), 0, st, (const T*)g, m * n, part);
+  const unsigned nb = (unsigned)batch;
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool wide = ((uintptr_t)g & 15) == 0 && m * n % V == 0;
+  const int64_t want = nof_div_up(m * n, 256 * 8 * 4);
+  const int n_part = (int)(want < ORT_NORM_BLOCKS ? want : ORT_NORM_BLOCKS);
+  if (wide) hipLaunchKernelGGL((k_ortho_norm<T, V>), dim3(n_part, nb), dim3(256), 0, st, (const T*)g, m * n, part);
+  else hipLaunchKernelGGL((k_ortho_norm<T, 1>), dim3(n_part, nb), dim3(256), 0, st, (const T*)g, m * n, part);
   hipLaunchKernelGGL(k_ortho_split<T>, dim3((p.tall ? p.rp : p.kp) / 64, (p.tall ? p.kp : p.rp) / 64, nb), dim3(256), 0, st, (const T*)g,
-                     (const double*)part, p, eps);
+                     (const double*)part, n_part, p, eps);
   for (int s = 0; s < steps; ++s, p.cur ^= 1) {
     p.ca = coef[3 * s]; p.cb = coef[3 * s + 1]; p.cc = coef[3 * s + 2];
-    hipLaunchKernelGGL((k_ortho_gemm<ORT_GRAM, float>), dim3(sym, 1, nb), dim3(256), 0, st, p, (float*)nullptr);
-    hipLaunchKernelGGL((k_ortho_gemm<ORT_POLY, float>), dim3(sym, 1, nb), dim3(256), 0, st, p, (float*)nullptr);
-    if (s + 1 < steps) hipLaunchKernelGGL((k_ortho_gemm<ORT_APPLY, float>), dim3(full, 1, nb), dim3(256), 0, st, p, (float*)nullptr);
-    else hipLaunchKernelGGL((k_ortho_gemm<ORT_LAST, T>), dim3(full, 1, nb), dim3(256), 0, st, p, (T*)out);
+    p.flat = 0;
+    ort_product<ORT_GRAM, float, true>(p, nullptr, batch, st);
+    p.flat = light && s + 1 == steps;
+    ort_product<ORT_POLY, float, true>(p, nullptr, batch, st);
+    p.flat = light && s + 2 == steps;
+    if (s + 1 < steps) ort_product<ORT_APPLY, float, true>(p, nullptr, batch, st);
+    else ort_product<ORT_LAST, T, !light>(p, (T*)out, batch, st);
   }
 }
 
