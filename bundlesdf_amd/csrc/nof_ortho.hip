@@ -261,7 +261,7 @@ __device__ __forceinline__ void ort_wave_sync() {
 }
 
 template <int MODE, typename T, typename S, bool PAIRS>
-__global__ __launch_bounds__(S::threads, S::ns * S::kg * S::stage <= 40960 ? 2 * S::kg : S::kg) void k_ortho_gemm(OrtArgs p, T* __restrict__ out) {
+__global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::stage <= 40960 ? 2 : 1)) void k_ortho_gemm(OrtArgs p, T* __restrict__ out) {
   __shared__ __attribute__((aligned(16))) _Float16 lds[S::ns * S::kg * S::stage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, l31 = lane & 31;
   const int w = wave % (S::group / 64), kg = wave / (S::group / 64), tid = threadIdx.x % S::group;
@@ -334,30 +334,34 @@ __global__ __launch_bounds__(S::threads, S::ns * S::kg * S::stage <= 40960 ? 2 *
     if (it + S::ns - 1 < stages) load(fill);
     const _Float16* st = lds + (slot * S::kg + kg) * S::stage;
     if (it < stages) {
-    f16x8 lh[kstep / 16][S::ti], ll[kstep / 16][S::ti], rh[kstep / 16][S::tj], rl[kstep / 16][S::tj];
+    constexpr int ahead = S::ti * S::tj > 4 ? 1 : kstep / 16;        // sixteens of the summed index whose fragments are read at once
 #pragma unroll
-    for (int kk = 0; kk < kstep / 16; ++kk) {
-      const int c = 2 * kk + hi;
+    for (int k0 = 0; k0 < kstep / 16; k0 += ahead) {
+      f16x8 lh[ahead][S::ti], ll[ahead][S::ti], rh[ahead][S::tj], rl[ahead][S::tj];
 #pragma unroll
-      for (int t = 0; t < S::ti; ++t) {
-        const int row = wi + 32 * t + l31, o = row * 64, z = ort_swizzle(row);
-        lh[kk][t] = *(const f16x8*)(st + o + (c ^ z) * 8);
-        if (PAIRS) ll[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
+      for (int kk = 0; kk < ahead; ++kk) {
+        const int c = 2 * (k0 + kk) + hi;
+#pragma unroll
+        for (int t = 0; t < S::ti; ++t) {
+          const int row = wi + 32 * t + l31, o = row * 64, z = ort_swizzle(row);
+          lh[kk][t] = *(const f16x8*)(st + o + (c ^ z) * 8);
+          if (PAIRS) ll[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
+        }
+#pragma unroll
+        for (int t = 0; t < S::tj; ++t) {
+          const int row = wj + 32 * t + l31, o = (S::M + row) * 64, z = ort_swizzle(row);
+          rh[kk][t] = *(const f16x8*)(st + o + (c ^ z) * 8);
+          if (PAIRS) rl[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
+        }
       }
 #pragma unroll
-      for (int t = 0; t < S::tj; ++t) {
-        const int row = wj + 32 * t + l31, o = (S::M + row) * 64, z = ort_swizzle(row);
-        rh[kk][t] = *(const f16x8*)(st + o + (c ^ z) * 8);
-        if (PAIRS) rl[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
-      }
+      for (int kk = 0; kk < ahead; ++kk)
+#pragma unroll
+        for (int i = 0; i < S::ti; ++i)
+#pragma unroll
+          for (int j = 0; j < S::tj; ++j)
+            acc[i][j] = PAIRS ? ort_mma3(lh[kk][i], ll[kk][i], rh[kk][j], rl[kk][j], acc[i][j]) : PrecF16::mma(lh[kk][i], rh[kk][j], acc[i][j]);
     }
-#pragma unroll
-    for (int kk = 0; kk < kstep / 16; ++kk)
-#pragma unroll
-      for (int i = 0; i < S::ti; ++i)
-#pragma unroll
-        for (int j = 0; j < S::tj; ++j)
-          acc[i][j] = PAIRS ? ort_mma3(lh[kk][i], ll[kk][i], rh[kk][j], rl[kk][j], acc[i][j]) : PrecF16::mma(lh[kk][i], rh[kk][j], acc[i][j]);
     }
     slot = slot + 1 == S::ns ? 0 : slot + 1;
     fill = fill + 1 == S::ns ? 0 : fill + 1;
