@@ -5,23 +5,24 @@
 //              dx[t] = r[t],  da[t] = sum over the group of r[t] h[t-1],  dstate = a[0] r[0]
 //
 // Bound by memory: the forward reads a, x and writes h once, the backward reads a, x, dh and writes da, dx.  Composition of two steps
-// (a, b) then (a', b') is (a a', a' b + b'), so time is cut twice: a workgroup takes a CHUNK of positions at a time, each of its slots
-// SCAN_U consecutive positions of one channel in registers; slots compose their (a, b) by shuffles within a wave and through LDS between
-// waves, the state between chunks stays in registers, and the next chunk's loads are in flight meanwhile.  Where batch x channels give
-// too few workgroups, time is also cut into segments: a first launch composes each segment, and every workgroup of the second folds
-// the segments before its own.
+// (a, b) then (a', b') is (a a', a' b + b'), so time is cut: a workgroup of up to four waves takes a CHUNK of positions at a time, each of its
+// slots SCAN_U consecutive positions of one lane's channels in registers (as loaded; converted where used); slots compose their (a, b) by
+// shuffles within a wave and through LDS between waves -- one barrier a chunk --, the state between chunks stays in registers.  Four such
+// workgroups a compute unit hide each other's loads.  Where batch x channels give too few workgroups, time is also cut into segments: a first
+// launch composes each segment (its slots walk their share without a barrier), and every workgroup of the second folds the segments before
+// its own.
 //
-// The backward needs h[t-1] in binary32, not as the output rounded it: the forward leaves the state in front of every chunk ("marks",
-// 4 / chunk bytes per element), and the backward runs the chunk forward again from there.  Rounded states instead would cost the gate's
-// gradient up to half a step of the value's type.
+// The backward needs h[t-1] in binary32, not as the output rounded it: the forward leaves the state in front of every chunk of the backward
+// ("marks", 4 / chunk bytes per element), and the backward runs the chunk forward again from there.  Rounded states instead would cost the
+// gate's gradient up to half a step of the value's type.
 //
-// Work is laid out as tiles of CT = 2^cs channels (times V per lane); 64 / CT positions side by side fill a wave where channels are few.
-// A tile never spans two groups of a shared gate, so the gate's gradient is one sum over the tile's lanes; a group of several tiles adds
-// them in a second launch, in order.
+// Lanes hold tiles of CT = 2^cs channels (V each); 64 / CT positions side by side fill a wave where channels are few.  In the backward a tile
+// never spans two groups of a shared gate, so the gate's gradient is one sum over the tile's lanes; a group of several tiles adds them in a
+// second launch, in order.
 #include "nof_learn_dev.h"
 
-#define SCAN_U 8
-#define SCAN_MAXW 16                    // waves per workgroup at most
+#define SCAN_U 16
+#define SCAN_MAXW 4                     // waves per workgroup at most
 
 struct ScanArgs {
   const void* gate; const void* value; const void* dh;
@@ -31,16 +32,16 @@ struct ScanArgs {
   void* h; float* last; float* marks;
   const float* dlast;
   void* dvalue; void* dgate; float* dstate; float* gpart;
-  float* seg;                           // segment summaries
+  float* seg;                           // segment summaries [segs][B][2][D]
   int64_t T;
-  int B, D, G, P;                       // P = channels per tile group (D where each channel has its gate)
-  int cs, tiles_per_group, groups, tiles;
-  int waves, chunk, n_chunks, segs, chunks_per_seg;
+  int B, D, G, P;                       // P = channels per gate
   int per_channel, reverse;
+  int mark, n_marks;                    // positions between marks (the backward's chunk)
+  // the layout of a launch
+  int span;                             // channels that a row of tiles covers: D, or P where tiles keep to a gate's group
+  int cs, tiles_per_span, tiles;
+  int waves, chunk, n_chunks, segs, chunks_per_seg;
 };
-
-// position i of the recurrence (0 first) as a row of the tensors
-__device__ __forceinline__ int64_t scan_row(const ScanArgs& p, int64_t n, int64_t i) { return p.reverse ? n - 1 - i : i; }
 
 __device__ __forceinline__ int64_t scan_len(const ScanArgs& p, int b) {
   if (!p.lengths) return p.T;
@@ -48,12 +49,87 @@ __device__ __forceinline__ int64_t scan_len(const ScanArgs& p, int b) {
   return n < 0 ? 0 : n > p.T ? p.T : n;
 }
 
-// inclusive composition of the slots' (A, B) over the workgroup, in slot order (REV: from the last slot down).  On return (A, B) is the
-// composition of all slots BEFORE this one (identity for the first), and (TA, TB) of all slots.  `sh` holds SCAN_MAXW * 64 * V pairs.
+struct ScanWhere { int b, ch, span, slot; bool on; int64_t n; };
+
+// this thread's channels (an idle lane of a ragged tile reads its span's first ones and stores nothing) and its slot
+template <int V>
+__device__ __forceinline__ ScanWhere scan_where(const ScanArgs& p) {
+  ScanWhere q;
+  const int lane = threadIdx.x & 63, ct = 1 << p.cs, tile = blockIdx.x % p.tiles;
+  q.b = blockIdx.x / p.tiles;
+  q.span = tile / p.tiles_per_span;
+  const int in_span = ((tile % p.tiles_per_span) * ct + (lane & (ct - 1))) * V;
+  q.on = in_span < p.span;
+  q.ch = q.span * p.span + (q.on ? in_span : 0);
+  q.slot = (threadIdx.x >> 6) * (64 >> p.cs) + (lane >> p.cs);
+  q.n = scan_len(p, q.b);
+  return q;
+}
+
+// rows of one lane's channels in the recurrence's order: position i of the tensor's n existing rows
+template <typename T> struct ScanRows {
+  T* base; int64_t step;
+  __device__ __forceinline__ ScanRows(T* first, int64_t st, const ScanArgs& p, int64_t n) : base(p.reverse ? first + (n - 1) * st : first), step(p.reverse ? -st : st) {}
+  __device__ __forceinline__ T* at(int64_t i) const { return base + i * step; }
+  // the step for a run of rows.  (No instruction: the rows' offsets are formed at the run; hoisted before the chunks they fill the scalar
+  // registers and spill.)
+  __device__ __forceinline__ int64_t stride() const {
+    int64_t s = step;
+    asm volatile("" : "+s"(s));
+    return s;
+  }
+};
+
+// V elements as they lie in memory, two 16-bit ones in one register (as elements, the compiler gives each a register of its own and spills)
+template <int BYTES> struct ScanBits;
+template <> struct ScanBits<2> { typedef uint16_t t; };
+template <> struct ScanBits<4> { typedef uint32_t t; };
+template <> struct ScanBits<8> { typedef uint2 t; };
+template <typename T, int V> using ScanRaw = typename ScanBits<sizeof(T) * V>::t;
+__device__ __forceinline__ float scan_16(uint16_t b, __bf16) { return __uint_as_float((uint32_t)b << 16); }
+__device__ __forceinline__ float scan_16(uint16_t b, _Float16) { return (float)__builtin_bit_cast(_Float16, b); }
+__device__ __forceinline__ float scan_16(uint16_t b, float) { return 0.0f; }
+template <typename T, int V> __device__ __forceinline__ float scan_get(const ScanRaw<T, V>& r, int v) {
+  if constexpr (sizeof(T) == 4) {
+    if constexpr (V == 2) return __uint_as_float(v ? r.y : r.x);
+    else return __uint_as_float(r);
+  } else if constexpr (V == 2) {
+    return scan_16((uint16_t)(v ? r >> 16 : r & 0xffffu), T());
+  } else {
+    return scan_16(r, T());
+  }
+}
+template <typename T, int V> __device__ __forceinline__ ScanRaw<T, V> scan_fill(float x) {
+  LearnVec<T, V> f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) f.v[v] = lt<T>(x);
+  return __builtin_bit_cast(ScanRaw<T, V>, f);
+}
+
+// SCAN_U positions from i0 on of n > 0; positions from n on are `fill` (their loads go to the last row: a branch per row, or a predicate
+// per row and array, costs the compiler its registers)
+template <typename T, int V>
+__device__ __forceinline__ void scan_fetch(const ScanRows<const T>& x, int64_t i0, int64_t n, bool full, float fill, ScanRaw<T, V> (&r)[SCAN_U]) {
+  const T* p = x.at(i0);
+  const int64_t st = x.stride();
+  if (full) {
+#pragma unroll
+    for (int u = 0; u < SCAN_U; ++u) r[u] = *reinterpret_cast<const ScanRaw<T, V>*>(p + u * st);
+  } else {
+    const int64_t left = n - i0;
+#pragma unroll
+    for (int u = 0; u < SCAN_U; ++u) {
+      const ScanRaw<T, V> in = *reinterpret_cast<const ScanRaw<T, V>*>(p + (u < left ? u : left - 1) * st), out = scan_fill<T, V>(fill);
+      r[u] = u < left ? in : out;
+    }
+  }
+}
+
+// Composition over the slots of a workgroup, in slot order (REV: from the last slot down), in three parts so that two directions share a
+// barrier.  scan_wave: (A, B) of this slot -> of the slots before it in its wave, and the wave's whole into `sh`.
 template <int V, bool REV>
-__device__ __forceinline__ void scan_compose(float (&A)[V], float (&B)[V], float (&TA)[V], float (&TB)[V], int cs, int waves, float2* sh) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ct = 1 << cs, sub = lane >> cs, nsub = 64 >> cs;
-  const int at = REV ? nsub - 1 - sub : sub;
+__device__ __forceinline__ void scan_wave(float (&A)[V], float (&B)[V], int cs, float2* sh) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ct = 1 << cs, sub = lane >> cs, nsub = 64 >> cs, at = REV ? nsub - 1 - sub : sub;
   for (int o = 1; o < nsub; o <<= 1) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -63,197 +139,163 @@ __device__ __forceinline__ void scan_compose(float (&A)[V], float (&B)[V], float
   }
   if (at == nsub - 1) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) sh[(w * V + v) * ct + (lane & (ct - 1))] = make_float2(A[v], B[v]);
+    for (int v = 0; v < V; ++v) sh[(w * V + v) * 64 + (lane & (ct - 1))] = make_float2(A[v], B[v]);
   }
-  // exclusive within the wave
-  if (nsub > 1) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float a = REV ? __shfl_down(A[v], ct) : __shfl_up(A[v], ct), b = REV ? __shfl_down(B[v], ct) : __shfl_up(B[v], ct);
-      A[v] = at > 0 ? a : 1.0f;
-      B[v] = at > 0 ? b : 0.0f;
-    }
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) { A[v] = 1.0f; B[v] = 0.0f; }
+  for (int v = 0; v < V; ++v) {
+    const float a = nsub == 1 ? 1.0f : REV ? __shfl_down(A[v], ct) : __shfl_up(A[v], ct);
+    const float b = nsub == 1 ? 0.0f : REV ? __shfl_down(B[v], ct) : __shfl_up(B[v], ct);
+    A[v] = at > 0 ? a : 1.0f;
+    B[v] = at > 0 ? b : 0.0f;
   }
-  __syncthreads();
+}
+// behind a barrier: (A, B) -> of all slots before this one, (TA, TB) = of all slots
+template <int V, bool REV>
+__device__ __forceinline__ void scan_fold(float (&A)[V], float (&B)[V], float (&TA)[V], float (&TB)[V], int cs, int waves, const float2* sh) {
+  const int l = threadIdx.x & ((1 << cs) - 1), w = threadIdx.x >> 6;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     float pa = 1.0f, pb = 0.0f;
-    TA[v] = 1.0f; TB[v] = 0.0f;
-    for (int k = 0; k < waves; ++k) {
-      const int q = REV ? waves - 1 - k : k;
-      if (q == w) { pa = TA[v]; pb = TB[v]; }
-      const float2 s = sh[(q * V + v) * ct + (lane & (ct - 1))];
-      TB[v] = s.x * TB[v] + s.y;
-      TA[v] *= s.x;
+    TA[v] = 1.0f;
+    TB[v] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < SCAN_MAXW; ++k) {
+      const int q = REV ? SCAN_MAXW - 1 - k : k;
+      if (q < waves) {
+        if (q == w) { pa = TA[v]; pb = TB[v]; }
+        const float2 s = sh[(q * V + v) * 64 + l];
+        TB[v] = s.x * TB[v] + s.y;
+        TA[v] *= s.x;
+      }
     }
     B[v] = A[v] * pb + B[v];
     A[v] *= pa;
   }
 }
 
-// SCAN_U positions from i0 on of one lane's channels; what lies outside [0, n) or the tile is the identity (gate 1, value 0)
-template <typename T, int V>
-__device__ __forceinline__ void scan_load(const T* __restrict__ x, int64_t st, const ScanArgs& p, int64_t n, int64_t i0, bool on, float fill, float (&f)[SCAN_U][V]) {
-#pragma unroll
-  for (int u = 0; u < SCAN_U; ++u) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) f[u][v] = fill;
-    if (on && i0 + u < n) lload<T, V>(x + scan_row(p, n, i0 + u) * st, f[u]);
-  }
-}
-template <typename T, int V>
-__device__ __forceinline__ void scan_gate(const T* __restrict__ g, const ScanArgs& p, int64_t n, int64_t i0, bool on, float (&f)[SCAN_U][V]) {
-  if (p.per_channel) {
-    scan_load<T, V>(g, p.gate_st, p, n, i0, on, 1.0f, f);
-  } else {
-#pragma unroll
-    for (int u = 0; u < SCAN_U; ++u) {
-      float a = 1.0f;
-      if (on && i0 + u < n) a = lf(g[scan_row(p, n, i0 + u) * p.gate_st]);
-#pragma unroll
-      for (int v = 0; v < V; ++v) f[u][v] = a;
-    }
-  }
-}
-
-struct ScanWhere { int b, ch, group, slot; bool on; int64_t n; };
-
-template <int V>
-__device__ __forceinline__ ScanWhere scan_where(const ScanArgs& p) {
-  ScanWhere q;
-  const int lane = threadIdx.x & 63, ct = 1 << p.cs;
-  const int tile = blockIdx.x % p.tiles;
-  q.b = blockIdx.x / p.tiles;
-  q.group = tile / p.tiles_per_group;
-  const int in_group = ((tile % p.tiles_per_group) * ct + (lane & (ct - 1))) * V;
-  q.on = in_group < p.P;
-  q.ch = q.group * p.P + (q.on ? in_group : 0);
-  q.slot = (threadIdx.x >> 6) * (64 >> p.cs) + (lane >> p.cs);
-  q.n = scan_len(p, q.b);
-  return q;
-}
-
-// (A, B) of a segment, seg [B, tiles' channels D, segs] as two planes: what the forward's launch of segments folds
-template <typename TG, typename T, int V, bool BACK>
-__global__ __launch_bounds__(64 * SCAN_MAXW) void k_scan_segments(ScanArgs p) {
-  __shared__ float2 sh[2][SCAN_MAXW * 64 * V];
+// The composition of a whole segment.  BACK: of the recurrence of what positions hand to the one before, c[t-1] = a[t] (dh[t] + c[t]).
+// The segment's slots take equal stretches of it, so that the only barrier is the last composition's.
+template <typename TG, typename T, int V, bool PC, bool BACK>
+__global__ __launch_bounds__(64 * SCAN_MAXW, 4) void k_scan_segments(ScanArgs p) {
+  __shared__ float2 sh[SCAN_MAXW * 64 * V];
   const ScanWhere q = scan_where<V>(p);
   const int seg = BACK ? blockIdx.y + 1 : blockIdx.y;               // nobody needs the forward's last or the backward's first
-  const TG* g = (const TG*)p.gate + q.b * p.gate_sb + (p.per_channel ? q.ch : q.group);
-  const T* x = BACK ? (const T*)p.dh + q.b * p.dh_sb + q.ch : (const T*)p.value + q.b * p.value_sb + q.ch;
-  const int64_t st = BACK ? p.dh_st : p.value_st;
-  const int64_t c0 = (int64_t)seg * p.chunks_per_seg, c1 = c0 + p.chunks_per_seg < p.n_chunks ? c0 + p.chunks_per_seg : p.n_chunks;
-  float SA[V], SB[V];
+  const ScanRows<const TG> g((const TG*)p.gate + q.b * p.gate_sb + (PC ? q.ch : q.ch / p.P), p.gate_st, p, q.n);
+  const ScanRows<const T> x(BACK ? (const T*)p.dh + q.b * p.dh_sb + q.ch : (const T*)p.value + q.b * p.value_sb + q.ch, BACK ? p.dh_st : p.value_st, p, q.n);
+  const int64_t seg0 = (int64_t)seg * p.chunks_per_seg * p.chunk, each = (int64_t)p.chunks_per_seg * SCAN_U, i0 = seg0 + q.slot * each;
+  const bool full = seg0 + (int64_t)p.chunks_per_seg * p.chunk <= q.n;
+  float A[V], B[V], TA[V], TB[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) { SA[v] = 1.0f; SB[v] = 0.0f; }
-  float a[SCAN_U][V], x_[SCAN_U][V];
-  int flip = 0;
-  for (int64_t k = 0; k < c1 - c0; ++k, flip ^= 1) {
-    const int64_t c = BACK ? c1 - 1 - k : c0 + k, i0 = c * p.chunk + (int64_t)q.slot * SCAN_U;
-    if (c * p.chunk >= q.n) { if (BACK) continue; else break; }
-    scan_gate<TG, V>(g, p, q.n, i0, q.on, a);
-    scan_load<T, V>(x, st, p, q.n, i0, q.on, 0.0f, x_);
-    float A[V], Bv[V], TA[V], TB[V];
+  for (int v = 0; v < V; ++v) { A[v] = 1.0f; B[v] = 0.0f; }
+  for (int k = 0; k < p.chunks_per_seg; ++k) {
+    const int64_t i = i0 + (int64_t)(BACK ? p.chunks_per_seg - 1 - k : k) * SCAN_U;
+    if (i >= q.n) continue;
+    ScanRaw<TG, PC ? V : 1> a[SCAN_U];
+    ScanRaw<T, V> r[SCAN_U];
+    scan_fetch<TG, PC ? V : 1>(g, i, q.n, full, 1.0f, a);
+    scan_fetch<T, V>(x, i, q.n, full, 0.0f, r);
 #pragma unroll
-    for (int v = 0; v < V; ++v) { A[v] = 1.0f; Bv[v] = 0.0f; }
-    if (BACK) {
-      // carry into position t-1 is a[t] (dh[t] + carry): composition (a, a dh)
+    for (int t = 0; t < SCAN_U; ++t) {
+      const int u = BACK ? SCAN_U - 1 - t : t;
 #pragma unroll
-      for (int u = SCAN_U - 1; u >= 0; --u)
-#pragma unroll
-        for (int v = 0; v < V; ++v) { Bv[v] = a[u][v] * (x_[u][v] + Bv[v]); A[v] *= a[u][v]; }
-    } else {
-#pragma unroll
-      for (int u = 0; u < SCAN_U; ++u)
-#pragma unroll
-        for (int v = 0; v < V; ++v) { Bv[v] = a[u][v] * Bv[v] + x_[u][v]; A[v] *= a[u][v]; }
+      for (int v = 0; v < V; ++v) {
+        const float av = scan_get<TG, PC ? V : 1>(a[u], PC ? v : 0), xv = scan_get<T, V>(r[u], v);
+        B[v] = BACK ? av * (xv + B[v]) : av * B[v] + xv;
+        A[v] *= av;
+      }
     }
-    scan_compose<V, BACK>(A, Bv, TA, TB, p.cs, p.waves, sh[flip]);
-#pragma unroll
-    for (int v = 0; v < V; ++v) { SB[v] = TA[v] * SB[v] + TB[v]; SA[v] *= TA[v]; }
   }
+  scan_wave<V, BACK>(A, B, p.cs, sh);
+  __syncthreads();
+  scan_fold<V, BACK>(A, B, TA, TB, p.cs, p.waves, sh);
   if (q.slot == 0 && q.on) {
     float* out = p.seg + (((int64_t)seg * p.B + q.b) * 2) * p.D + q.ch;
-    lstore<float, V>(out, SA);
-    lstore<float, V>(out + p.D, SB);
+    lstore<float, V>(out, TA);
+    lstore<float, V>(out + p.D, TB);
   }
 }
 
-template <typename TG, typename T, int V>
-__global__ __launch_bounds__(64 * SCAN_MAXW) void k_scan_fwd(ScanArgs p) {
+// S -> what it becomes over segments lo, lo + step, ... (count of them)
+template <int V>
+__device__ __forceinline__ void scan_over(const ScanArgs& p, const ScanWhere& q, int lo, int step, int count, float (&S)[V]) {
+#pragma unroll 4
+  for (int k = 0; k < count; ++k) {
+    float A[V], B[V];
+    const float* s = p.seg + (((int64_t)(lo + k * step) * p.B + q.b) * 2) * p.D + q.ch;
+    lload<float, V>(s, A);
+    lload<float, V>(s + p.D, B);
+#pragma unroll
+    for (int v = 0; v < V; ++v) S[v] = A[v] * S[v] + B[v];
+  }
+}
+
+template <typename TG, typename T, int V, bool PC>
+__global__ __launch_bounds__(64 * SCAN_MAXW, 3) void k_scan_fwd(ScanArgs p) {
   __shared__ float2 sh[2][SCAN_MAXW * 64 * V];
   const ScanWhere q = scan_where<V>(p);
-  const TG* g = (const TG*)p.gate + q.b * p.gate_sb + (p.per_channel ? q.ch : q.group);
-  const T* x = (const T*)p.value + q.b * p.value_sb + q.ch;
-  T* h = p.h ? (T*)p.h + (int64_t)q.b * p.T * p.D + q.ch : nullptr;
-  const int seg = blockIdx.y;
-  const int64_t c0 = (int64_t)seg * p.chunks_per_seg, c1 = c0 + p.chunks_per_seg < p.n_chunks ? c0 + p.chunks_per_seg : p.n_chunks;
+  const ScanRows<const TG> g((const TG*)p.gate + q.b * p.gate_sb + (PC ? q.ch : q.ch / p.P), p.gate_st, p, q.n);
+  const ScanRows<const T> x((const T*)p.value + q.b * p.value_sb + q.ch, p.value_st, p, q.n);
+  T* h0 = p.h ? (T*)p.h + (int64_t)q.b * p.T * p.D + q.ch : nullptr;
+  const ScanRows<T> h(h0, p.D, p, q.n);
+  const int seg = blockIdx.y, c0 = seg * p.chunks_per_seg, c1 = c0 + p.chunks_per_seg < p.n_chunks ? c0 + p.chunks_per_seg : p.n_chunks;
   float S[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) S[v] = 0.0f;
-  if (p.state && q.on) lload<float, V>(p.state + (int64_t)q.b * p.D + q.ch, S);
-  for (int k = 0; k < seg; ++k) {
-    float A[V], Bv[V];
-    const float* s = p.seg + (((int64_t)k * p.B + q.b) * 2) * p.D + q.ch;
-    lload<float, V>(s, A);
-    lload<float, V>(s + p.D, Bv);
-#pragma unroll
-    for (int v = 0; v < V; ++v) S[v] = A[v] * S[v] + Bv[v];
+  if (p.state) lload<float, V>(p.state + (int64_t)q.b * p.D + q.ch, S);
+  ScanRaw<TG, PC ? V : 1> a[SCAN_U];
+  ScanRaw<T, V> r[SCAN_U];
+  const int64_t at0 = (int64_t)c0 * p.chunk;
+  if (at0 < q.n) {
+    scan_fetch<TG, PC ? V : 1>(g, at0 + q.slot * SCAN_U, q.n, at0 + p.chunk <= q.n, 1.0f, a);
+    scan_fetch<T, V>(x, at0 + q.slot * SCAN_U, q.n, at0 + p.chunk <= q.n, 0.0f, r);
   }
-  float a[SCAN_U][V], b[SCAN_U][V];
-  scan_gate<TG, V>(g, p, q.n, c0 * p.chunk + (int64_t)q.slot * SCAN_U, q.on, a);
-  scan_load<T, V>(x, p.value_st, p, q.n, c0 * p.chunk + (int64_t)q.slot * SCAN_U, q.on, 0.0f, b);
-  int flip = 0;
-  for (int64_t c = c0; c < c1; ++c, flip ^= 1) {
-    const int64_t i0 = c * p.chunk + (int64_t)q.slot * SCAN_U;
-    if (p.marks && q.slot == 0 && q.on) lstore<float, V>(p.marks + ((int64_t)q.b * p.n_chunks + c) * p.D + q.ch, S);
-    if (c * p.chunk < q.n) {
-      float A[V], Bv[V], TA[V], TB[V];
+  scan_over<V>(p, q, 0, 1, seg, S);
+  for (int c = c0; c < c1; ++c) {
+    const int64_t at = (int64_t)c * p.chunk, i0 = at + q.slot * SCAN_U;
+    const bool full = at + p.chunk <= q.n;
+    if (at < q.n) {
+      float A[V], B[V], TA[V], TB[V], s[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) { A[v] = 1.0f; Bv[v] = 0.0f; }
+      for (int v = 0; v < V; ++v) { A[v] = 1.0f; B[v] = 0.0f; }
 #pragma unroll
       for (int u = 0; u < SCAN_U; ++u)
 #pragma unroll
-        for (int v = 0; v < V; ++v) { Bv[v] = a[u][v] * Bv[v] + b[u][v]; A[v] *= a[u][v]; }
-      float a2[SCAN_U][V], b2[SCAN_U][V];
-      const int64_t i1 = i0 + p.chunk;
-      const bool more = c + 1 < c1;
-      scan_gate<TG, V>(g, p, more ? q.n : 0, i1, q.on, a2);
-      scan_load<T, V>(x, p.value_st, p, more ? q.n : 0, i1, q.on, 0.0f, b2);
-      scan_compose<V, false>(A, Bv, TA, TB, p.cs, p.waves, sh[flip]);
-      float s[V];
+        for (int v = 0; v < V; ++v) { const float av = scan_get<TG, PC ? V : 1>(a[u], PC ? v : 0); B[v] = av * B[v] + scan_get<T, V>(r[u], v); A[v] *= av; }
+      scan_wave<V, false>(A, B, p.cs, sh[c & 1]);
+      __syncthreads();
+      scan_fold<V, false>(A, B, TA, TB, p.cs, p.waves, sh[c & 1]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) { s[v] = A[v] * S[v] + Bv[v]; S[v] = TA[v] * S[v] + TB[v]; }
+      for (int v = 0; v < V; ++v) { s[v] = A[v] * S[v] + B[v]; S[v] = TA[v] * S[v] + TB[v]; }
+      if (p.marks && q.on && i0 < q.n && (uint32_t)i0 % (uint32_t)p.mark == 0) lstore<float, V>(p.marks + ((int64_t)q.b * p.n_marks + (uint32_t)i0 / (uint32_t)p.mark) * p.D + q.ch, s);
+      T* o = h.at(i0);
+      const int64_t ost = h.stride();
+      const int64_t left = full ? SCAN_U : q.n - i0;
 #pragma unroll
       for (int u = 0; u < SCAN_U; ++u) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) s[v] = a[u][v] * s[v] + b[u][v];
-        if (h && q.on && i0 + u < q.n) lstore<T, V>(h + scan_row(p, q.n, i0 + u) * p.D, s);
-        if (p.last && q.on && i0 + u == q.n - 1) lstore<float, V>(p.last + (int64_t)q.b * p.D + q.ch, s);
+        for (int v = 0; v < V; ++v) s[v] = scan_get<TG, PC ? V : 1>(a[u], PC ? v : 0) * s[v] + scan_get<T, V>(r[u], v);
+        if (h0 && q.on && u < left) lstore<T, V>(o + u * ost, s);
       }
-#pragma unroll
-      for (int u = 0; u < SCAN_U; ++u)
-#pragma unroll
-        for (int v = 0; v < V; ++v) { a[u][v] = a2[u][v]; b[u][v] = b2[u][v]; }
+      // (positions behind the end keep the state)
+      if (p.last && q.on && i0 < q.n && i0 + SCAN_U >= q.n) lstore<float, V>(p.last + (int64_t)q.b * p.D + q.ch, s);
+      if (c + 1 < c1 && at + p.chunk < q.n) {
+        scan_fetch<TG, PC ? V : 1>(g, i0 + p.chunk, q.n, at + 2 * p.chunk <= q.n, 1.0f, a);
+        scan_fetch<T, V>(x, i0 + p.chunk, q.n, at + 2 * p.chunk <= q.n, 0.0f, r);
+      }
     }
-    if (h && q.on) {                                                  // rows behind the sequence's end
+    if (h0 && q.on && !full) {                                        // rows behind the sequence's end
       float z[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) z[v] = 0.0f;
-#pragma unroll
-      for (int u = 0; u < SCAN_U; ++u)
-        if (i0 + u >= q.n && i0 + u < p.T) lstore<T, V>(h + (i0 + u) * p.D, z);
+      for (int64_t i = i0 > q.n ? i0 : q.n; i < i0 + SCAN_U && i < p.T; ++i) lstore<T, V>(h0 + i * p.D, z);
     }
   }
   if (q.n == 0 && seg == 0 && q.slot == 0 && q.on && p.last) lstore<float, V>(p.last + (int64_t)q.b * p.D + q.ch, S);
 }
 
-// sum of f[u] over the 2^cs lanes of a tile, for all SCAN_U values: each exchange halves what is left to add, so 8 values over 64 lanes
-// take 4 + 2 + 1 + 3 exchanges instead of 48.  Lane l ends with the sum of f[u], u = the top three bits of its index in the tile
-// (for tiles of fewer lanes: of the value(s) that its bits name).
+// sum of f[u] over the 2^cs lanes of a tile, for all SCAN_U values: each exchange halves what is left to add, so 16 values over 64 lanes
+// take 8 + 4 + 2 + 1 + 2 exchanges instead of 96.  The highest bits of a lane's index in the tile choose between the upper and the
+// lower half of what was left; lanes that agree in them end with the same sums f[0 .. left).
 __device__ __forceinline__ void scan_tile_sum(float (&f)[SCAN_U], int cs) {
   const int lane = threadIdx.x & 63;
   int left = SCAN_U;
@@ -276,112 +318,108 @@ __device__ __forceinline__ void scan_tile_sum(float (&f)[SCAN_U], int cs) {
   }
 }
 
-template <typename TG, typename T, int V>
-__global__ __launch_bounds__(64 * SCAN_MAXW) void k_scan_bwd(ScanArgs p) {
-  __shared__ float2 sh[2][SCAN_MAXW * 64 * V];
+template <typename TG, typename T, int V, bool PC>
+__global__ __launch_bounds__(64 * SCAN_MAXW, PC || V == 1 ? 3 : 2) void k_scan_bwd(ScanArgs p) {
+  __shared__ float2 sh[2][2][SCAN_MAXW * 64 * V];
   const ScanWhere q = scan_where<V>(p);
-  const int lane = threadIdx.x & 63, ct = 1 << p.cs, tile = blockIdx.x % p.tiles;
-  const TG* g = (const TG*)p.gate + q.b * p.gate_sb + (p.per_channel ? q.ch : q.group);
-  const T* x = (const T*)p.value + q.b * p.value_sb + q.ch;
-  const T* dh = (const T*)p.dh + q.b * p.dh_sb + q.ch;
-  T* dx = (T*)p.dvalue + (int64_t)q.b * p.T * p.D + q.ch;
-  const int seg = blockIdx.y;
-  const int64_t c0 = (int64_t)seg * p.chunks_per_seg, c1 = c0 + p.chunks_per_seg < p.n_chunks ? c0 + p.chunks_per_seg : p.n_chunks;
+  const int lane = threadIdx.x & 63, ct = 1 << p.cs, part = blockIdx.x % p.tiles % p.tiles_per_span, group = PC ? 0 : q.span;
+  const ScanRows<const TG> g((const TG*)p.gate + q.b * p.gate_sb + (PC ? q.ch : group), p.gate_st, p, q.n);
+  const ScanRows<const T> x((const T*)p.value + q.b * p.value_sb + q.ch, p.value_st, p, q.n), y((const T*)p.dh + q.b * p.dh_sb + q.ch, p.dh_st, p, q.n);
+  T* dx0 = (T*)p.dvalue + (int64_t)q.b * p.T * p.D + q.ch;
+  const ScanRows<T> dx(dx0, p.D, p, q.n);
+  TG* dg0 = PC ? (TG*)p.dgate + (int64_t)q.b * p.T * p.D + q.ch : (TG*)p.dgate + (int64_t)q.b * p.T * p.G + group;
+  const ScanRows<TG> dg(dg0, PC ? p.D : p.G, p, q.n);
+  float* gp0 = p.gpart + ((int64_t)q.b * p.T * p.G + group) * p.tiles_per_span + part;               // (a shared gate of several tiles)
+  const ScanRows<float> gp(gp0, (int64_t)p.G * p.tiles_per_span, p, q.n);
+  const int seg = blockIdx.y, c0 = seg * p.chunks_per_seg, c1 = c0 + p.chunks_per_seg < p.n_chunks ? c0 + p.chunks_per_seg : p.n_chunks;
   float R[V];                                                       // what later positions hand to this one
 #pragma unroll
   for (int v = 0; v < V; ++v) R[v] = 0.0f;
-  if (p.dlast && q.on) lload<float, V>(p.dlast + (int64_t)q.b * p.D + q.ch, R);
-  for (int k = p.segs - 1; k > seg; --k) {
-    float A[V], Bv[V];
-    const float* s = p.seg + (((int64_t)k * p.B + q.b) * 2) * p.D + q.ch;
-    lload<float, V>(s, A);
-    lload<float, V>(s + p.D, Bv);
+  if (p.dlast) lload<float, V>(p.dlast + (int64_t)q.b * p.D + q.ch, R);
+  scan_over<V>(p, q, p.segs - 1, -1, p.segs - 1 - seg, R);
+  for (int c = c1 - 1; c >= c0; --c) {
+    const int64_t at = (int64_t)c * p.chunk, i0 = at + q.slot * SCAN_U;
+    const bool full = at + p.chunk <= q.n;
+    if (at < q.n) {
+      ScanRaw<TG, PC ? V : 1> a[SCAN_U];
+      ScanRaw<T, V> r[SCAN_U], d[SCAN_U];
+      float A[V], B[V], A2[V], B2[V], TA[V], TB[V], m[V], s[V], hp[SCAN_U][V];
+      scan_fetch<TG, PC ? V : 1>(g, i0, q.n, full, 1.0f, a);
+      scan_fetch<T, V>(x, i0, q.n, full, 0.0f, r);
+      scan_fetch<T, V>(y, i0, q.n, full, 0.0f, d);
+      lload<float, V>(p.marks + ((int64_t)q.b * p.n_marks + c) * p.D + q.ch, m);
 #pragma unroll
-    for (int v = 0; v < V; ++v) R[v] = A[v] * R[v] + Bv[v];
-  }
-  for (int64_t c = c1 - 1; c >= c0; --c) {
-    const int64_t i0 = c * p.chunk + (int64_t)q.slot * SCAN_U;
-    if (c * p.chunk < q.n) {
-      float a[SCAN_U][V], b[SCAN_U][V], d[SCAN_U][V], A[V], Bv[V], A2[V], B2[V], TA[V], TB[V], m[V];
-      scan_gate<TG, V>(g, p, q.n, i0, q.on, a);
-      scan_load<T, V>(x, p.value_st, p, q.n, i0, q.on, 0.0f, b);
-      scan_load<T, V>(dh, p.dh_st, p, q.n, i0, q.on, 0.0f, d);
-#pragma unroll
-      for (int v = 0; v < V; ++v) m[v] = 0.0f;
-      if (q.on) lload<float, V>(p.marks + ((int64_t)q.b * p.n_chunks + c) * p.D + q.ch, m);
-#pragma unroll
-      for (int v = 0; v < V; ++v) { A[v] = 1.0f; Bv[v] = 0.0f; B2[v] = 0.0f; }
+      for (int v = 0; v < V; ++v) { A[v] = 1.0f; B[v] = 0.0f; B2[v] = 0.0f; }
 #pragma unroll
       for (int u = 0; u < SCAN_U; ++u)
 #pragma unroll
-        for (int v = 0; v < V; ++v) { Bv[v] = a[u][v] * Bv[v] + b[u][v]; A[v] *= a[u][v]; }
+        for (int v = 0; v < V; ++v) { const float av = scan_get<TG, PC ? V : 1>(a[u], PC ? v : 0); B[v] = av * B[v] + scan_get<T, V>(r[u], v); A[v] *= av; }
 #pragma unroll
       for (int u = SCAN_U - 1; u >= 0; --u)
 #pragma unroll
-        for (int v = 0; v < V; ++v) B2[v] = a[u][v] * (d[u][v] + B2[v]);
+        for (int v = 0; v < V; ++v) B2[v] = scan_get<TG, PC ? V : 1>(a[u], PC ? v : 0) * (scan_get<T, V>(d[u], v) + B2[v]);
 #pragma unroll
       for (int v = 0; v < V; ++v) A2[v] = A[v];
-      scan_compose<V, false>(A, Bv, TA, TB, p.cs, p.waves, sh[0]);
-      float s[V], r[V];
+      scan_wave<V, false>(A, B, p.cs, sh[c & 1][0]);
+      scan_wave<V, true>(A2, B2, p.cs, sh[c & 1][1]);
+      __syncthreads();
+      scan_fold<V, false>(A, B, TA, TB, p.cs, p.waves, sh[c & 1][0]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) s[v] = A[v] * m[v] + Bv[v];
-      scan_compose<V, true>(A2, B2, TA, TB, p.cs, p.waves, sh[1]);
+      for (int v = 0; v < V; ++v) s[v] = A[v] * m[v] + B[v];
+      scan_fold<V, true>(A2, B2, TA, TB, p.cs, p.waves, sh[c & 1][1]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) { r[v] = A2[v] * R[v] + B2[v]; R[v] = TA[v] * R[v] + TB[v]; }
-#pragma unroll
-      for (int u = 0; u < SCAN_U; ++u)                              // b: h before each position
-#pragma unroll
-        for (int v = 0; v < V; ++v) { const float x0 = b[u][v]; b[u][v] = s[v]; s[v] = a[u][v] * s[v] + x0; }
-#pragma unroll
-      for (int u = SCAN_U - 1; u >= 0; --u)                         // d: r; b: the gate's gradient
-#pragma unroll
-        for (int v = 0; v < V; ++v) { d[u][v] += r[v]; r[v] = a[u][v] * d[u][v]; b[u][v] *= d[u][v]; }
+      for (int v = 0; v < V; ++v) { B2[v] = A2[v] * R[v] + B2[v]; R[v] = TA[v] * R[v] + TB[v]; }
 #pragma unroll
       for (int u = 0; u < SCAN_U; ++u)
-        if (q.on && i0 + u < q.n) {
-          const int64_t row = scan_row(p, q.n, i0 + u);
-          lstore<T, V>(dx + row * p.D, d[u]);
-          if (p.per_channel) lstore<TG, V>((TG*)p.dgate + ((int64_t)q.b * p.T + row) * p.D + q.ch, b[u]);
-        }
-      if (!p.per_channel) {
-        float f[SCAN_U];
 #pragma unroll
-        for (int u = 0; u < SCAN_U; ++u) {
-          f[u] = 0.0f;
+        for (int v = 0; v < V; ++v) { hp[u][v] = s[v]; s[v] = scan_get<TG, PC ? V : 1>(a[u], PC ? v : 0) * s[v] + scan_get<T, V>(r[u], v); }
+      T* o = dx.at(i0);
+      TG* og = dg.at(i0);
+      const int64_t ost = dx.stride(), gst = dg.stride();
+      float f[SCAN_U];
+      const int64_t left = full ? SCAN_U : q.n - i0;
 #pragma unroll
-          for (int v = 0; v < V; ++v) f[u] += q.on ? b[u][v] : 0.0f;
+      for (int u = SCAN_U - 1; u >= 0; --u) {
+        float e[V];
+        f[u] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          e[v] = scan_get<T, V>(d[u], v) + B2[v];                               // r[t]
+          hp[u][v] *= e[v];
+          B2[v] = scan_get<TG, PC ? V : 1>(a[u], PC ? v : 0) * e[v];
+          f[u] += q.on ? hp[u][v] : 0.0f;
         }
+        if (q.on && u < left) {
+          lstore<T, V>(o + u * ost, e);
+          if (PC) lstore<TG, V>(og + u * gst, hp[u]);
+        }
+      }
+      if (!PC) {
         scan_tile_sum(f, p.cs);
-        // lane bits cs-1, cs-2, cs-3 chose between the upper and the lower half of what was left
         const int in = lane & (ct - 1);
-        int left = SCAN_U, u0 = 0;
-        for (int k = 0; k < 3 && k < p.cs; ++k) { left >>= 1; if (in >> (p.cs - 1 - k) & 1) u0 += left; }
-        const int low = p.cs > 3 ? in & ((1 << (p.cs - 3)) - 1) : 0;
+        int mine = SCAN_U, u0 = 0;
+        for (int k = 0; k < 4 && k < p.cs; ++k) { mine >>= 1; if (in >> (p.cs - 1 - k) & 1) u0 += mine; }
+        const int low = p.cs > 4 ? in & ((1 << (p.cs - 4)) - 1) : 0;
 #pragma unroll
         for (int j = 0; j < SCAN_U; ++j)
-          if (low == 0 && j < left && i0 + u0 + j < q.n) {
-            const int64_t at = ((int64_t)q.b * p.T + scan_row(p, q.n, i0 + u0 + j)) * p.G + q.group;
-            if (p.tiles_per_group == 1) ((TG*)p.dgate)[at] = lt<TG>(f[j]);
-            else p.gpart[at * p.tiles_per_group + tile % p.tiles_per_group] = f[j];
+          if (low == 0 && j < mine && u0 + j < left) {
+            if (p.tiles_per_span == 1) *dg.at(i0 + u0 + j) = lt<TG>(f[j]);
+            else *gp.at(i0 + u0 + j) = f[j];
           }
       }
-      __syncthreads();                                              // sh is written again by the next chunk
     }
-    if (q.on) {                                                       // rows behind the sequence's end have no gradient
+    if (q.on && !full) {                                              // rows behind the sequence's end have no gradient
       float z[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) z[v] = 0.0f;
-#pragma unroll
-      for (int u = 0; u < SCAN_U; ++u)
-        if (i0 + u >= q.n && i0 + u < p.T) {
-          lstore<T, V>(dx + (i0 + u) * p.D, z);
-          const int64_t row = (int64_t)q.b * p.T + i0 + u;
-          if (p.per_channel) lstore<TG, V>((TG*)p.dgate + row * p.D + q.ch, z);
-          else if ((lane & (ct - 1)) == 0) {
-            if (p.tiles_per_group == 1) ((TG*)p.dgate)[row * p.G + q.group] = lt<TG>(0.0f);
-            else p.gpart[(row * p.G + q.group) * p.tiles_per_group + tile % p.tiles_per_group] = 0.0f;
-          }
+      for (int64_t i = i0 > q.n ? i0 : q.n; i < i0 + SCAN_U && i < p.T; ++i) {
+        lstore<T, V>(dx0 + i * p.D, z);
+        if (PC) lstore<TG, V>(dg0 + i * p.D, z);
+        else if ((lane & (ct - 1)) == 0) {
+          if (p.tiles_per_span == 1) dg0[i * p.G] = lt<TG>(0.0f);
+          else gp0[i * p.G * p.tiles_per_span] = 0.0f;
         }
+      }
     }
   }
   if (seg == 0 && q.slot == 0 && q.on && p.dstate) lstore<float, V>(p.dstate + (int64_t)q.b * p.D + q.ch, R);
@@ -420,26 +458,32 @@ __global__ __launch_bounds__(256) void k_scan_step(const TG* __restrict__ gate, 
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 // Everything here depends on the sizes alone, so that the forward's marks fit the backward.
-static bool scan_plan(ScanArgs& p, int64_t B, int64_t T, int32_t D, int32_t G, int v) {
-  p.T = T; p.B = (int)B; p.D = D; p.G = G;
-  p.per_channel = G == D;
-  p.groups = p.per_channel ? 1 : G;
-  p.P = D / p.groups;
-  const int nv = p.P / v;
+// Segments: from one wave per SIMD on, a workgroup's own look-ahead keeps the memory busy and a second pass over the inputs would cost more
+// than it gives; below, two waves per SIMD, of two chunks at least.
+static void scan_layout(ScanArgs& p, int span, int v) {
+  p.span = span;
+  const int nv = span / v;
   p.cs = learn_log2_up(nv < 64 ? nv : 64);
-  p.tiles_per_group = (int)nof_div_up(nv, (int64_t)1 << p.cs);
-  p.tiles = p.groups * p.tiles_per_group;
-  const int64_t slots = nof_div_up(T, SCAN_U), per_wave = 64 >> p.cs;
-  p.waves = 1;
-  while (p.waves < SCAN_MAXW && p.waves * per_wave < slots) p.waves *= 2;
+  p.tiles_per_span = (int)nof_div_up(nv, (int64_t)1 << p.cs);
+  p.tiles = p.D / span * p.tiles_per_span;
+  const int64_t slots = nof_div_up(p.T, SCAN_U), per_wave = 64 >> p.cs, need = nof_div_up(slots, per_wave);
+  p.waves = (int)(need < 1 ? 1 : need < SCAN_MAXW ? need : SCAN_MAXW);
   p.chunk = (int)(p.waves * per_wave * SCAN_U);
-  p.n_chunks = (int)nof_div_up(T, p.chunk);
-  // segments: enough workgroups for two per compute unit, of two chunks at least
-  const int64_t wgs = B * p.tiles, want = wgs > 0 ? nof_div_up(512, wgs) : 1, most = p.n_chunks / 2 > 1 ? p.n_chunks / 2 : 1;
+  p.n_chunks = (int)nof_div_up(p.T, p.chunk);
+  const int64_t waves = (int64_t)p.B * p.tiles * p.waves, want = waves >= 1024 ? 1 : nof_div_up(2048, waves), most = p.n_chunks / 2 > 1 ? p.n_chunks / 2 : 1;
   p.segs = (int)(want < most ? want : most);
   p.chunks_per_seg = (int)nof_div_up(p.n_chunks > 0 ? p.n_chunks : 1, p.segs);
   p.segs = (int)nof_div_up(p.n_chunks > 0 ? p.n_chunks : 1, p.chunks_per_seg);
-  return wgs < (int64_t)1 << 31;
+}
+static bool scan_plan(ScanArgs& p, int64_t B, int64_t T, int32_t D, int32_t G, int v, bool back) {
+  p.T = T; p.B = (int)B; p.D = D; p.G = G;
+  p.per_channel = G == D;
+  p.P = D / G;
+  scan_layout(p, p.per_channel ? D : p.P, v);
+  p.mark = p.chunk;
+  p.n_marks = p.n_chunks;
+  if (!back) scan_layout(p, D, v);
+  return B * p.tiles < (int64_t)1 << 31;
 }
 
 // two 16-bit channels a lane where a group is even
@@ -458,43 +502,51 @@ static bool scan_aligned(const void* x, int64_t sb, int64_t st, int size, int v)
   return ((uintptr_t)x % (uintptr_t)(size * v)) == 0 && sb % v == 0 && st % v == 0;
 }
 
-#define SCAN_PICK(KERNEL, GRID, BLOCK, ...)                                                                                            \
-  do {                                                                                                                                \
-    if (type == NOF_TYPE_F32) hipLaunchKernelGGL((KERNEL<float, float, 1 __VA_ARGS__>), GRID, BLOCK, 0, st, p);                        \
-    else if (type == NOF_TYPE_BF16 && gate_type == type) {                                                                            \
-      if (v == 2) hipLaunchKernelGGL((KERNEL<__bf16, __bf16, 2 __VA_ARGS__>), GRID, BLOCK, 0, st, p);                                  \
-      else hipLaunchKernelGGL((KERNEL<__bf16, __bf16, 1 __VA_ARGS__>), GRID, BLOCK, 0, st, p);                                         \
-    } else if (type == NOF_TYPE_BF16) {                                                                                               \
-      if (v == 2) hipLaunchKernelGGL((KERNEL<float, __bf16, 2 __VA_ARGS__>), GRID, BLOCK, 0, st, p);                                   \
-      else hipLaunchKernelGGL((KERNEL<float, __bf16, 1 __VA_ARGS__>), GRID, BLOCK, 0, st, p);                                          \
-    } else if (gate_type == type) {                                                                                                   \
-      if (v == 2) hipLaunchKernelGGL((KERNEL<_Float16, _Float16, 2 __VA_ARGS__>), GRID, BLOCK, 0, st, p);                              \
-      else hipLaunchKernelGGL((KERNEL<_Float16, _Float16, 1 __VA_ARGS__>), GRID, BLOCK, 0, st, p);                                     \
-    } else {                                                                                                                          \
-      if (v == 2) hipLaunchKernelGGL((KERNEL<float, _Float16, 2 __VA_ARGS__>), GRID, BLOCK, 0, st, p);                                 \
-      else hipLaunchKernelGGL((KERNEL<float, _Float16, 1 __VA_ARGS__>), GRID, BLOCK, 0, st, p);                                        \
-    }                                                                                                                                 \
+#define SCAN_GO(KERNEL, GRID, BLOCK, TG, T, V, ...)                                                          \
+  do {                                                                                                       \
+    if (p.per_channel) hipLaunchKernelGGL((KERNEL<TG, T, V, true, ##__VA_ARGS__>), GRID, BLOCK, 0, st, p);      \
+    else hipLaunchKernelGGL((KERNEL<TG, T, V, false, ##__VA_ARGS__>), GRID, BLOCK, 0, st, p);                   \
+  } while (0)
+#define SCAN_PICK(KERNEL, GRID, BLOCK, ...)                                                                  \
+  do {                                                                                                       \
+    if (type == NOF_TYPE_F32) SCAN_GO(KERNEL, GRID, BLOCK, float, float, 1, ##__VA_ARGS__);                    \
+    else if (type == NOF_TYPE_BF16 && gate_type == type) {                                                   \
+      if (v == 2) SCAN_GO(KERNEL, GRID, BLOCK, __bf16, __bf16, 2, ##__VA_ARGS__);                              \
+      else SCAN_GO(KERNEL, GRID, BLOCK, __bf16, __bf16, 1, ##__VA_ARGS__);                                     \
+    } else if (type == NOF_TYPE_BF16) {                                                                      \
+      if (v == 2) SCAN_GO(KERNEL, GRID, BLOCK, float, __bf16, 2, ##__VA_ARGS__);                               \
+      else SCAN_GO(KERNEL, GRID, BLOCK, float, __bf16, 1, ##__VA_ARGS__);                                      \
+    } else if (gate_type == type) {                                                                          \
+      if (v == 2) SCAN_GO(KERNEL, GRID, BLOCK, _Float16, _Float16, 2, ##__VA_ARGS__);                          \
+      else SCAN_GO(KERNEL, GRID, BLOCK, _Float16, _Float16, 1, ##__VA_ARGS__);                                 \
+    } else {                                                                                                 \
+      if (v == 2) SCAN_GO(KERNEL, GRID, BLOCK, float, _Float16, 2, ##__VA_ARGS__);                             \
+      else SCAN_GO(KERNEL, GRID, BLOCK, float, _Float16, 1, ##__VA_ARGS__);                                    \
+    }                                                                                                        \
   } while (0)
 
 static int64_t scan_seg_bytes(const ScanArgs& p) { return p.segs > 1 ? learn_align((int64_t)p.segs * p.B * 2 * p.D * 4) : 0; }
 static int64_t scan_gpart_bytes(const ScanArgs& p) {
-  return !p.per_channel && p.tiles_per_group > 1 ? learn_align((int64_t)p.B * p.T * p.G * p.tiles_per_group * 4) : 0;
+  return !p.per_channel && p.tiles_per_span > 1 ? learn_align((int64_t)p.B * p.T * p.G * p.tiles_per_span * 4) : 0;
 }
 
 extern "C" int64_t nof_gated_scan_marks_bytes(int64_t B, int64_t T, int32_t D, int32_t G, int32_t type) {
   if (!scan_sizes_ok(B, T, D, G) || !learn_type_ok(type)) return -1;
   if (B == 0 || D == 0) return 0;
   ScanArgs p = {};
-  if (!scan_plan(p, B, T, D, G, scan_vec(type, D, G))) return -1;
-  return (int64_t)p.B * p.n_chunks * p.D * 4;
+  if (!scan_plan(p, B, T, D, G, scan_vec(type, D, G), false)) return -1;
+  return (int64_t)p.B * p.n_marks * p.D * 4;
 }
 
 extern "C" int64_t nof_gated_scan_workspace_bytes(int64_t B, int64_t T, int32_t D, int32_t G, int32_t type) {
   if (!scan_sizes_ok(B, T, D, G) || !learn_type_ok(type)) return -1;
   if (B == 0 || D == 0) return 0;
   ScanArgs p = {};
-  if (!scan_plan(p, B, T, D, G, scan_vec(type, D, G))) return -1;
-  return scan_seg_bytes(p) + scan_gpart_bytes(p);
+  if (!scan_plan(p, B, T, D, G, scan_vec(type, D, G), false)) return -1;
+  const int64_t fwd = scan_seg_bytes(p);
+  if (!scan_plan(p, B, T, D, G, scan_vec(type, D, G), true)) return -1;
+  const int64_t bwd = scan_seg_bytes(p) + scan_gpart_bytes(p);
+  return fwd > bwd ? fwd : bwd;
 }
 
 extern "C" int nof_gated_scan_fwd(const void* gate, int64_t gate_sb, int64_t gate_st, int32_t gate_type, const void* value, int64_t value_sb,
@@ -507,7 +559,7 @@ extern "C" int nof_gated_scan_fwd(const void* gate, int64_t gate_sb, int64_t gat
   NOF_ARG((gate && value) || T == 0);
   const int v = scan_vec(type, D, G);
   ScanArgs p = {};
-  NOF_ARG(scan_plan(p, B, T, D, G, v));
+  NOF_ARG(scan_plan(p, B, T, D, G, v, false));
   NOF_ARG(scan_aligned(value, value_sb, value_st, (int)learn_type_size(type), v) && scan_aligned(h, 0, 0, (int)learn_type_size(type), v));
   NOF_ARG(!p.per_channel || scan_aligned(gate, gate_sb, gate_st, (int)learn_type_size(gate_type), v));
   NOF_ARG(scan_aligned(state, 0, 0, 4, v) && scan_aligned(last, 0, 0, 4, v) && scan_aligned(marks, 0, 0, 4, v));
@@ -519,7 +571,7 @@ extern "C" int nof_gated_scan_fwd(const void* gate, int64_t gate_sb, int64_t gat
   p.seg = (float*)workspace;
   hipStream_t st = (hipStream_t)stream;
   const unsigned x = (unsigned)(B * p.tiles);
-  if (p.segs > 1) SCAN_PICK(k_scan_segments, dim3(x, p.segs - 1), dim3(64 * p.waves), , false);
+  if (p.segs > 1) SCAN_PICK(k_scan_segments, dim3(x, p.segs - 1), dim3(64 * p.waves), false);
   SCAN_PICK(k_scan_fwd, dim3(x, p.segs), dim3(64 * p.waves));
   NOF_LAUNCH_OK();
   return 0;
@@ -535,7 +587,7 @@ extern "C" int nof_gated_scan_bwd(const void* gate, int64_t gate_sb, int64_t gat
   NOF_ARG((gate && value && dh && marks && dgate && dvalue) || T == 0);
   const int v = scan_vec(type, D, G), size = (int)learn_type_size(type), gsize = (int)learn_type_size(gate_type);
   ScanArgs p = {};
-  NOF_ARG(scan_plan(p, B, T, D, G, v));
+  NOF_ARG(scan_plan(p, B, T, D, G, v, true));
   NOF_ARG(scan_aligned(value, value_sb, value_st, size, v) && scan_aligned(dh, dh_sb, dh_st, size, v) && scan_aligned(dvalue, 0, 0, size, v));
   NOF_ARG(!p.per_channel || (scan_aligned(gate, gate_sb, gate_st, gsize, v) && scan_aligned(dgate, 0, 0, gsize, v)));
   NOF_ARG(scan_aligned(dlast, 0, 0, 4, v) && scan_aligned(dstate, 0, 0, 4, v) && scan_aligned(marks, 0, 0, 4, v));
@@ -550,14 +602,14 @@ extern "C" int nof_gated_scan_bwd(const void* gate, int64_t gate_sb, int64_t gat
   p.gpart = (float*)((char*)workspace + seg);
   hipStream_t st = (hipStream_t)stream;
   const unsigned x = (unsigned)(B * p.tiles);
-  if (p.segs > 1) SCAN_PICK(k_scan_segments, dim3(x, p.segs - 1), dim3(64 * p.waves), , true);
+  if (p.segs > 1) SCAN_PICK(k_scan_segments, dim3(x, p.segs - 1), dim3(64 * p.waves), true);
   SCAN_PICK(k_scan_bwd, dim3(x, p.segs), dim3(64 * p.waves));
   if (gpart > 0) {
     const int64_t n = B * T * G, blocks = nof_div_up(n, 256);
     const dim3 grid((unsigned)(blocks < 1 << 16 ? blocks : 1 << 16));
-    if (gate_type == NOF_TYPE_F32) hipLaunchKernelGGL(k_scan_gate_sum<float>, grid, dim3(256), 0, st, (const float*)p.gpart, (float*)dgate, n, p.tiles_per_group);
-    else if (gate_type == NOF_TYPE_BF16) hipLaunchKernelGGL(k_scan_gate_sum<__bf16>, grid, dim3(256), 0, st, (const float*)p.gpart, (__bf16*)dgate, n, p.tiles_per_group);
-    else hipLaunchKernelGGL(k_scan_gate_sum<_Float16>, grid, dim3(256), 0, st, (const float*)p.gpart, (_Float16*)dgate, n, p.tiles_per_group);
+    if (gate_type == NOF_TYPE_F32) hipLaunchKernelGGL(k_scan_gate_sum<float>, grid, dim3(256), 0, st, (const float*)p.gpart, (float*)dgate, n, p.tiles_per_span);
+    else if (gate_type == NOF_TYPE_BF16) hipLaunchKernelGGL(k_scan_gate_sum<__bf16>, grid, dim3(256), 0, st, (const float*)p.gpart, (__bf16*)dgate, n, p.tiles_per_span);
+    else hipLaunchKernelGGL(k_scan_gate_sum<_Float16>, grid, dim3(256), 0, st, (const float*)p.gpart, (_Float16*)dgate, n, p.tiles_per_span);
   }
   NOF_LAUNCH_OK();
   return 0;

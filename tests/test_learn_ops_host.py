@@ -136,4 +136,4 @@ def test_orthogonalize_entry_point_refuses():
         assert call(**bad) < 0 and b'argument check' in so.nof_last_error(), bad
     assert call(batch=0) == 0 and call(m=0) == 0 and call(n=0) == 0
     assert so.nof_orthogonalize_workspace_bytes(1, 16385, 4) == -1 and so.nof_orthogonalize_workspace_bytes(1, 128, 128) == 0
-    assert so.nof_orthogonalize_workspace_bytes(3, 129, 20) > 3 * 4 * 256 * 256
+    assert so.nof_orthogonalize_workspace_bytes(3, 129, 20) > 3 * 2 * 3 * 129 * 20 * 2
