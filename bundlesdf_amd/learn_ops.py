@@ -23,36 +23,46 @@ _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # NOF_TYP
 _INT64 = {torch.int32: 0, torch.int64: 1}
 
 
-def _need(ok, what):
-    if not ok:
-        raise NofError(what)
-
-
 def _on_device(what, *tensors):
-    """one CUDA device for all of them, no autograd history lost"""
-    dev = None
+    """the index of the one CUDA device of all of them; no autograd history lost.  (These run a few times per call that takes a few
+    microseconds on the GPU: plain loops, integers.)"""
+    dev = -2
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise NofError(f'{what}: tensors must be on the GPU')
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise NofError(f'{what}: tensors are on different devices ({dev}, {t.device})')
+        d = t.get_device()
+        if d != dev:
+            if d < 0:
+                raise NofError(f'{what}: tensors must be on the GPU')
+            if dev >= 0:
+                raise NofError(f'{what}: tensors are on different devices (cuda:{dev}, cuda:{d})')
+            dev = d
         if t.requires_grad and torch.is_grad_enabled():
             raise NofError(f'{what} records no autograd history: call it under torch.no_grad() or with detached tensors, '
                            'and its gradient function for the gradients')
     return dev
 
 
+_fn = {}
+_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)     # (no Stream object)
+
+
 def _call(dev, name, *args):
-    """the C call on the current stream of `dev`, whichever device is current"""
-    if dev.index == torch.cuda.current_device():
-        lib.call(name, *args)
+    """the C call (addresses and numbers) on the current stream of device `dev`, whichever device is current"""
+    fn = _fn.get(name)
+    if fn is None:
+        fn = _fn[name] = getattr(lib.load(), name)
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
-            lib.call(name, *args)
+            rc = fn(*args, _stream(dev))
+    if rc != 0:
+        raise NofError(f'{name} failed with code {rc}: {lib.load().nof_last_error().decode()}')
+
+
+def _at(x):
+    return None if x is None else x.data_ptr()
 
 
 def _rows(x):
@@ -62,18 +72,33 @@ def _rows(x):
     return x, x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+@functools.lru_cache(maxsize=1024)
+def _bytes(name, *sizes):
+    """a size query of the library: of the sizes alone"""
+    n = getattr(lib.load(), name)(*sizes)
+    if not (n >= 0):
+        raise NofError(f'{name}: sizes out of range {sizes}')
+    return n
+
+
+def _scratch(like, nbytes):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
 # ---- rows of a table ------------------------------------------------------------------------------------------------------------------
 def embed_lookup(table, ids, scale=1.0):
     """table [V, D], ids int32 or int64 of any shape -> scale * table[ids], [*ids.shape, D] in the table's type.  An id outside [0, V)
     -- padding, a ray without a frame -- gives zeros."""
-    _need(table.dim() == 2 and table.dtype in _TYPE, 'embed_lookup: table must be [V, D] float32, bfloat16 or float16')
-    _need(ids.dtype in _INT64, 'embed_lookup: ids must be int32 or int64')
-    dev = _on_device('embed_lookup', table, ids)
+    if not (table.dim() == 2 and table.dtype in _TYPE):
+        raise NofError('embed_lookup: table must be [V, D] float32, bfloat16 or float16')
+    if not (ids.dtype in _INT64):
+        raise NofError('embed_lookup: ids must be int32 or int64')
+    dev, scale = _on_device('embed_lookup', table, ids), float(scale)
     table, stride = _rows(table)
     ids = ids.contiguous()
     V, D = table.shape
-    out = torch.empty((*ids.shape, D), dtype=table.dtype, device=dev)
-    _call(dev, 'nof_embed_fwd', table.data_ptr(), stride, _TYPE[table.dtype], ids, _INT64[ids.dtype], float(scale), out, ids.numel(), V, D)
+    out = table.new_empty((*ids.shape, D))
+    _call(dev, 'nof_embed_fwd', table.data_ptr(), stride, _TYPE[table.dtype], ids.data_ptr(), _INT64[ids.dtype], scale, out.data_ptr(), ids.numel(), V, D)
     return out
 
 
@@ -82,19 +107,23 @@ def embed_lookup_grad(dout, ids, n_rows, scale=1.0):
     ids = v (zeros where nobody asks for v; ids outside [0, n_rows) contribute nothing).  The sum's order depends on the ids alone:
     equal inputs give equal bits."""
     n_rows = int(n_rows)
-    _need(dout.dtype in _TYPE, 'embed_lookup_grad: dout must be float32, bfloat16 or float16')
-    _need(ids.dtype in _INT64, 'embed_lookup_grad: ids must be int32 or int64')
-    _need(dout.dim() >= 1 and dout.shape[:-1] == ids.shape, 'embed_lookup_grad: dout must be [*ids.shape, D]')
-    _need(0 <= n_rows < 1 << 30, 'embed_lookup_grad: n_rows must be in [0, 2^30)')
-    dev = _on_device('embed_lookup_grad', dout, ids)
+    if not (dout.dtype in _TYPE):
+        raise NofError('embed_lookup_grad: dout must be float32, bfloat16 or float16')
+    if not (ids.dtype in _INT64):
+        raise NofError('embed_lookup_grad: ids must be int32 or int64')
+    if not (dout.dim() >= 1 and dout.shape[:-1] == ids.shape):
+        raise NofError('embed_lookup_grad: dout must be [*ids.shape, D]')
+    if not (0 <= n_rows < 1 << 30):
+        raise NofError('embed_lookup_grad: n_rows must be in [0, 2^30)')
+    dev, scale = _on_device('embed_lookup_grad', dout, ids), float(scale)
     N, D = ids.numel(), dout.shape[-1]
     dout, stride = _rows(dout.reshape(N, D))
     ids = ids.contiguous()
-    grad = torch.empty((n_rows, D), dtype=dout.dtype, device=dev)
-    nbytes = lib.load().nof_embed_bwd_workspace_bytes(N, n_rows, D)
-    _need(nbytes >= 0, f'embed_lookup_grad: sizes out of range (N = {N}, n_rows = {n_rows}, D = {D})')
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    _call(dev, 'nof_embed_bwd', dout.data_ptr(), stride, _TYPE[dout.dtype], ids, _INT64[ids.dtype], float(scale), grad, ws, nbytes, N, n_rows, D)
+    grad = dout.new_empty((n_rows, D))
+    nbytes = _bytes('nof_embed_bwd_workspace_bytes', N, n_rows, D)
+    ws = _scratch(dout, nbytes)
+    _call(dev, 'nof_embed_bwd', dout.data_ptr(), stride, _TYPE[dout.dtype], ids.data_ptr(), _INT64[ids.dtype], scale, grad.data_ptr(), _at(ws), nbytes,
+          N, n_rows, D)
     return grad
 
 
@@ -105,38 +134,48 @@ def _scan_even(dtype, D, G):
 
 
 def _scan_strided(x, even):
-    """x [B, T, C] (or [B, C]) as the kernels take it: channels side by side, two-channel loads on their border"""
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    """x [B, T, C] (or [B, C]) as the kernels take it -- channels side by side, two-channel loads on their border -- and its strides"""
+    st = x.stride()
+    if st[-1] != 1 and x.shape[-1] > 1:
         x = x.contiguous()
-    if even and (x.data_ptr() % (2 * x.element_size()) or any(s % 2 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1)):
+        st = x.stride()
+    st = tuple([s if n > 1 else 0 for s, n in zip(st[:-1], x.shape)])
+    if even and (x.data_ptr() % (2 * x.element_size()) or any([s % 2 for s in st])):
         x = x.clone(memory_format=torch.contiguous_format)
-    return x
+        st = tuple([s if n > 1 else 0 for s, n in zip(x.stride()[:-1], x.shape)])
+    return x, st
 
 
-def _scan_strides(x):
-    return tuple(s if n > 1 else 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]))
+def _flat(x, even):
+    """a [B, D] float32 argument as the kernels take it, or None"""
+    if x is None:
+        return None
+    x = x.contiguous()
+    return x.clone() if even and x.data_ptr() % 8 else x
 
 
 def _state_ok(what, name, x, B, D):
-    _need(x is None or (x.dtype == torch.float32 and x.shape == (B, D)), f'{what}: {name} must be [B, D] float32')
+    if not (x is None or (x.dtype == torch.float32 and x.shape == (B, D))):
+        raise NofError(f'{what}: {name} must be [B, D] float32')
 
 
 def _scan_args(what, gate, value, lengths, dims):
-    _need(value.dim() == dims and value.dtype in _TYPE, f'{what}: value must be [{"B, T, D" if dims == 3 else "B, D"}] float32, bfloat16 or float16')
-    _need(gate.dim() == dims and gate.shape[:-1] == value.shape[:-1], f"{what}: gate must have value's shape but for the channels")
-    _need(gate.dtype in (value.dtype, torch.float32), f"{what}: gate must be float32 or of value's type")
-    D, G = value.shape[-1], gate.shape[-1]
-    _need(D == 0 or (G > 0 and D % G == 0), f'{what}: the number of gates per position must divide the number of channels')
-    _need(D <= 1 << 20 and value.shape[0] < 1 << 24 and (dims == 2 or value.shape[1] < 1 << 31), f'{what}: sizes out of range')
+    vs, gs = value.shape, gate.shape
+    if not (len(vs) == dims and value.dtype in _TYPE):
+        raise NofError(f'{what}: value must be [{"B, T, D" if dims == 3 else "B, D"}] float32, bfloat16 or float16')
+    if not (len(gs) == dims and gs[:-1] == vs[:-1]):
+        raise NofError(f"{what}: gate must have value's shape but for the channels")
+    if not (gate.dtype is value.dtype or gate.dtype is torch.float32):
+        raise NofError(f"{what}: gate must be float32 or of value's type")
+    D, G = vs[-1], gs[-1]
+    if not (D == 0 or (G > 0 and D % G == 0)):
+        raise NofError(f'{what}: the number of gates per position must divide the number of channels')
+    if not (D <= 1 << 20 and vs[0] < 1 << 24 and (dims == 2 or vs[1] < 1 << 31)):
+        raise NofError(f'{what}: sizes out of range')
     if lengths is not None:
-        _need(lengths.dtype == torch.int32 and lengths.shape == value.shape[:1], f'{what}: lengths must be [B] int32')
+        if not (lengths.dtype == torch.int32 and lengths.shape == vs[:1]):
+            raise NofError(f'{what}: lengths must be [B] int32')
     return D, G
-
-
-def _scan_bytes(kind, B, T, D, G, dtype):
-    n = getattr(lib.load(), f'nof_gated_scan_{kind}_bytes')(B, T, D, G, _TYPE[dtype])
-    _need(n >= 0, f'gated_scan: sizes out of range (B = {B}, T = {T}, D = {D}, G = {G})')
-    return n
 
 
 def gated_scan(gate, value, state=None, lengths=None, reverse=False, want_marks=False):
@@ -156,19 +195,17 @@ def gated_scan(gate, value, state=None, lengths=None, reverse=False, want_marks=
 
 def _scan_forward(dev, gate, value, state, lengths, reverse, want_marks, want_h):
     B, T, D = value.shape
-    G = gate.shape[-1]
-    dt = value.dtype
-    even = _scan_even(dt, D, G)
-    value, gate = _scan_strided(value, even), _scan_strided(gate, even and G == D)
-    state = _scan_strided(state.contiguous(), even) if state is not None else None
+    G, dt = gate.shape[-1], value.dtype
+    even, ty = _scan_even(dt, D, G), _TYPE[dt]
+    (value, vst), (gate, gst), state = _scan_strided(value, even), _scan_strided(gate, even and G == D), _flat(state, even)
     lengths = lengths.contiguous() if lengths is not None else None
-    h = torch.empty((B, T, D), dtype=dt, device=dev) if want_h else None
-    last = torch.empty((B, D), dtype=torch.float32, device=dev) if want_h else None
-    marks = torch.empty(_scan_bytes('marks', B, T, D, G, dt) // 4, dtype=torch.float32, device=dev) if want_marks else None
-    nbytes = _scan_bytes('workspace', B, T, D, G, dt)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call(dev, 'nof_gated_scan_fwd', gate.data_ptr(), *_scan_strides(gate), _TYPE[gate.dtype], value.data_ptr(), *_scan_strides(value), _TYPE[dt],
-          state, lengths, int(bool(reverse)), h, last, marks, ws, nbytes, B, T, D, G)
+    h = value.new_empty((B, T, D)) if want_h else None
+    last = value.new_empty((B, D), dtype=torch.float32) if want_h else None
+    marks = value.new_empty(_bytes('nof_gated_scan_marks_bytes', B, T, D, G, ty) // 4, dtype=torch.float32) if want_marks else None
+    nbytes = _bytes('nof_gated_scan_workspace_bytes', B, T, D, G, ty)
+    ws = _scratch(value, nbytes)
+    _call(dev, 'nof_gated_scan_fwd', gate.data_ptr(), *gst, _TYPE[gate.dtype], value.data_ptr(), *vst, ty, _at(state), _at(lengths),
+          1 if reverse else 0, _at(h), _at(last), _at(marks), _at(ws), nbytes, B, T, D, G)
     return (h, last, marks) if want_marks else (h, last)
 
 
@@ -179,26 +216,25 @@ def gated_scan_grad(gate, value, dh, dlast=None, state=None, marks=None, lengths
     D, G = _scan_args('gated_scan_grad', gate, value, lengths, 3)
     B, T = value.shape[:2]
     dt = value.dtype
-    _need(dh.shape == value.shape and dh.dtype == dt, "gated_scan_grad: dh must have value's shape and type")
+    if not (dh.shape == value.shape and dh.dtype == dt):
+        raise NofError("gated_scan_grad: dh must have value's shape and type")
     _state_ok('gated_scan_grad', 'state', state, B, D)
     _state_ok('gated_scan_grad', 'dlast', dlast, B, D)
     if marks is not None:
-        _need(marks.dtype == torch.float32 and marks.dim() == 1 and marks.numel() * 4 == _scan_bytes('marks', B, T, D, G, dt),
-              'gated_scan_grad: marks are not those of a forward pass of these sizes')
+        if not (marks.dtype == torch.float32 and marks.dim() == 1 and marks.numel() * 4 == _bytes('nof_gated_scan_marks_bytes', B, T, D, G, _TYPE[dt])):
+            raise NofError('gated_scan_grad: marks are not those of a forward pass of these sizes')
     dev = _on_device('gated_scan_grad', gate, value, dh, dlast, state, marks, lengths)
     if marks is None:
         marks = _scan_forward(dev, gate, value, state, lengths, reverse, True, False)[2]
-    even = _scan_even(dt, D, G)
-    value, gate, dh = _scan_strided(value, even), _scan_strided(gate, even and G == D), _scan_strided(dh, even)
-    dlast = _scan_strided(dlast.contiguous(), even) if dlast is not None else None
+    even, ty = _scan_even(dt, D, G), _TYPE[dt]
+    (value, vst), (gate, gst), (dh, dst) = _scan_strided(value, even), _scan_strided(gate, even and G == D), _scan_strided(dh, even)
+    dlast, marks = _flat(dlast, even), _flat(marks, even)
     lengths = lengths.contiguous() if lengths is not None else None
-    dgate = torch.empty((B, T, G), dtype=gate.dtype, device=dev)
-    dvalue = torch.empty((B, T, D), dtype=dt, device=dev)
-    dstate = torch.empty((B, D), dtype=torch.float32, device=dev)
-    nbytes = _scan_bytes('workspace', B, T, D, G, dt)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call(dev, 'nof_gated_scan_bwd', gate.data_ptr(), *_scan_strides(gate), _TYPE[gate.dtype], value.data_ptr(), *_scan_strides(value), _TYPE[dt],
-          dh.data_ptr(), *_scan_strides(dh), dlast, marks.contiguous(), lengths, int(bool(reverse)), dgate, dvalue, dstate, ws, nbytes, B, T, D, G)
+    dgate, dvalue, dstate = gate.new_empty((B, T, G)), value.new_empty((B, T, D)), value.new_empty((B, D), dtype=torch.float32)
+    nbytes = _bytes('nof_gated_scan_workspace_bytes', B, T, D, G, ty)
+    ws = _scratch(value, nbytes)
+    _call(dev, 'nof_gated_scan_bwd', gate.data_ptr(), *gst, _TYPE[gate.dtype], value.data_ptr(), *vst, ty, dh.data_ptr(), *dst, _at(dlast),
+          marks.data_ptr(), _at(lengths), 1 if reverse else 0, dgate.data_ptr(), dvalue.data_ptr(), dstate.data_ptr(), _at(ws), nbytes, B, T, D, G)
     return dgate, dvalue, dstate
 
 
@@ -207,20 +243,23 @@ def gated_scan_step(gate, value, state, new_state=None):
     new_state: where the new state goes (`state` itself for an update in place); None allocates it."""
     D, G = _scan_args('gated_scan_step', gate, value, None, 2)
     B = value.shape[0]
-    _need(state is not None, 'gated_scan_step: state must be [B, D] float32')
+    if not (state is not None):
+        raise NofError('gated_scan_step: state must be [B, D] float32')
     _state_ok('gated_scan_step', 'state', state, B, D)
     _state_ok('gated_scan_step', 'new_state', new_state, B, D)
     dev = _on_device('gated_scan_step', gate, value, state, new_state)
-    _need(new_state is None or new_state.is_contiguous(), 'gated_scan_step: new_state must be contiguous')
-    even = _scan_even(value.dtype, D, G)
-    value, gate = _scan_strided(value, even), _scan_strided(gate, even and G == D)
-    state = _scan_strided(state.contiguous(), even)
-    _need(new_state is None or not even or new_state.data_ptr() % 8 == 0, 'gated_scan_step: new_state must start on an 8-byte border')
+    if not (new_state is None or new_state.is_contiguous()):
+        raise NofError('gated_scan_step: new_state must be contiguous')
+    dt = value.dtype
+    even = _scan_even(dt, D, G)
+    (value, vst), (gate, gst), state = _scan_strided(value, even), _scan_strided(gate, even and G == D), _flat(state, even)
     if new_state is None:
-        new_state = torch.empty((B, D), dtype=torch.float32, device=dev)
-    h = torch.empty((B, D), dtype=value.dtype, device=dev)
-    _call(dev, 'nof_gated_scan_step', gate.data_ptr(), *_scan_strides(gate), _TYPE[gate.dtype], value.data_ptr(), *_scan_strides(value),
-          _TYPE[value.dtype], state, new_state, h, B, D, G)
+        new_state = state.new_empty((B, D))
+    elif even and new_state.data_ptr() % 8:
+        raise NofError('gated_scan_step: new_state must start on an 8-byte border')
+    h = value.new_empty((B, D))
+    _call(dev, 'nof_gated_scan_step', gate.data_ptr(), *gst, _TYPE[gate.dtype], value.data_ptr(), *vst, _TYPE[dt], state.data_ptr(),
+          new_state.data_ptr(), h.data_ptr(), B, D, G)
     return h, new_state
 
 
@@ -231,8 +270,10 @@ QUINTIC = (3.4445, -4.7750, 2.0315)     # steep at 0 (a small singular value gro
 @functools.lru_cache(maxsize=64)
 def _coefficients(steps, coefficients):
     flat = coefficients if isinstance(coefficients[0], (tuple, list)) else (coefficients,) * steps
-    _need(1 <= steps <= 32, 'orthogonalize: steps must be in [1, 32]')
-    _need(len(flat) == steps and all(len(c) == 3 for c in flat), 'orthogonalize: coefficients must be (a, b, c) or one such triple per step')
+    if not (1 <= steps <= 32):
+        raise NofError('orthogonalize: steps must be in [1, 32]')
+    if not (len(flat) == steps and all(len(c) == 3 for c in flat)):
+        raise NofError('orthogonalize: coefficients must be (a, b, c) or one such triple per step')
     return (C.c_float * (3 * steps))(*[float(x) for c in flat for x in c])
 
 
@@ -241,19 +282,22 @@ def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-30, out=None):
     X <- (a + b A + c A A) X, A = X X^T (over the shorter side), with coefficients (a, b, c) -- one triple, or a tuple of `steps` of them.
     The singular vectors stay, the singular values go to the quintic's fixed band around 1.  Result in the update's type, in `out` (which
     may be `update`) where given.  Coefficients that let a singular value leave [0, 2] are refused."""
-    _need(update.dim() >= 2 and update.dtype in _TYPE, 'orthogonalize: update must be [..., m, n] float32, bfloat16 or float16')
+    if not (update.dim() >= 2 and update.dtype in _TYPE):
+        raise NofError('orthogonalize: update must be [..., m, n] float32, bfloat16 or float16')
     m, n = update.shape[-2:]
-    _need(m <= 16384 and n <= 16384, 'orthogonalize: m and n must be at most 16384')
+    if not (m <= 16384 and n <= 16384):
+        raise NofError('orthogonalize: m and n must be at most 16384')
     batch = update.shape[:-2].numel()
-    _need(batch < 65536, 'orthogonalize: at most 65535 matrices')
+    if not (batch < 65536):
+        raise NofError('orthogonalize: at most 65535 matrices')
     coef = _coefficients(int(steps), tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients))
-    _need(out is None or (out.shape == update.shape and out.dtype == update.dtype and out.is_contiguous()),
-          "orthogonalize: out must be contiguous, of update's shape and type")
+    if not (out is None or (out.shape == update.shape and out.dtype == update.dtype and out.is_contiguous())):
+        raise NofError("orthogonalize: out must be contiguous, of update's shape and type")
     dev = _on_device('orthogonalize', update, out)
     update = update.contiguous()
     if out is None:
-        out = torch.empty(update.shape, dtype=update.dtype, device=dev)
-    nbytes = lib.load().nof_orthogonalize_workspace_bytes(batch, m, n)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call(dev, 'nof_orthogonalize', update, out, _TYPE[update.dtype], int(steps), coef, float(eps), ws, nbytes, batch, m, n)
+        out = update.new_empty(update.shape)
+    nbytes = _bytes('nof_orthogonalize_workspace_bytes', batch, m, n)
+    ws = _scratch(update, nbytes)
+    _call(dev, 'nof_orthogonalize', update.data_ptr(), out.data_ptr(), _TYPE[update.dtype], int(steps), coef, float(eps), _at(ws), nbytes, batch, m, n)
     return out
