@@ -5,7 +5,7 @@
 //
 // Both are bound by memory: the rows read and written once each.  The gradient adds in a fixed order, so equal inputs give equal
 // bits (the hash table's scatter beside it, nof_hash.hip, adds with atomics):
-//   1. a stable radix sort of (id, position): k_embed_hist + one k_embed_scatter per digit, or k_embed_sort_small as one workgroup;
+//   1. a stable radix sort of (id, position): one k_embed_hist + k_embed_scatter per digit, or k_embed_sort_small as one workgroup;
 //   2. k_embed_reduce: a group of lanes owns a run of C sorted positions and one slice of the columns, reads the rows of dout behind
 //      them and writes the sum of every id that lies within the run; an id cut by the run's ends leaves a partial sum.  Further
 //      workgroups of the same launch write the zeros of the rows that no id names -- most of the bytes of a large table;
@@ -71,47 +71,49 @@ struct EmbSort {
   int n_blocks, passes, bits;
 };
 
-// hist[block][digit] of the first pass; clears the histograms of the later ones, which the scatter before each fills
-__global__ __launch_bounds__(EMB_SORT_T) void k_embed_hist(EmbSort s, uint32_t* __restrict__ hist) {
+// hist[block][digit] of a pass.  (Counted with atomics by the scatter before instead, an id that many positions hold is one address:
+// 15 us for 8192 positions against 8 + 3.)
+__global__ __launch_bounds__(EMB_SORT_T) void k_embed_hist(EmbSort s, int pass, const uint32_t* __restrict__ key_in, uint32_t* __restrict__ hist) {
   __shared__ uint32_t cnt[1 << EMB_BITS];
-  const int bins = 1 << s.bits;
+  const int bins = 1 << s.bits, shift = pass * s.bits;
   for (int d = threadIdx.x; d < bins; d += EMB_SORT_T) cnt[d] = 0;
   __syncthreads();
   const uint32_t lo = blockIdx.x * s.per, hi = lo + s.per < s.N ? lo + s.per : s.N;
-  for (uint32_t i = lo + threadIdx.x; i < hi; i += EMB_SORT_T) atomicAdd(&cnt[emb_key(s.ids, s.ids64, i, s.rows) & (bins - 1)], 1u);
-  __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += EMB_SORT_T) {
-    hist[blockIdx.x * bins + d] = cnt[d];
-    for (int p = 1; p < s.passes; ++p) hist[((size_t)p * s.n_blocks + blockIdx.x) * bins + d] = 0;
+  for (uint32_t i = lo + threadIdx.x; i < hi; i += EMB_SORT_T) {
+    const uint32_t k = pass == 0 ? emb_key(s.ids, s.ids64, i, s.rows) : key_in[i];
+    atomicAdd(&cnt[(k >> shift) & (bins - 1)], 1u);
   }
+  __syncthreads();
+  for (int d = threadIdx.x; d < bins; d += EMB_SORT_T) hist[blockIdx.x * bins + d] = cnt[d];
 }
 
 // One digit: a workgroup knows where its keys go from the histogram of all workgroups (at most EMB_MAX_BLOCKS * 4 KiB, from L2), a
 // wave from the counts of the waves before it, a lane from its rank among the equal digits of its wave: no order is left to chance.
 __global__ __launch_bounds__(EMB_SORT_T) void k_embed_scatter(EmbSort s, int pass, const uint32_t* __restrict__ key_in,
                                                               const uint32_t* __restrict__ pos_in, uint32_t* __restrict__ key_out,
-                                                              uint32_t* __restrict__ pos_out, uint32_t* __restrict__ hist) {
+                                                              uint32_t* __restrict__ pos_out, const uint32_t* __restrict__ hist) {
   __shared__ uint32_t cnt[EMB_SORT_W][1 << EMB_BITS];
   __shared__ uint32_t wsum[EMB_SORT_W];
   const int bins = 1 << s.bits, shift = pass * s.bits, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const uint32_t lo = blockIdx.x * s.per, hi = lo + s.per < s.N ? lo + s.per : s.N, per_wave = s.per / EMB_SORT_W;
   const uint32_t wlo = lo + w * per_wave < hi ? lo + w * per_wave : hi, whi = wlo + per_wave < hi ? wlo + per_wave : hi;
-  for (int d = threadIdx.x; d < bins * EMB_SORT_W; d += EMB_SORT_T) cnt[d / bins][d % bins] = 0;
+  for (int d = threadIdx.x; d < bins * EMB_SORT_W; d += EMB_SORT_T) cnt[d >> s.bits][d & (bins - 1)] = 0;
   __syncthreads();
   for (uint32_t i = wlo + lane; i < whi; i += 64) {
     const uint32_t k = pass == 0 ? emb_key(s.ids, s.ids64, i, s.rows) : key_in[i];
     atomicAdd(&cnt[w][(k >> shift) & (bins - 1)], 1u);
   }
   // digits 2t and 2t + 1 are thread t's (bins <= 2 * EMB_SORT_T): totals over all workgroups, and over those before this one
-  const uint32_t* h = hist + (size_t)pass * s.n_blocks * bins;
   uint32_t tot[2] = {0, 0}, before[2] = {0, 0};
   const int d0 = 2 * threadIdx.x;
-  if (d0 < bins)
+  if (d0 < bins) {
+#pragma unroll 16                        // (sixteen loads in flight: one at a time is a trip to L2 per workgroup of the sort)
     for (int b = 0; b < s.n_blocks; ++b) {
-      const uint2 x = *reinterpret_cast<const uint2*>(h + (size_t)b * bins + d0);
+      const uint2 x = *reinterpret_cast<const uint2*>(hist + (size_t)b * bins + d0);
       tot[0] += x.x; tot[1] += x.y;
       if (b < (int)blockIdx.x) { before[0] += x.x; before[1] += x.y; }
     }
+  }
   uint32_t run = tot[0] + tot[1];
   for (int o = 1; o < 64; o <<= 1) {
     const uint32_t y = __shfl_up(run, o);
@@ -152,7 +154,6 @@ __global__ __launch_bounds__(EMB_SORT_T) void k_embed_scatter(EmbSort s, int pas
       const uint32_t to = old + (uint32_t)__popcll(same & (((uint64_t)1 << lane) - 1));
       key_out[to] = k;
       pos_out[to] = p;
-      if (pass + 1 < s.passes) atomicAdd(&hist[((size_t)(pass + 1) * s.n_blocks + to / s.per) * bins + ((k >> (shift + s.bits)) & (bins - 1))], 1u);
     }
   }
 }
@@ -272,7 +273,7 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
   float acc[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = 0.0f;
-  constexpr int U = 4;
+  constexpr int U = 8;                                                // rows in flight per group
   for (uint32_t i = lo; i < hi; i += U) {
     uint32_t kk[U];
     float x[U][V];
@@ -306,7 +307,8 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
   else emb_put<T, V>(grad, cur, D, col, scale, acc);
 }
 
-// the run in which a cut id starts adds what the runs behind it inherited
+// the run in which a cut id starts adds what the runs behind it inherited.  At most a wave a row and four columns a lane: an id that many
+// runs hold is one chain of loads, and its columns spread over compute units
 template <typename T, int V>
 __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict__ key, uint32_t N, uint32_t rows, int D, float scale,
                                                       T* __restrict__ grad, const float* __restrict__ part, int ls, int C) {
@@ -321,7 +323,7 @@ __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict
   const uint32_t last = (emb_lower(key + end, (uint32_t)(N - end), id + 1) + (uint32_t)end - 1) / C;    // the run that it ends in
   float acc[V], x[V];
   lload<float, V>(part + ((size_t)chunk * 2 + 1) * D + col, acc);
-#pragma unroll 4
+#pragma unroll 8
   for (uint32_t c = chunk + 1; c <= last; ++c) {
     lload<float, V>(part + ((size_t)c * 2) * D + col, x);
 #pragma unroll
@@ -362,7 +364,7 @@ static EmbPlan emb_plan(int64_t N, int64_t rows, int32_t D) {
     p.key[k] = at; at += learn_align(4 * N);
     p.pos[k] = at; at += learn_align(4 * N);
   }
-  p.hist = at; at += learn_align(p.small ? 0 : (int64_t)4 * p.s.passes * p.s.n_blocks << p.s.bits);
+  p.hist = at; at += learn_align(p.small ? 0 : (int64_t)4 * p.s.n_blocks << p.s.bits);
   p.part = at; at += learn_align((int64_t)p.chunks * 2 * D * 4);
   p.bytes = at;
   return p;
@@ -408,9 +410,13 @@ static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* ke
   const unsigned n_zero = (unsigned)nof_div_up(p.s.rows, EMB_ZROWS);
   hipLaunchKernelGGL((k_embed_reduce<T, V>), dim3(n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N,
                      (uint32_t)p.s.rows, D, scale, (T*)grad, part, ls, p.C, n_red);
-  if (p.chunks > 1)
-    hipLaunchKernelGGL((k_embed_join<T, V>), dim3(n_red, cols), dim3(EMB_T), 0, st, key, p.s.N, (uint32_t)p.s.rows, D, scale, (T*)grad,
-                       (const float*)part, ls, p.C);
+  if (p.chunks > 1) {
+    constexpr int JV = V > 4 ? 4 : V;
+    const int64_t jv = D / JV;
+    const int jl = learn_log2_up(jv < 64 ? jv : 64);
+    hipLaunchKernelGGL((k_embed_join<T, JV>), dim3((unsigned)nof_div_up(p.chunks, EMB_T >> jl), (unsigned)nof_div_up(jv, (int64_t)1 << jl)), dim3(EMB_T), 0, st,
+                       key, p.s.N, (uint32_t)p.s.rows, D, scale, (T*)grad, (const float*)part, jl, p.C);
+  }
 }
 
 extern "C" int nof_embed_fwd(const void* table, int64_t table_stride, int32_t type, const void* ids, int32_t ids64, float scale, void* out,
@@ -452,10 +458,11 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
     if (p.small) {
       hipLaunchKernelGGL(k_embed_sort_small, dim3(1), dim3(1024), 0, st, ids, (int)ids64, V, (int)N, p.s.passes, key[0], pos[0]);
     } else {
-      hipLaunchKernelGGL(k_embed_hist, dim3(p.s.n_blocks), dim3(EMB_SORT_T), 0, st, p.s, hist);
-      for (int pass = 0; pass < p.s.passes; ++pass, cur ^= 1)
+      for (int pass = 0; pass < p.s.passes; ++pass, cur ^= 1) {
+        hipLaunchKernelGGL(k_embed_hist, dim3(p.s.n_blocks), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur], hist);
         hipLaunchKernelGGL(k_embed_scatter, dim3(p.s.n_blocks), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur],
-                           (const uint32_t*)pos[cur], key[cur ^ 1], pos[cur ^ 1], hist);
+                           (const uint32_t*)pos[cur], key[cur ^ 1], pos[cur ^ 1], (const uint32_t*)hist);
+      }
     }
     NOF_LAUNCH_OK();
   }
