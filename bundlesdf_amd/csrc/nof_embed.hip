@@ -25,24 +25,47 @@ __device__ __forceinline__ int64_t emb_id(const void* __restrict__ ids, int ids6
   return ids64 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
 }
 
+// 16 bytes of a row per access, wherever the row starts: gfx950 takes them at any border, and rows of odd length would otherwise go one
+// element at a time.  The last access of a row may be short (n < V elements, the others as zeros).
+template <typename T> struct EmbVec { static constexpr int V = 16 / (int)sizeof(T); };
+typedef uint32_t emb_u4 __attribute__((ext_vector_type(4)));
+template <int SIZE> struct EmbAt;
+template <> struct EmbAt<2> { typedef emb_u4 t __attribute__((aligned(2))); };
+template <> struct EmbAt<4> { typedef emb_u4 t __attribute__((aligned(4))); };
+template <typename T> using EmbBits = typename EmbAt<sizeof(T)>::t;
+template <typename T, int V>
+__device__ __forceinline__ void emb_load(const T* __restrict__ p, int n, float (&f)[V]) {
+  if (n >= V) {
+    const emb_u4 bits = *reinterpret_cast<const EmbBits<T>*>(p);
+    const LearnVec<T, V> x = __builtin_bit_cast(LearnVec<T, V>, bits);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = lf(x.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i < n ? lf(p[i]) : 0.0f;
+  }
+}
 // a store past the caches: nothing here reads it again, and the rows that are read stay (65536 x 2048 bf16 looked up: 59 us, 91 without;
 // the gradient of a 131072-row table by them 222 us, 248 without)
-template <typename T, int V> __device__ __forceinline__ void emb_stream(T* __restrict__ p, const float (&f)[V]) {
-  if constexpr (sizeof(T) * V == 16) {
-    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+template <typename T, int V>
+__device__ __forceinline__ void emb_store(T* __restrict__ p, int n, const float (&f)[V]) {
+  if (n >= V) {
     LearnVec<T, V> x;
 #pragma unroll
     for (int i = 0; i < V; ++i) x.v[i] = lt<T>(f[i]);
-    __builtin_nontemporal_store(__builtin_bit_cast(u4, x), reinterpret_cast<u4*>(p));
+    __builtin_nontemporal_store(__builtin_bit_cast(emb_u4, x), reinterpret_cast<EmbBits<T>*>(p));
   } else {
-    lstore<T, V>(p, f);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) p[i] = lt<T>(f[i]);
   }
 }
 
 // 2^ls lanes a row, further columns by blockIdx.y
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(EMB_T) void k_embed_fwd(const T* __restrict__ table, int64_t stride, const void* __restrict__ ids, int ids64,
                                                      float scale, T* __restrict__ out, int64_t N, int64_t rows, int D, int ls) {
+  constexpr int V = EmbVec<T>::V;
   const int lane = threadIdx.x & ((1 << ls) - 1);
   const int col = (((int)blockIdx.y << ls) + lane) * V;
   const int64_t step = (int64_t)gridDim.x * (EMB_T >> ls);
@@ -53,11 +76,11 @@ __global__ __launch_bounds__(EMB_T) void k_embed_fwd(const T* __restrict__ table
 #pragma unroll
     for (int k = 0; k < V; ++k) f[k] = 0.0f;
     if (id >= 0 && id < rows) {
-      lload<T, V>(table + id * stride + col, f);
+      emb_load<T, V>(table + id * stride + col, D - col, f);
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] *= scale;
     }
-    emb_stream<T, V>(out + i * D + col, f);
+    emb_store<T, V>(out + i * D + col, D - col, f);
   }
 }
 
@@ -250,14 +273,16 @@ __device__ __forceinline__ void emb_put(T* __restrict__ grad, int64_t row, int D
   float f[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) f[k] = acc[k] * scale;
-  emb_stream<T, V>(grad + row * D + col, f);
+  emb_store<T, V>(grad + row * D + col, D - col, f);
 }
 
-// part [chunk][2][D]: the sum of the id that a run inherits from the run before it, and of the one that it starts and hands on
-template <typename T, int V>
+// part [chunk][2][DP], DP = D up to a multiple of 8: the sum of the id that a run inherits from the run before it, and of the one that it starts and hands on
+template <typename T>
 __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ dout, int64_t stride, const uint32_t* __restrict__ key,
                                                         const uint32_t* __restrict__ pos, uint32_t N, uint32_t rows, int D, float scale,
                                                         T* __restrict__ grad, float* __restrict__ part, int ls, int C, uint32_t n_red) {
+  constexpr int V = EmbVec<T>::V;
+  const int DP = (D + 7) & ~7;
   const int lane = threadIdx.x & ((1 << ls) - 1);
   const int col = (((int)blockIdx.y << ls) + lane) * V;
   if (blockIdx.x >= n_red) {                                          // the zero role
@@ -274,7 +299,7 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
     for (int k = 0; k < V; ++k) z[k] = 0.0f;
     if (col < D)
       for (int r = threadIdx.x >> ls; r < EMB_ZROWS; r += EMB_T >> ls)
-        if (!named[r]) emb_stream<T, V>(grad + (int64_t)(v0 + r) * D + col, z);
+        if (!named[r]) emb_store<T, V>(grad + (int64_t)(v0 + r) * D + col, D - col, z);
     return;
   }
   const uint32_t chunk = blockIdx.x * (EMB_T >> ls) + (threadIdx.x >> ls);
@@ -294,13 +319,13 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       kk[u] = i + u < hi ? key[i + u] : rows;
-      if (kk[u] < rows) lload<T, V>(dout + (int64_t)pos[i + u] * stride + col, x[u]);
+      if (kk[u] < rows) emb_load<T, V>(dout + (int64_t)pos[i + u] * stride + col, D - col, x[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (kk[u] != cur) {                                             // an id ends here (or the run does: `rows`)
         if (cur < rows && i + u < hi) {
-          if (inherited) lstore<float, V>(part + ((size_t)chunk * 2) * D + col, acc);
+          if (inherited) lstore<float, V>(part + ((size_t)chunk * 2) * DP + col, acc);
           else emb_put<T, V>(grad, cur, D, col, scale, acc);
           inherited = false;
           cur = kk[u];
@@ -316,17 +341,19 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
   }
   if (cur >= rows) return;
   const bool on = hi < N && key[hi] == cur;
-  if (inherited) lstore<float, V>(part + ((size_t)chunk * 2) * D + col, acc);
-  else if (on) lstore<float, V>(part + ((size_t)chunk * 2 + 1) * D + col, acc);
+  if (inherited) lstore<float, V>(part + ((size_t)chunk * 2) * DP + col, acc);
+  else if (on) lstore<float, V>(part + ((size_t)chunk * 2 + 1) * DP + col, acc);
   else emb_put<T, V>(grad, cur, D, col, scale, acc);
 }
 
 // The run in which a cut id starts adds what the runs behind it inherited: a workgroup per run and slice of at most 64 x V columns, whose
 // groups of lanes each add a stretch of the runs; their sums meet in LDS, neighbours first.  (One group for all of an id that many runs hold
 // is a chain of loads: 17 us of the 222 above, 8 so.)
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict__ key, uint32_t N, uint32_t rows, int D, float scale,
                                                       T* __restrict__ grad, const float* __restrict__ part, int ls, int C) {
+  constexpr int V = 4;
+  const int DP = (D + 7) & ~7;
   __shared__ float sums[EMB_T * V];
   const uint32_t chunk = blockIdx.x;
   const uint64_t first = (uint64_t)chunk * C, end = first + C;
@@ -345,10 +372,10 @@ __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = 0.0f;
   if (col < D) {
-    if (group == 0) lload<float, V>(part + ((size_t)chunk * 2 + 1) * D + col, acc);
+    if (group == 0) lload<float, V>(part + ((size_t)chunk * 2 + 1) * DP + col, acc);
 #pragma unroll 4
     for (uint32_t c = c0; c < c1; ++c) {
-      lload<float, V>(part + ((size_t)c * 2) * D + col, x);
+      lload<float, V>(part + ((size_t)c * 2) * DP + col, x);
 #pragma unroll
       for (int k = 0; k < V; ++k) acc[k] += x[k];
     }
@@ -363,7 +390,11 @@ __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict
     }
     __syncthreads();
   }
-  if (group == 0 && col < D) emb_put<T, V>(grad, id, D, col, scale, acc);
+  if (group == 0 && col < D) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (col + k < D) grad[(int64_t)id * D + col + k] = lt<T>(acc[k] * scale);
+  }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
@@ -399,7 +430,7 @@ static EmbPlan emb_plan(int64_t N, int64_t rows, int32_t D) {
     p.pos[k] = at; at += learn_align(4 * N);
   }
   p.hist = at; at += learn_align(p.small ? 0 : (int64_t)4 * p.s.n_blocks << p.s.bits);
-  p.part = at; at += learn_align((int64_t)p.chunks * 2 * D * 4);
+  p.part = at; at += learn_align((int64_t)p.chunks * 2 * ((D + 7) & ~7) * 4);
   p.bytes = at;
   return p;
 }
@@ -408,48 +439,30 @@ static bool emb_sizes_ok(int64_t N, int64_t V, int32_t D) {
   return N >= 0 && N < ((int64_t)1 << 31) - 65536 && V >= 0 && V < (int64_t)1 << 30 && D >= 0 && D <= 1 << 20;
 }
 
-// elements per access: 16 bytes where every row starts on a 16-byte border, else 4, else one element
-static int emb_vec(int32_t type, int32_t D, int64_t stride, const void* a, const void* b) {
-  const int size = (int)learn_type_size(type);
-  for (int v = 16 / size; v > 1; v = v * size == 16 ? 4 / size : 1)
-    if (D % v == 0 && stride % v == 0 && (((uintptr_t)a | (uintptr_t)b) % (uintptr_t)(v * size)) == 0) return v;
-  return 1;
-}
-
-#define EMB_PICK(NAME, ...)                                                                                                    \
-  do {                                                                                                                         \
-    if (type == NOF_TYPE_F32) { if (v == 4) NAME<float, 4>(__VA_ARGS__); else NAME<float, 1>(__VA_ARGS__); }                   \
-    else if (type == NOF_TYPE_BF16) { if (v == 8) NAME<__bf16, 8>(__VA_ARGS__); else if (v == 2) NAME<__bf16, 2>(__VA_ARGS__); \
-                                      else NAME<__bf16, 1>(__VA_ARGS__); }                                                     \
-    else { if (v == 8) NAME<_Float16, 8>(__VA_ARGS__); else if (v == 2) NAME<_Float16, 2>(__VA_ARGS__);                        \
-           else NAME<_Float16, 1>(__VA_ARGS__); }                                                                              \
-  } while (0)
-
-template <typename T, int V>
+template <typename T>
 static void emb_launch_fwd(const void* table, int64_t stride, const void* ids, int ids64, float scale, void* out, int64_t N, int64_t rows,
                            int32_t D, hipStream_t st) {
-  const int64_t nv = D / V;
+  const int64_t nv = nof_div_up(D, EmbVec<T>::V);
   const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
   const int64_t want = nof_div_up(N, EMB_T >> ls), most = (int64_t)1 << 20;
-  hipLaunchKernelGGL((k_embed_fwd<T, V>), dim3((unsigned)(want < most ? want : most), (unsigned)nof_div_up(nv, (int64_t)1 << ls)), dim3(EMB_T), 0, st,
+  hipLaunchKernelGGL(k_embed_fwd<T>, dim3((unsigned)(want < most ? want : most), (unsigned)nof_div_up(nv, (int64_t)1 << ls)), dim3(EMB_T), 0, st,
                      (const T*)table, stride, ids, ids64, scale, (T*)out, N, rows, D, ls);
 }
 
-template <typename T, int V>
+template <typename T>
 static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* key, const uint32_t* pos, float scale, void* grad, float* part,
                             const EmbPlan& p, int32_t D, hipStream_t st) {
-  const int64_t nv = D / V;
+  const int64_t nv = nof_div_up(D, EmbVec<T>::V);
   const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
   const unsigned cols = (unsigned)nof_div_up(nv, (int64_t)1 << ls), n_red = (unsigned)nof_div_up(p.chunks, EMB_T >> ls);
   const unsigned n_zero = (unsigned)nof_div_up(p.s.rows, EMB_ZROWS);
-  hipLaunchKernelGGL((k_embed_reduce<T, V>), dim3(n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N,
+  hipLaunchKernelGGL(k_embed_reduce<T>, dim3(n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N,
                      (uint32_t)p.s.rows, D, scale, (T*)grad, part, ls, p.C, n_red);
   if (p.chunks > 1) {
-    constexpr int JV = V > 4 ? 4 : V;
-    const int64_t jv = D / JV;
+    const int64_t jv = nof_div_up(D, 4);
     const int jl = learn_log2_up(jv < 64 ? jv : 64);
-    hipLaunchKernelGGL((k_embed_join<T, JV>), dim3(p.chunks, (unsigned)nof_div_up(jv, (int64_t)1 << jl)), dim3(EMB_T), 0, st,
-                       key, p.s.N, (uint32_t)p.s.rows, D, scale, (T*)grad, (const float*)part, jl, p.C);
+    hipLaunchKernelGGL(k_embed_join<T>, dim3(p.chunks, (unsigned)nof_div_up(jv, (int64_t)1 << jl)), dim3(EMB_T), 0, st, key, p.s.N,
+                       (uint32_t)p.s.rows, D, scale, (T*)grad, (const float*)part, jl, p.C);
   }
 }
 
@@ -459,8 +472,10 @@ extern "C" int nof_embed_fwd(const void* table, int64_t table_stride, int32_t ty
   NOF_ARG(emb_sizes_ok(N, V, D) && table_stride >= 0);
   if (N == 0 || D == 0) return 0;
   NOF_ARG(ids && out && (table || V == 0));
-  const int v = emb_vec(type, D, table_stride, table, out);
-  EMB_PICK(emb_launch_fwd, table, table_stride, ids, ids64, scale, out, N, V, D, (hipStream_t)stream);
+  hipStream_t st = (hipStream_t)stream;
+  if (type == NOF_TYPE_F32) emb_launch_fwd<float>(table, table_stride, ids, ids64, scale, out, N, V, D, st);
+  else if (type == NOF_TYPE_BF16) emb_launch_fwd<__bf16>(table, table_stride, ids, ids64, scale, out, N, V, D, st);
+  else emb_launch_fwd<_Float16>(table, table_stride, ids, ids64, scale, out, N, V, D, st);
   NOF_LAUNCH_OK();
   return 0;
 }
@@ -500,8 +515,9 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
     }
     NOF_LAUNCH_OK();
   }
-  const int v = emb_vec(type, D, dout_stride, dout, grad_table);
-  EMB_PICK(emb_launch_sums, dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
+  if (type == NOF_TYPE_F32) emb_launch_sums<float>(dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
+  else if (type == NOF_TYPE_BF16) emb_launch_sums<__bf16>(dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
+  else emb_launch_sums<_Float16>(dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
   NOF_LAUNCH_OK();
   return 0;
 }
