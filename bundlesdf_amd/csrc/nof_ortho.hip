@@ -55,7 +55,10 @@ __device__ __forceinline__ double ort_factor(double sumsq, float eps) {
 
 // ---- one workgroup a matrix -------------------------------------------------------------------------------------------------------
 // One wave per 32 x 32 tile of X (r <= k after the turn; tiles rt x KT).  LDS: two pairs of images, rows of 32 KT + 8 halves (the pad
-// spreads a column's 16-byte reads over all banks; known at compile time, or sixteen row offsets per store stay live and spill).  The first holds X for the Gram product and X^T for the last one, the second A, then P.
+// spreads a column's 16-byte reads over all banks; known at compile time, or sixteen row offsets per store stay live and spill).  The first holds X for the Gram product and X^T for the last one, the second A, then P: symmetric, so their tiles are stored
+// turned, four halves at a time.  Bound by the chain of products, barriers and LDS round trips: 1.7 us a step for 16 x 16, 2.5 for 64 x 64,
+// 7.7 for 128 x 128 (half of it the matrix cores); four waves of 2 x 2 tiles instead of sixteen of one read half as much LDS and take 1.4
+// times as long.
 struct OrtCoef { float c[3 * ORT_MAX_STEPS]; };
 
 template <typename T, int KT>
@@ -66,11 +69,11 @@ __global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restric
   const int r = tall ? n : m, k = tall ? m : n, rt = (r + 31) / 32;
   int tid = threadIdx.x;
   int hi = (tid >> 5) & 1, l31 = tid & 31, w = __builtin_amdgcn_readfirstlane(tid >> 6), ti = w / KT, tj = w % KT;      // rt * KT waves
-  constexpr int px = 32 * KT + 8, pa = px;
+  constexpr int px = 32 * KT + 8;
   _Float16* xh = (_Float16*)ort_lds;
   _Float16* xl = xh + 32 * KT * px;
   _Float16* ah = xl + 32 * KT * px;
-  _Float16* al = ah + 32 * KT * pa;
+  _Float16* al = ah + 32 * KT * px;
   g += (size_t)blockIdx.x * m * n;
   out += (size_t)blockIdx.x * m * n;
   int j = 32 * tj + l31;
@@ -90,6 +93,17 @@ __global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restric
   for (int step = 0; step < steps; ++step) {
     asm volatile("" : "+v"(tid));                                     // (no instruction: lane places are formed in the step, not before the loop and spilled)
     hi = (tid >> 5) & 1; l31 = tid & 31; j = 32 * tj + l31;
+    auto put = [&](_Float16* h, _Float16* l, const auto& y) {         // this wave's tile, turned: four i side by side to row j
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f16x4 h4, l4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { _Float16 a, b; ort_split(y[4 * q + e], a, b); h4[e] = a; l4[e] = b; }
+        const int at = j * px + 32 * ti + 8 * q + 4 * hi;
+        *(f16x4*)(h + at) = h4;
+        *(f16x4*)(l + at) = l4;
+      }
+    };
     const float ca = coef.c[3 * step], cb = coef.c[3 * step + 1], cc = coef.c[3 * step + 2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
@@ -105,26 +119,15 @@ __global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restric
         acc = ort_mma3(*(const f16x8*)(xh + lo), *(const f16x8*)(xl + lo), *(const f16x8*)(xh + ro), *(const f16x8*)(xl + ro), acc);
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {                                  // 4096 A
-        acc[e] *= 1.0f / ORT_SCALE;
-        const int at = (32 * ti + nloc(hi, e)) * pa + 32 * tj + l31;
-        ort_split(acc[e], ah[at], al[at]);
-      }
+      for (int e = 0; e < 16; ++e) acc[e] *= 1.0f / ORT_SCALE;         // 4096 A
+      put(ah, al, acc);
     }
     __syncthreads();                                                  // X has been read, A is there
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {                                     // X^T over X: rows j, four i side by side
-      f16x4 h4, l4;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { _Float16 a, b; ort_split(x[4 * q + e], a, b); h4[e] = a; l4[e] = b; }
-      const int at = j * px + 32 * ti + 8 * q + 4 * hi;
-      *(f16x4*)(xh + at) = h4;
-      *(f16x4*)(xl + at) = l4;
-    }
+    put(xh, xl, x);                                                   // X^T over X
     if (gram) {
 #pragma unroll 2
       for (int q = 0; q < 2 * rt; ++q) {
-        const int lo = (32 * ti + l31) * pa + 16 * q + 8 * hi, ro = (32 * tj + l31) * pa + 16 * q + 8 * hi;
+        const int lo = (32 * ti + l31) * px + 16 * q + 8 * hi, ro = (32 * tj + l31) * px + 16 * q + 8 * hi;
         sq = ort_mma3(*(const f16x8*)(ah + lo), *(const f16x8*)(al + lo), *(const f16x8*)(ah + ro), *(const f16x8*)(al + ro), sq);
       }
     }
@@ -132,16 +135,16 @@ __global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restric
     if (gram) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int i = 32 * ti + nloc(hi, e), at = i * pa + 32 * tj + l31;
-        const float p = (i == 32 * tj + l31 ? ca * ORT_SCALE : 0.0f) + cb * acc[e] + cc * (sq[e] * (1.0f / ORT_SCALE));
-        ort_split(p, ah[at], al[at]);
+        const int i = 32 * ti + nloc(hi, e);
+        acc[e] = (i == j ? ca * ORT_SCALE : 0.0f) + cb * acc[e] + cc * (sq[e] * (1.0f / ORT_SCALE));
       }
+      put(ah, al, acc);
     }
     __syncthreads();
     f32x16 y = {};
 #pragma unroll 2
     for (int q = 0; q < 2 * rt; ++q) {
-      const int lo = (32 * ti + l31) * pa + 16 * q + 8 * hi, ro = (32 * tj + l31) * px + 16 * q + 8 * hi;
+      const int lo = (32 * ti + l31) * px + 16 * q + 8 * hi, ro = (32 * tj + l31) * px + 16 * q + 8 * hi;
       y = ort_mma3(*(const f16x8*)(ah + lo), *(const f16x8*)(al + lo), *(const f16x8*)(xh + ro), *(const f16x8*)(xl + ro), y);
     }
 #pragma unroll
@@ -182,6 +185,7 @@ __global__ __launch_bounds__(256) void k_ortho_norm(const T* __restrict__ g, int
   g += (size_t)blockIdx.y * count;
   double s[4] = {0.0, 0.0, 0.0, 0.0};
   const int64_t step = (int64_t)gridDim.x * 256 * V;
+#pragma unroll 4
   for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < count; i += step) {
     float f[V];
     lload<T, V>(g + i, f);
@@ -508,19 +512,10 @@ static bool ort_sizes_ok(int64_t batch, int64_t m, int64_t n) {
 }
 static bool ort_is_small(int64_t m, int64_t n) { return m <= ORT_SMALL && n <= ORT_SMALL; }
 // The tile of a product: 128 x 128 where that gives a workgroup per compute unit, else 64 x 64.  Images are padded to whole tiles.
-#ifndef ORT_ND
-#define ORT_ND 2, 4
-#endif
-#ifndef ORT_N
-#define ORT_N 2, 2
-#endif
-#ifndef ORT_WD
-#define ORT_WD 2, 2
-#endif
 typedef OrtShape<2, 2, 2, 2, 2, 1> OrtWide;
-typedef OrtShape<2, 2, 2, 2, ORT_WD> OrtWideDeep;                      // one workgroup per compute unit at most: all of LDS is its ring
-typedef OrtShape<2, 2, 1, 1, ORT_N> OrtNarrow;
-typedef OrtShape<2, 2, 1, 1, ORT_ND> OrtNarrowDeep;
+typedef OrtShape<2, 2, 2, 2, 2, 2> OrtWideDeep;                        // one workgroup per compute unit at most: all of LDS is its ring
+typedef OrtShape<2, 2, 1, 1, 2, 2> OrtNarrow;
+typedef OrtShape<2, 2, 1, 1, 2, 4> OrtNarrowDeep;
 static bool ort_wide(int64_t tiles_of_128) { return tiles_of_128 >= 256; }
 static int64_t ort_up(int64_t x, int64_t unit) { return nof_div_up(x, unit) * unit; }
 static int64_t ort_unit(int64_t batch, int64_t r, int64_t k) { return ort_wide(batch * nof_div_up(r, 128) * nof_div_up(k, 128)) ? 128 : 64; }
@@ -584,7 +579,7 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
   const unsigned nb = (unsigned)batch;
   constexpr int V = 16 / (int)sizeof(T);
   const bool wide = ((uintptr_t)g & 15) == 0 && m * n % V == 0;
-  const int64_t want = nof_div_up(m * n, 256 * 8 * 4);
+  const int64_t want = nof_div_up(m * n, 256 * 8 * (wide ? 4 : 1));
   const int n_part = (int)(want < ORT_NORM_BLOCKS ? want : ORT_NORM_BLOCKS);
   if (wide) hipLaunchKernelGGL((k_ortho_norm<T, V>), dim3(n_part, nb), dim3(256), 0, st, (const T*)g, m * n, part);
   else hipLaunchKernelGGL((k_ortho_norm<T, 1>), dim3(n_part, nb), dim3(256), 0, st, (const T*)g, m * n, part);
