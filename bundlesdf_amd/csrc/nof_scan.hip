@@ -216,18 +216,36 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, 4) void k_scan_segments(ScanArgs p)
   }
 }
 
-// S -> what it becomes over segments lo, lo + step, ... (count of them)
+// S -> what it becomes over segments lo, lo + step, ... (count of them).  Many of them are composed by the workgroup's slots, a stretch each:
+// one slot's walk over 511 segments is a chain of 511 loads (1 x 65536 x 64 fp32 forward: 49 us so, 22 by slots).
 template <int V>
-__device__ __forceinline__ void scan_over(const ScanArgs& p, const ScanWhere& q, int lo, int step, int count, float (&S)[V]) {
-#pragma unroll 4
-  for (int k = 0; k < count; ++k) {
-    float A[V], B[V];
-    const float* s = p.seg + (((int64_t)(lo + k * step) * p.B + q.b) * 2) * p.D + q.ch;
-    lload<float, V>(s, A);
-    lload<float, V>(s + p.D, B);
+__device__ __forceinline__ void scan_over(const ScanArgs& p, const ScanWhere& q, int lo, int step, int count, float (&S)[V], float2* sh) {
+  const bool share = count > 16;
+  const int slots = p.waves * (64 >> p.cs), each = share ? (count + slots - 1) / slots : count;
+  const int k0 = share ? q.slot * each : 0, k1 = k0 + each < count ? k0 + each : count;
+  float A[V], B[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) S[v] = A[v] * S[v] + B[v];
+  for (int v = 0; v < V; ++v) { A[v] = 1.0f; B[v] = 0.0f; }
+#pragma unroll 8
+  for (int k = k0; k < k1; ++k) {
+    float a[V], b[V];
+    const float* s = p.seg + (((int64_t)(lo + k * step) * p.B + q.b) * 2) * p.D + q.ch;
+    lload<float, V>(s, a);
+    lload<float, V>(s + p.D, b);
+#pragma unroll
+    for (int v = 0; v < V; ++v) { B[v] = a[v] * B[v] + b[v]; A[v] *= a[v]; }
   }
+  if (share) {
+    float TA[V], TB[V];
+    scan_wave<V, false>(A, B, p.cs, sh);
+    __syncthreads();
+    scan_fold<V, false>(A, B, TA, TB, p.cs, p.waves, sh);
+    __syncthreads();                                                  // (sh is the chunks' next)
+#pragma unroll
+    for (int v = 0; v < V; ++v) { A[v] = TA[v]; B[v] = TB[v]; }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) S[v] = A[v] * S[v] + B[v];
 }
 
 template <typename TG, typename T, int V, bool PC>
@@ -250,7 +268,7 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, 3) void k_scan_fwd(ScanArgs p) {
     scan_fetch<TG, PC ? V : 1>(g, at0 + q.slot * SCAN_U, q.n, at0 + p.chunk <= q.n, 1.0f, a);
     scan_fetch<T, V>(x, at0 + q.slot * SCAN_U, q.n, at0 + p.chunk <= q.n, 0.0f, r);
   }
-  scan_over<V>(p, q, 0, 1, seg, S);
+  scan_over<V>(p, q, 0, 1, seg, S, sh[0]);
   for (int c = c0; c < c1; ++c) {
     const int64_t at = (int64_t)c * p.chunk, i0 = at + q.slot * SCAN_U;
     const bool full = at + p.chunk <= q.n;
@@ -347,7 +365,7 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, PC || V == 1 ? 3 : 2) void k_scan_b
 #pragma unroll
   for (int v = 0; v < V; ++v) R[v] = 0.0f;
   if (p.dlast) lload<float, V>(p.dlast + (int64_t)q.b * p.D + q.ch, R);
-  scan_over<V>(p, q, p.segs - 1, -1, p.segs - 1 - seg, R);
+  scan_over<V>(p, q, p.segs - 1, -1, p.segs - 1 - seg, R, sh[0][0]);
   for (int c = c1 - 1; c >= c0; --c) {
     const int64_t at = (int64_t)c * p.chunk, i0 = at + q.slot * SCAN_U;
     const bool full = at + p.chunk <= q.n;

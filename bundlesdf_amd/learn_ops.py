@@ -65,6 +65,13 @@ def _at(x):
     return None if x is None else x.data_ptr()
 
 
+def _apart(a, b):
+    """whether two contiguous tensors share no memory, or all of it (same start, same length)"""
+    n, m = a.numel() * a.element_size(), b.numel() * b.element_size()
+    x, y = a.data_ptr(), b.data_ptr()
+    return x + n <= y or y + m <= x or (x == y and n == m) or n == 0 or m == 0
+
+
 def _rows(x):
     """x [N, D] with its elements side by side in a row: (tensor, elements between rows)"""
     if x.shape[1] > 1 and x.stride(1) != 1:
@@ -255,8 +262,11 @@ def gated_scan_step(gate, value, state, new_state=None):
     (value, vst), (gate, gst), state = _scan_strided(value, even), _scan_strided(gate, even and G == D), _flat(state, even)
     if new_state is None:
         new_state = state.new_empty((B, D))
-    elif even and new_state.data_ptr() % 8:
-        raise NofError('gated_scan_step: new_state must start on an 8-byte border')
+    else:
+        if even and new_state.data_ptr() % 8:
+            raise NofError('gated_scan_step: new_state must start on an 8-byte border')
+        if not _apart(new_state, state):
+            raise NofError('gated_scan_step: new_state must be state itself or lie apart from it')
     h = value.new_empty((B, D))
     _call(dev, 'nof_gated_scan_step', gate.data_ptr(), *gst, _TYPE[gate.dtype], value.data_ptr(), *vst, _TYPE[dt], state.data_ptr(),
           new_state.data_ptr(), h.data_ptr(), B, D, G)
@@ -297,6 +307,8 @@ def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-30, out=None):
     update = update.contiguous()
     if out is None:
         out = update.new_empty(update.shape)
+    elif not _apart(out, update):
+        raise NofError('orthogonalize: out must be update itself or lie apart from it')
     nbytes = _bytes('nof_orthogonalize_workspace_bytes', batch, m, n)
     ws = _scratch(update, nbytes)
     _call(dev, 'nof_orthogonalize', update.data_ptr(), out.data_ptr(), _TYPE[update.dtype], int(steps), coef, float(eps), _at(ws), nbytes, batch, m, n)

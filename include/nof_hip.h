@@ -574,7 +574,7 @@ int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type, const voi
  * (state NULL: zeros; last, h and marks may be NULL).  lengths [B] int32 or NULL: only the first lengths[b] rows (clamped to [0, T]) exist;
  * the others are not read, their rows of h, dgate, dvalue are zeros.  reverse = 1: the recurrence runs from row lengths[b] - 1 down to 0.
  * Positions compose in parallel, so products of gates over a run of positions must stay within binary32 (|gate| <= 1 always does).
- * 16-bit types with an even number of channels per group: pointers and strides are multiples of two elements.
+ * 16-bit types with an even number of channels per group: pointers and strides (a shared gate's aside) are multiples of two elements.
  * B < 2^24, T < 2^31, D <= 2^20. */
 int64_t nof_gated_scan_marks_bytes(int64_t B, int64_t T, int32_t D, int32_t G, int32_t type);
 int64_t nof_gated_scan_workspace_bytes(int64_t B, int64_t T, int32_t D, int32_t G, int32_t type);

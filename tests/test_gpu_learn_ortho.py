@@ -93,6 +93,9 @@ def test_steps_coefficients_layout_and_place(nof, m, n):
     v = u.clone()
     L.orthogonalize(v, out=v)                                                             # in place
     assert torch.equal(v, want)
+    line = torch.zeros(u.numel() + 8, device='cuda')
+    with pytest.raises(nof.NofError, match='apart'):
+        L.orthogonalize(line[:u.numel()].view(u.shape), out=line[8:].view(u.shape))
     assert L.orthogonalize(u[:0]).shape == (0, 2, m, n) and L.orthogonalize(u[..., :0]).shape == (3, 2, m, 0)
 
 

@@ -76,7 +76,7 @@ def make(B, T, D, G, dtype, gdtype, seed, signed=False):
 
 
 SIZES = [(1, 1, 1, 1), (2, 0, 3, 3), (3, 7, 5, 5), (2, 65, 64, 64), (5, 193, 16, 1), (1, 1025, 33, 3), (2, 600, 130, 2), (1, 5000, 8, 8), (40, 100, 6, 2),
-         (1, 4097, 256, 1), (2, 700, 200, 200), (1, 9001, 3, 1), (2, 130, 1, 1), (3, 64, 24, 3), (1, 3000, 390, 1), (600, 9, 64, 4)]
+         (1, 4097, 256, 1), (2, 700, 200, 200), (1, 9001, 3, 1), (2, 130, 1, 1), (3, 64, 24, 3), (1, 3000, 390, 1), (600, 9, 64, 4), (1, 40000, 4, 4)]
 
 
 @pytest.mark.parametrize('B,T,D,G', SIZES)
@@ -161,6 +161,14 @@ def test_step(nof, kind, B, D, G):
     assert torch.equal(last, new) and torch.equal(h1[:, 0], h)           # one position of the scan is the step
     h2, same = L.gated_scan_step(gate[:, 0], value[:, 0], state, new_state=state)
     assert same.data_ptr() == state.data_ptr() and torch.equal(state, new) and torch.equal(h2, h)
+
+
+def test_step_refuses_a_state_that_overlaps_another(nof):
+    from bundlesdf_amd import learn_ops as L
+    line = torch.zeros(100, device='cuda')
+    gate, value = torch.ones(4, 1, device='cuda'), torch.zeros(4, 8, device='cuda')
+    with pytest.raises(nof.NofError, match='apart'):
+        L.gated_scan_step(gate, value, line[:32].view(4, 8), new_state=line[8:40].view(4, 8))
 
 
 def test_step_by_step_is_the_scan(nof):

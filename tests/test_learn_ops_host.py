@@ -137,3 +137,9 @@ def test_orthogonalize_entry_point_refuses():
     assert call(batch=0) == 0 and call(m=0) == 0 and call(n=0) == 0
     assert so.nof_orthogonalize_workspace_bytes(1, 16385, 4) == -1 and so.nof_orthogonalize_workspace_bytes(1, 128, 128) == 0
     assert so.nof_orthogonalize_workspace_bytes(3, 129, 20) > 3 * 2 * 3 * 129 * 20 * 2
+
+
+def test_overlap_of_results_and_inputs():
+    x = torch.zeros(100)
+    assert L._apart(x[:50], x[50:]) and L._apart(x[:50], x[:50]) and L._apart(x[:0], x[:9]) and L._apart(x[50:], x[:50])
+    assert not L._apart(x[:50], x[49:]) and not L._apart(x[:50], x[:49]) and not L._apart(x[10:20], x)
