@@ -44,6 +44,7 @@ def _on_device(what, *tensors):
 
 
 _fn = {}
+_device = getattr(torch._C, '_cuda_getDevice', None) or torch.cuda.current_device
 _stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)     # (no Stream object)
 
 
@@ -52,7 +53,7 @@ def _call(dev, name, *args):
     fn = _fn.get(name)
     if fn is None:
         fn = _fn[name] = getattr(lib.load(), name)
-    if dev == torch.cuda.current_device():
+    if dev == _device():
         rc = fn(*args, _stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -142,6 +143,12 @@ def _scan_even(dtype, D, G):
 
 def _scan_strided(x, even):
     """x [B, T, C] (or [B, C]) as the kernels take it -- channels side by side, two-channel loads on their border -- and its strides"""
+    if x.is_contiguous():
+        n = x.shape
+        st = (n[1],) if len(n) == 2 else (n[1] * n[2], n[2])
+        if not even or x.data_ptr() % (2 * x.element_size()) == 0:         # (even: so are the strides)
+            return x, st
+        return x.clone(), st
     st = x.stride()
     if st[-1] != 1 and x.shape[-1] > 1:
         x = x.contiguous()
@@ -157,7 +164,8 @@ def _flat(x, even):
     """a [B, D] float32 argument as the kernels take it, or None"""
     if x is None:
         return None
-    x = x.contiguous()
+    if not x.is_contiguous():
+        x = x.contiguous()
     return x.clone() if even and x.data_ptr() % 8 else x
 
 
@@ -168,7 +176,7 @@ def _state_ok(what, name, x, B, D):
 
 def _scan_args(what, gate, value, lengths, dims):
     vs, gs = value.shape, gate.shape
-    if not (len(vs) == dims and value.dtype in _TYPE):
+    if len(vs) != dims or value.dtype not in _TYPE:
         raise NofError(f'{what}: value must be [{"B, T, D" if dims == 3 else "B, D"}] float32, bfloat16 or float16')
     if not (len(gs) == dims and gs[:-1] == vs[:-1]):
         raise NofError(f"{what}: gate must have value's shape but for the channels")
