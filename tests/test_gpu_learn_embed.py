@@ -140,3 +140,21 @@ def test_stream_and_graph(nof):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(grad, L.embed_lookup_grad(dout, ids, 900, 1.0)) and torch.equal(out, L.embed_lookup(want, ids, 0.5))
+
+
+def test_offsets_past_32_bits(nof):
+    """a table and a gradient of more than 2^32 bytes and 2^31 elements"""
+    from bundlesdf_amd import learn_ops as L
+    V, D = 1100000, 2048
+    table = torch.empty(V, D, dtype=torch.bfloat16, device='cuda')
+    ids = torch.tensor([V - 1, 0, V - 2, V // 2, V - 1, -1, V], device='cuda')
+    gen = torch.Generator(device='cuda').manual_seed(0)
+    rows = torch.randn(7, D, device='cuda', generator=gen).to(torch.bfloat16)
+    table[ids[:4]] = rows[:4]
+    out = L.embed_lookup(table, ids)
+    assert torch.equal(out[:4], rows[:4]) and torch.equal(out[4], rows[0]) and (out[5:] == 0).all()
+    del table
+    grad = L.embed_lookup_grad(rows, ids, V)
+    assert torch.equal(grad[V - 1], (rows[0].float() + rows[4].float()).to(torch.bfloat16)) and torch.equal(grad[V - 2], rows[2])
+    grad[ids[:4]] = 0
+    assert all(int(torch.count_nonzero(part)) == 0 for part in grad.split(1 << 17))

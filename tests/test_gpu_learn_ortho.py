@@ -119,7 +119,7 @@ def test_zero_and_not_finite(nof, m, n):
 
 def test_stream_and_graph(nof):
     from bundlesdf_amd import learn_ops as L
-    a, b = make('noise', (6, 64, 32), torch.float32, 1), make('noise', (300, 140), torch.bfloat16, 2)
+    a, b = make('noise', (6, 100, 128), torch.float32, 1), make('noise', (300, 140), torch.bfloat16, 2)
     want = L.orthogonalize(a), L.orthogonalize(b)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

@@ -238,3 +238,24 @@ def test_stream_and_graph(nof):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, both()))
+
+
+def test_offsets_past_32_bits(nof):
+    """more than 2^31 elements: the last channels of the last sequence against the recurrence on them alone"""
+    from bundlesdf_amd import learn_ops as L
+    B, T, D = 2, 2000, 540672
+    gen = torch.Generator(device='cuda').manual_seed(0)
+    gate = torch.sigmoid(torch.randn(B, T, 1, device='cuda', generator=gen) + 2)
+    value = torch.empty(B, T, D, dtype=torch.bfloat16, device='cuda')
+    assert value.numel() > 1 << 31
+    value.zero_()
+    ends = [0, 1, D // 2, D - 2, D - 1]
+    value[..., ends] = torch.randn(B, T, len(ends), device='cuda', generator=gen).to(torch.bfloat16)
+    want = recurrence(gate, value[..., ends], None, None, True, value[..., ends])
+    h, last, marks = L.gated_scan(gate, value, reverse=True, want_marks=True)
+    check(h[..., ends], want['h'], 'h')
+    check(last[:, ends], want['last'], 'last')
+    del h
+    dgate, dvalue, dstate = L.gated_scan_grad(gate, value, value, None, None, marks, reverse=True)
+    check(dvalue[..., ends], want['dvalue'], 'dvalue')
+    check(dgate, want['dgate'], 'dgate')                                  # (the other channels add nothing: their values are zeros)
