@@ -12,7 +12,7 @@
 // values and the polynomial amplifies it.
 //
 // Matrices of at most 128 x 128 take one workgroup and one launch (k_ortho_small): X lives in accumulator registers, operands in LDS.
-// Larger ones are three launches a step over images of X, X^T, A, P in the workspace, every product C = L R^T with both operands'
+// Thin ones, of at most 128 on one side, take a launch a step (k_ortho_thin).  Larger ones are three launches a step over images of X, X^T, A, P in the workspace, every product C = L R^T with both operands'
 // rows along the summed index, so X is stored in both orientations.
 #include "nof_learn_dev.h"
 #include "nof_mfma_dev.h"
@@ -157,6 +157,145 @@ __global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restric
   for (int e = 0; e < 16; ++e) {
     const int i = 32 * ti + nloc(hi, e);
     if (i < r && j < k) out[i * si + j * sj] = lt<T>(x[e] * (1.0f / ORT_SCALE));
+  }
+}
+
+// ---- thin matrices ----------------------------------------------------------------------------------------------------------------
+// At most 128 on the shorter side, more on the longer: a launch a step instead of three.  A workgroup owns a stretch of X's columns, 128 at a
+// time through LDS, and knows the Gram matrix as the sum of all workgroups' parts of it, which the launch before left behind: it forms A and
+// P for itself, then X <- P X of its columns and the new part.  X stays in memory as the accumulators hold it.  Parts are added in the order
+// of the workgroups.  64 x 1000 fp32: 49 us (109 as tiles of the larger matrices, whose Gram product is one tile's chain over the long side),
+// 64 x 16384: 130 us (599), 128 x 4096: 141 us (222).
+struct OrtThin {
+  const double* part; int n_part;
+  float* x; const float* gram_in; float* gram_out;
+  int m, n, r, k, tall, blocks, chunks; // chunks of 128 columns per workgroup
+  float ca, cb, cc, eps;
+};
+#define ORT_FIRST 0                     // X from the update, its part of the Gram matrix
+#define ORT_STEP 1
+#define ORT_FINAL 2                     // a step to the result
+
+// one wave's tile as memory holds it: sixteen values a lane, whole lines
+__device__ __forceinline__ void ort_tile_load(const float* p, int lane, float (&x)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float4 v = *(const float4*)(p + q * 256 + lane * 4);
+    x[4 * q] = v.x; x[4 * q + 1] = v.y; x[4 * q + 2] = v.z; x[4 * q + 3] = v.w;
+  }
+}
+template <typename A> __device__ __forceinline__ void ort_tile_store(float* p, int lane, const A& x) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) *(float4*)(p + q * 256 + lane * 4) = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+}
+// 32 x 32 tile of L R^T over 16 n columns; rows of `pl`, `pr` halves, lo planes dl, dr halves behind
+__device__ __forceinline__ f32x16 ort_tile_product(const _Float16* L, int dl, const _Float16* R, int dr, int n, f32x16 acc) {
+#pragma unroll 2
+  for (int q = 0; q < n; ++q)
+    acc = ort_mma3(*(const f16x8*)(L + 16 * q), *(const f16x8*)(L + dl + 16 * q), *(const f16x8*)(R + 16 * q), *(const f16x8*)(R + dr + 16 * q), acc);
+  return acc;
+}
+
+template <typename T, int RT, int MODE>
+__global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g, T* __restrict__ out, OrtThin p) {
+  extern __shared__ __attribute__((aligned(16))) char ort_lds[];
+  __shared__ double red[4 * RT];
+  constexpr int PX = 136, PA = 32 * RT + 8, plane_x = 128 * PA > 32 * RT * PX ? 128 * PA : 32 * RT * PX, plane_a = 32 * RT * PA;
+  _Float16* X = (_Float16*)ort_lds;                                   // X [32 RT][PX] or X^T [128][PA]
+  _Float16* A = X + 2 * plane_x;                                      // A, then P, [32 RT][PA]
+  const int b = blockIdx.x / p.blocks, block = blockIdx.x % p.blocks, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ti = w / 4, tj = w % 4;
+  int tid = threadIdx.x, lane = tid & 63, hi = lane >> 5, l31 = lane & 31;
+  const bool gram = tj < RT;                                          // this wave also owns tile (ti, tj) of A and P
+  const int si = p.tall ? 1 : p.n, sj = p.tall ? p.n : 1;
+  g += (size_t)b * p.m * p.n;
+  out += (size_t)b * p.m * p.n;
+  auto put = [&](_Float16* image, int plane, int column, const auto& y) {       // this wave's tile, turned: four i side by side to row `column`
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f16x4 h4, l4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { _Float16 h, l; ort_split(y[4 * q + e], h, l); h4[e] = h; l4[e] = l; }
+      _Float16* at = image + column * PA + 32 * ti + 8 * q + 4 * hi;
+      *(f16x4*)at = h4;
+      *(f16x4*)(at + plane) = l4;
+    }
+  };
+  double f = 0.0;
+  if (MODE == ORT_FIRST) {
+    double s = 0.0;
+    for (int q = tid; q < p.n_part; q += 256 * RT) s += p.part[b * p.n_part + q];
+    f = ort_factor(ort_block_sum(s, red), p.eps);
+  } else {
+    float a[16];
+    f32x16 sq = {};
+    if (gram) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) a[e] = 0.0f;
+      const float* in = p.gram_in + ((size_t)b * p.blocks * RT * RT + ti * RT + tj) * 1024;
+#pragma unroll 4
+      for (int q = 0; q < p.blocks; ++q) {
+        float y[16];
+        ort_tile_load(in + (size_t)q * RT * RT * 1024, lane, y);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) a[e] += y[e];
+      }
+      put(A, plane_a, 32 * tj + l31, a);
+    }
+    __syncthreads();
+    if (gram) sq = ort_tile_product(A + (32 * ti + l31) * PA + 8 * hi, plane_a, A + (32 * tj + l31) * PA + 8 * hi, plane_a, 2 * RT, sq);
+    __syncthreads();
+    if (gram) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        a[e] = (32 * ti + nloc(hi, e) == 32 * tj + l31 ? p.ca * ORT_SCALE : 0.0f) + p.cb * a[e] + p.cc * (sq[e] * (1.0f / ORT_SCALE));
+      put(A, plane_a, 32 * tj + l31, a);
+    }
+  }
+  f32x16 part = {};
+  for (int c = 0; c < p.chunks; ++c) {
+    asm volatile("" : "+v"(tid));                                     // (no instruction: lane places are formed in the loop, not before it and spilled)
+    lane = tid & 63; hi = lane >> 5; l31 = lane & 31;
+    const int chunk = block * p.chunks + c, j = chunk * 128 + 32 * tj + l31;
+    if (chunk * 128 >= p.k) break;
+    float* at = p.x + (((size_t)(b * p.blocks + block) * p.chunks + c) * RT * 4 + w) * 1024;
+    float x[16];
+    if (MODE == ORT_FIRST) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int i = 32 * ti + nloc(hi, e);
+        x[e] = i < p.r && j < p.k ? (float)((double)lf(g[(size_t)i * si + (size_t)j * sj]) * f) : 0.0f;
+      }
+    } else {
+      ort_tile_load(at, lane, x);
+      put(X, plane_x, 32 * tj + l31, x);
+      __syncthreads();                                                // X^T is there (and P)
+      f32x16 y = {};
+      y = ort_tile_product(A + (32 * ti + l31) * PA + 8 * hi, plane_a, X + (32 * tj + l31) * PA + 8 * hi, plane_x, 2 * RT, y);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = y[e] * (1.0f / ORT_SCALE);
+    }
+    if (MODE == ORT_FINAL) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int i = 32 * ti + nloc(hi, e);
+        if (i < p.r && j < p.k) out[(size_t)i * si + (size_t)j * sj] = lt<T>(x[e] * (1.0f / ORT_SCALE));
+      }
+      __syncthreads();                                                // X^T has been read
+    } else {
+      ort_tile_store(at, lane, x);
+      __syncthreads();
+      _Float16* to = X + (32 * ti + 4 * hi) * PX + 32 * tj + l31;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) ort_split(x[e], to[nloc(0, e) * PX], to[plane_x + nloc(0, e) * PX]);
+      __syncthreads();
+      if (gram) part = ort_tile_product(X + (32 * ti + l31) * PX + 8 * hi, plane_x, X + (32 * tj + l31) * PX + 8 * hi, plane_x, 8, part);
+      __syncthreads();
+    }
+  }
+  if (MODE != ORT_FINAL && gram) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) part[e] *= 1.0f / ORT_SCALE;         // 4096 of A
+    ort_tile_store(p.gram_out + (((size_t)b * p.blocks + block) * RT * RT + ti * RT + tj) * 1024, lane, part);
   }
 }
 
@@ -520,9 +659,23 @@ static bool ort_wide(int64_t tiles_of_128) { return tiles_of_128 >= 256; }
 static int64_t ort_up(int64_t x, int64_t unit) { return nof_div_up(x, unit) * unit; }
 static int64_t ort_unit(int64_t batch, int64_t r, int64_t k) { return ort_wide(batch * nof_div_up(r, 128) * nof_div_up(k, 128)) ? 128 : 64; }
 
+// workgroups per thin matrix: what each reads of the others' parts grows with the square of the shorter side
+static void ort_thin_plan(int64_t r, int64_t k, int& blocks, int& chunks) {
+  const int rt = (int)nof_div_up(r, 32), all = (int)nof_div_up(k, 128), most = rt <= 2 ? 32 : 16;
+  chunks = (int)nof_div_up(all, all < most ? all : most);
+  blocks = (int)nof_div_up(all, chunks);
+}
+static bool ort_is_thin(int64_t m, int64_t n) { return (m <= ORT_SMALL) != (n <= ORT_SMALL); }
+
 extern "C" int64_t nof_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n) {
   if (!ort_sizes_ok(batch, m, n)) return -1;
   if (batch == 0 || m == 0 || n == 0 || ort_is_small(m, n)) return 0;
+  if (ort_is_thin(m, n)) {
+    int blocks, chunks;
+    const int64_t rt = nof_div_up(m < n ? m : n, 32);
+    ort_thin_plan(m < n ? m : n, m < n ? n : m, blocks, chunks);
+    return learn_align(batch * ORT_NORM_BLOCKS * 8) + batch * blocks * (chunks * rt * 4 + 2 * rt * rt) * 4096;
+  }
   const int64_t r = m < n ? m : n, k = m < n ? n : m, unit = ort_unit(batch, r, k), rp = ort_up(r, unit), kp = ort_up(k, unit);
   return learn_align(batch * ORT_NORM_BLOCKS * 8) + batch * (6 * rp * kp + 4 * rp * rp) * 2;
 }
@@ -555,6 +708,48 @@ static void ort_product(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
   else ort_gemm<MODE, T, OrtNarrowDeep, PAIRS>(p, out, batch, st);
 }
 
+// the sums of squares, as many as it says
+template <typename T>
+static int ort_launch_norm(const void* g, double* part, int64_t batch, int64_t m, int64_t n, hipStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const bool wide = ((uintptr_t)g & 15) == 0 && m * n % V == 0;
+  const int64_t want = nof_div_up(m * n, 256 * 8 * (wide ? 4 : 1));
+  const int n_part = (int)(want < ORT_NORM_BLOCKS ? want : ORT_NORM_BLOCKS);
+  if (wide) hipLaunchKernelGGL((k_ortho_norm<T, V>), dim3(n_part, (unsigned)batch), dim3(256), 0, st, (const T*)g, m * n, part);
+  else hipLaunchKernelGGL((k_ortho_norm<T, 1>), dim3(n_part, (unsigned)batch), dim3(256), 0, st, (const T*)g, m * n, part);
+  return n_part;
+}
+
+template <typename T, int RT, int MODE>
+static void ort_thin_step(const void* g, void* out, const OrtThin& p, int64_t batch, hipStream_t st) {
+  constexpr int px = 128 * (32 * RT + 8) > 32 * RT * 136 ? 128 * (32 * RT + 8) : 32 * RT * 136;
+  constexpr size_t lds = 2 * 2 * (size_t)(px + 32 * RT * (32 * RT + 8));                              // 136 KiB for RT = 4
+  if (lds > 64 << 10) (void)hipFuncSetAttribute((const void*)&k_ortho_thin<T, RT, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  hipLaunchKernelGGL((k_ortho_thin<T, RT, MODE>), dim3((unsigned)(batch * p.blocks)), dim3(256 * RT), lds, st, (const T*)g, (T*)out, p);
+}
+template <typename T, int RT>
+static void ort_launch_thin(const void* g, void* out, void* workspace, int64_t batch, int64_t m, int64_t n, int32_t steps, const float* coef, float eps,
+                            hipStream_t st) {
+  OrtThin p = {};
+  p.m = (int)m; p.n = (int)n; p.tall = m > n; p.r = (int)(m < n ? m : n); p.k = (int)(m < n ? n : m); p.eps = eps;
+  ort_thin_plan(p.r, p.k, p.blocks, p.chunks);
+  double* part = (double*)workspace;
+  p.part = part;
+  p.n_part = ort_launch_norm<T>(g, part, batch, m, n, st);
+  p.x = (float*)((char*)workspace + learn_align(batch * ORT_NORM_BLOCKS * 8));
+  float* grams = p.x + (size_t)batch * p.blocks * p.chunks * RT * 4 * 1024;
+  const size_t each = (size_t)batch * p.blocks * RT * RT * 1024;
+  p.gram_out = grams;
+  ort_thin_step<T, RT, ORT_FIRST>(g, out, p, batch, st);
+  for (int s = 0; s < steps; ++s) {
+    p.ca = coef[3 * s]; p.cb = coef[3 * s + 1]; p.cc = coef[3 * s + 2];
+    p.gram_in = grams + (s & 1 ? each : 0);
+    p.gram_out = grams + (s & 1 ? 0 : each);
+    if (s + 1 < steps) ort_thin_step<T, RT, ORT_STEP>(g, out, p, batch, st);
+    else ort_thin_step<T, RT, ORT_FINAL>(g, out, p, batch, st);
+  }
+}
+
 template <typename T>
 static void ort_launch(const void* g, void* out, void* workspace, int64_t batch, int64_t m, int64_t n, int32_t steps, const float* coef, float eps,
                        hipStream_t st) {
@@ -567,6 +762,14 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
     else ort_launch_small<T, 4>(g, out, batch, m, n, steps, coef, eps, st);
     return;
   }
+  if (ort_is_thin(m, n)) {
+    const int rt = (int)nof_div_up(r, 32);
+    if (rt == 1) ort_launch_thin<T, 1>(g, out, workspace, batch, m, n, steps, coef, eps, st);
+    else if (rt == 2) ort_launch_thin<T, 2>(g, out, workspace, batch, m, n, steps, coef, eps, st);
+    else if (rt == 3) ort_launch_thin<T, 3>(g, out, workspace, batch, m, n, steps, coef, eps, st);
+    else ort_launch_thin<T, 4>(g, out, workspace, batch, m, n, steps, coef, eps, st);
+    return;
+  }
   const int64_t unit = ort_unit(batch, r, k);
   OrtArgs p = {};
   p.r = (int)r; p.k = (int)k; p.rp = (int)ort_up(r, unit); p.kp = (int)ort_up(k, unit);
@@ -577,12 +780,7 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
   double* part = (double*)workspace;
   p.ws = (_Float16*)((char*)workspace + learn_align(batch * ORT_NORM_BLOCKS * 8));
   const unsigned nb = (unsigned)batch;
-  constexpr int V = 16 / (int)sizeof(T);
-  const bool wide = ((uintptr_t)g & 15) == 0 && m * n % V == 0;
-  const int64_t want = nof_div_up(m * n, 256 * 8 * (wide ? 4 : 1));
-  const int n_part = (int)(want < ORT_NORM_BLOCKS ? want : ORT_NORM_BLOCKS);
-  if (wide) hipLaunchKernelGGL((k_ortho_norm<T, V>), dim3(n_part, nb), dim3(256), 0, st, (const T*)g, m * n, part);
-  else hipLaunchKernelGGL((k_ortho_norm<T, 1>), dim3(n_part, nb), dim3(256), 0, st, (const T*)g, m * n, part);
+  const int n_part = ort_launch_norm<T>(g, part, batch, m, n, st);
   hipLaunchKernelGGL(k_ortho_split<T>, dim3((p.tall ? p.rp : p.kp) / 64, (p.tall ? p.kp : p.rp) / 64, nb), dim3(256), 0, st, (const T*)g,
                      (const double*)part, n_part, p, eps);
   for (int s = 0; s < steps; ++s, p.cur ^= 1) {
