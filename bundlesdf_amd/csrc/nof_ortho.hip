@@ -310,6 +310,7 @@ struct OrtArgs {
   float ca, cb, cc;
   int cur;                              // which X^T holds X
   int tiles;                            // of a matrix in this launch
+  int split; float* parts;              // the Gram product's long axis in `split` parts, joined by a launch of its own
   int flat;                             // this launch's P or X^T is read for hi alone
 };
 __device__ __forceinline__ _Float16* ort_x(const OrtArgs& p, int b) { return p.ws + b * p.per; }
@@ -378,6 +379,7 @@ __global__ __launch_bounds__(256) void k_ortho_split(const T* __restrict__ g, co
 #define ORT_POLY 1
 #define ORT_APPLY 2
 #define ORT_LAST 3
+#define ORT_JOIN 4                      // the Gram product's parts, added in order
 
 // A stage is 64 halves of every row: 32 of the summed index as hi and lo, or 64 of it as hi alone.  16-byte piece c of row `row`
 // sits at piece c ^ ort_swizzle(row): a fragment's reads (one piece of 32 consecutive rows) then touch every bank equally, for eight lanes
@@ -411,11 +413,18 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
   // Workgroups go round the eight XCDs: each takes a stretch of neighbouring tiles, whose operands its L2 then holds once
   const int total = gridDim.x, each = total / 8, more = total % 8, xcd = blockIdx.x % 8;
   int t = xcd * each + (xcd < more ? xcd : more) + blockIdx.x / 8, bi, bj;
+  int slice = 0;                                                      // of the summed axis
+  if (MODE == ORT_GRAM && p.split > 1) {                             
+    const int whole = t / p.tiles;
+    slice = whole % p.split;
+    t -= (whole - whole / p.split) * p.tiles;                         // batch entry * tiles + tile
+  }
   const int b = t / p.tiles;
   t -= b * p.tiles;
+  const size_t part = ((size_t)b * p.tiles + t) * p.split * S::M * S::N;       // where the parts of this tile begin
   // within it, blocks of 8 x 8 tiles
   const int nt = p.rp / S::M;
-  if (MODE == ORT_GRAM || MODE == ORT_POLY) {                         // tiles on and above the diagonal
+  if (MODE == ORT_GRAM || MODE == ORT_POLY || MODE == ORT_JOIN) {     // tiles on and above the diagonal
     int bI = 0, bJ = 0;
     for (;;) {
       const int h = nt - 8 * bI < 8 ? nt - 8 * bI : 8, v = nt - 8 * bJ < 8 ? nt - 8 * bJ : 8, n = bI == bJ ? h * (h + 1) / 2 : h * v;
@@ -442,10 +451,16 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
   }
   const _Float16 *L, *R;
   int K;
-  if (MODE == ORT_GRAM) { L = R = ort_x(p, b); K = p.kp; }
+  if (MODE == ORT_GRAM || MODE == ORT_JOIN) { L = R = ort_x(p, b); K = p.kp; }
   else if (MODE == ORT_POLY) { L = R = ort_a(p, b); K = p.rp; }
   else { L = ort_p(p, b); R = ort_xt(p, b, p.cur); K = p.rp; }
   constexpr int kstep = PAIRS ? 32 : 64;
+  int s0 = 0, s1 = MODE == ORT_JOIN ? 0 : K / kstep;                  // the stages of this part
+  if (MODE == ORT_GRAM && p.split > 1) {
+    const unsigned n = s1;                                            // (at most 512, in at most 64 parts)
+    s0 = n * slice / p.split;
+    s1 = n * (slice + 1) / p.split;
+  }
   const size_t pitch = PAIRS ? 2 * (size_t)K : (size_t)K;
   // where this thread's pieces of a stage come from: L's rows, then R's
   const _Float16* src[S::loads];
@@ -453,7 +468,7 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
   for (int q = 0; q < S::loads; ++q) {
     const bool left = q * S::group < 8 * S::M;                        // (a turn of the group lies within one of the two)
     const int piece = q * S::group + tid - (left ? 0 : 8 * S::M), row = piece / 8, c = (piece % 8) ^ ort_swizzle(row);
-    src[q] = (left ? L + (size_t)(bi * S::M + row) * pitch : R + (size_t)(bj * S::N + row) * pitch) + kg * 64 + c * 8;
+    src[q] = (left ? L + (size_t)(bi * S::M + row) * pitch : R + (size_t)(bj * S::N + row) * pitch) + (size_t)(s0 + kg) * 64 + c * 8;
   }
   auto load = [&](int slot) {
 #pragma unroll
@@ -464,7 +479,7 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
     }
   };
   f32x16 acc[S::ti][S::tj] = {};
-  const int wi = (w / S::wn) * S::ti * 32, wj = (w % S::wn) * S::tj * 32, rounds = (K / kstep + S::kg - 1) / S::kg, stages = (K / kstep - kg + S::kg - 1) / S::kg;      // this group's stages
+  const int wi = (w / S::wn) * S::ti * 32, wj = (w % S::wn) * S::tj * 32, n_stages = s1 - s0, rounds = (n_stages + S::kg - 1) / S::kg, stages = (n_stages - kg + S::kg - 1) / S::kg;      // this group's stages
 #pragma unroll
   for (int q = 0; q < S::ns - 1; ++q)
     if (q < stages) load(q);
@@ -542,6 +557,30 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
     __syncthreads();
     if (kg > 0) return;
   }
+  if constexpr (MODE == ORT_GRAM || MODE == ORT_JOIN) {
+    float* mine = p.parts + part + (size_t)slice * S::M * S::N + w * S::ti * S::tj * 1024;
+    if (MODE == ORT_GRAM && p.split > 1) {
+#pragma unroll
+      for (int i = 0; i < S::ti; ++i)
+#pragma unroll
+        for (int j = 0; j < S::tj; ++j) ort_tile_store(mine + (i * S::tj + j) * 1024, lane, acc[i][j]);
+      return;
+    }
+    if (MODE == ORT_JOIN) {
+#pragma unroll 4
+      for (int q = 0; q < p.split; ++q) {
+#pragma unroll
+        for (int i = 0; i < S::ti; ++i)
+#pragma unroll
+          for (int j = 0; j < S::tj; ++j) {
+            float x[16];
+            ort_tile_load(mine + (size_t)q * S::M * S::N + (i * S::tj + j) * 1024, lane, x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] += x[e];
+          }
+      }
+    }
+  }
   const int i0 = bi * S::M + wi, j0 = bj * S::N + wj;
   if (MODE == ORT_LAST) {
     T* o = out + (size_t)b * p.m * p.n;
@@ -589,7 +628,7 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
         for (int e = 0; e < 16; ++e) v[e] *= 1.0f / ORT_SCALE;
       }
     }
-  _Float16* c = MODE == ORT_GRAM ? ort_a(p, b) : MODE == ORT_POLY ? ort_p(p, b) : ort_x(p, b);
+  _Float16* c = MODE == ORT_GRAM || MODE == ORT_JOIN ? ort_a(p, b) : MODE == ORT_POLY ? ort_p(p, b) : ort_x(p, b);
   _Float16* ct = MODE == ORT_APPLY ? ort_xt(p, b, p.cur ^ 1) : c;
   const int ld = MODE == ORT_APPLY ? p.kp : p.rp;
   _Float16* band = lds + w * 32 * wmax;
@@ -655,6 +694,15 @@ typedef OrtShape<2, 2, 2, 2, 2, 1> OrtWide;
 typedef OrtShape<2, 2, 2, 2, 2, 2> OrtWideDeep;                        // one workgroup per compute unit at most: all of LDS is its ring
 typedef OrtShape<2, 2, 1, 1, 2, 2> OrtNarrow;
 typedef OrtShape<2, 2, 1, 1, 2, 4> OrtNarrowDeep;
+typedef OrtShape<2, 2, 1, 1, 2, 1> OrtSingle;                          // the join's
+// The Gram product of few tiles over a long axis is cut along it: at most two workgroups a compute unit, and eight stages a part at least.
+// Five steps of 200 x 4096: 255 us uncut, 153 cut; 600 x 2900: 282 and 241; 333 x 1001, 3 of them: 174 and 170.  Below 1024 the join costs
+// more than the parts save (512 x 512: 146 and 154); parts of four stages gain nothing (200 x 4096: 171).
+static int ort_split(int64_t batch, int64_t rp, int64_t kp) {
+  const int64_t n = rp / 64, tiles = batch * n * (n + 1) / 2, most = kp / 256, want = 512 / tiles;
+  if (kp < 1024 || want < 2) return 1;
+  return (int)(want < most ? want : most);
+}
 static bool ort_wide(int64_t tiles_of_128) { return tiles_of_128 >= 256; }
 static int64_t ort_up(int64_t x, int64_t unit) { return nof_div_up(x, unit) * unit; }
 static int64_t ort_unit(int64_t batch, int64_t r, int64_t k) { return ort_wide(batch * nof_div_up(r, 128) * nof_div_up(k, 128)) ? 128 : 64; }
@@ -677,7 +725,8 @@ extern "C" int64_t nof_orthogonalize_workspace_bytes(int64_t batch, int64_t m, i
     return learn_align(batch * ORT_NORM_BLOCKS * 8) + batch * blocks * (chunks * rt * 4 + 2 * rt * rt) * 4096;
   }
   const int64_t r = m < n ? m : n, k = m < n ? n : m, unit = ort_unit(batch, r, k), rp = ort_up(r, unit), kp = ort_up(k, unit);
-  return learn_align(batch * ORT_NORM_BLOCKS * 8) + batch * (6 * rp * kp + 4 * rp * rp) * 2;
+  const int64_t split = ort_split(batch, rp, kp), side = rp / 64;
+  return learn_align(batch * ORT_NORM_BLOCKS * 8) + batch * (6 * rp * kp + 4 * rp * rp) * 2 + (split > 1 ? batch * side * (side + 1) / 2 * split * 64 * 64 * 4 : 0);
 }
 
 template <typename T, int KT>
@@ -692,17 +741,22 @@ static void ort_launch_small(const void* g, void* out, int64_t batch, int64_t m,
 
 template <int MODE, typename S> static int64_t ort_tiles(const OrtArgs& p) {
   const int64_t ni = p.rp / S::M, nj = p.kp / S::N;
-  return MODE == ORT_GRAM || MODE == ORT_POLY ? ni * (ni + 1) / 2 : ni * nj;
+  return MODE == ORT_GRAM || MODE == ORT_POLY || MODE == ORT_JOIN ? ni * (ni + 1) / 2 : ni * nj;
 }
 template <int MODE, typename T, typename S, bool PAIRS>
 static void ort_gemm(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
   p.tiles = (int)ort_tiles<MODE, S>(p);
-  hipLaunchKernelGGL((k_ortho_gemm<MODE, T, S, PAIRS>), dim3((unsigned)(p.tiles * batch)), dim3(S::threads), 0, st, p, out);
+  const int64_t parts = MODE == ORT_GRAM ? p.split : 1;
+  hipLaunchKernelGGL((k_ortho_gemm<MODE, T, S, PAIRS>), dim3((unsigned)(p.tiles * batch * parts)), dim3(S::threads), 0, st, p, out);
 }
 template <int MODE, typename T, bool PAIRS>
 static void ort_product(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
   const int64_t wide = p.rp % 128 == 0 && p.kp % 128 == 0 ? batch * ort_tiles<MODE, OrtWide>(p) : 0;
-  if (wide > 256) ort_gemm<MODE, T, OrtWide, PAIRS>(p, out, batch, st);
+  if (MODE == ORT_GRAM && p.split > 1) {
+    if (batch * ort_tiles<MODE, OrtNarrow>(p) * p.split > 256) ort_gemm<MODE, T, OrtNarrow, PAIRS>(p, out, batch, st);
+    else ort_gemm<MODE, T, OrtNarrowDeep, PAIRS>(p, out, batch, st);
+    ort_gemm<ORT_JOIN, T, OrtSingle, PAIRS>(p, out, batch, st);
+  } else if (wide > 256) ort_gemm<MODE, T, OrtWide, PAIRS>(p, out, batch, st);
   else if (ort_wide(wide)) ort_gemm<MODE, T, OrtWideDeep, PAIRS>(p, out, batch, st);
   else if (batch * ort_tiles<MODE, OrtNarrow>(p) > 256) ort_gemm<MODE, T, OrtNarrow, PAIRS>(p, out, batch, st);
   else ort_gemm<MODE, T, OrtNarrowDeep, PAIRS>(p, out, batch, st);
@@ -779,6 +833,8 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
   p.flat = light && steps == 1;
   double* part = (double*)workspace;
   p.ws = (_Float16*)((char*)workspace + learn_align(batch * ORT_NORM_BLOCKS * 8));
+  p.split = ort_split(batch, p.rp, p.kp);
+  p.parts = (float*)(p.ws + batch * p.per);
   const unsigned nb = (unsigned)batch;
   const int n_part = ort_launch_norm<T>(g, part, batch, m, n, st);
   hipLaunchKernelGGL(k_ortho_split<T>, dim3((p.tall ? p.rp : p.kp) / 64, (p.tall ? p.kp : p.rp) / 64, nb), dim3(256), 0, st, (const T*)g,

@@ -50,7 +50,7 @@ def check(got, u, **k):
 
 SHAPES = [(1, 1), (1, 7), (5, 1), (3, 64), (16, 64), (64, 31), (64, 32), (64, 64), (33, 65), (128, 128), (127, 100), (128, 1), (129, 128), (4, 130),
           (130, 130), (1, 300), (300, 1), (256, 128), (257, 385), (600, 130), (333, 1001), (512, 512),
-          (20, 2000), (3000, 50), (90, 700), (128, 4200), (2500, 97), (32, 129), (300, 64)]
+          (20, 2000), (3000, 50), (90, 700), (128, 4200), (2500, 97), (32, 129), (300, 64), (140, 2300)]
 
 
 @pytest.mark.parametrize('m,n', SHAPES)
