@@ -697,10 +697,11 @@ typedef OrtShape<2, 2, 1, 1, 2, 4> OrtNarrowDeep;
 typedef OrtShape<2, 2, 1, 1, 2, 1> OrtSingle;                          // the join's
 // The Gram product of few tiles over a long axis is cut along it: at most two workgroups a compute unit, and eight stages a part at least.
 // Five steps of 200 x 4096: 255 us uncut, 153 cut; 600 x 2900: 282 and 241; 333 x 1001, 3 of them: 174 and 170.  Below 1024 the join costs
-// more than the parts save (512 x 512: 146 and 154); parts of four stages gain nothing (200 x 4096: 171).
+// more than the parts save (512 x 512: 146 and 154), and so it does with many tiles of a middling length (1024 x 1024: 209 and 221;
+// 1024 x 2048: 285 either way; 1024 x 4096: 435 and 424).  Parts of four stages gain nothing (200 x 4096: 171).
 static int ort_split(int64_t batch, int64_t rp, int64_t kp) {
   const int64_t n = rp / 64, tiles = batch * n * (n + 1) / 2, most = kp / 256, want = 512 / tiles;
-  if (kp < 1024 || want < 2) return 1;
+  if (kp < 1024 || want < 2 || kp * want < 6144) return 1;
   return (int)(want < most ? want : most);
 }
 static bool ort_wide(int64_t tiles_of_128) { return tiles_of_128 >= 256; }
