@@ -344,34 +344,45 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_ortho_split(const T* __restrict__ g, const double* __restrict__ part, int n_part, OrtArgs p, float eps) {
   __shared__ double red[4];
   __shared__ float tile[64][65];
-  const int b = blockIdx.z;
+  const int b = blockIdx.z, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int rows = p.tall ? p.kp : p.rp, cols = p.tall ? p.rp : p.kp;  // of G's own orientation, padded
+  const int y0 = blockIdx.y * 64, x0 = blockIdx.x * 64;
+  g += (size_t)b * p.m * p.n;
+  T v[16];                                                            // sixteen loads in flight, under the sum of the squares
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const int gy = y0 + 4 * q + w, gx = x0 + lane;
+    v[q] = gy < p.m && gx < p.n ? g[(size_t)gy * p.n + gx] : (T)0.0f;
+  }
   double s = 0.0;
   for (int q = threadIdx.x; q < n_part; q += 256) s += part[b * n_part + q];
   const double f = ort_factor(ort_block_sum(s, red), eps);
-  g += (size_t)b * p.m * p.n;
-  const int rows = p.tall ? p.kp : p.rp, cols = p.tall ? p.rp : p.kp;  // of G's own orientation, padded
-  const int y0 = blockIdx.y * 64, x0 = blockIdx.x * 64;
-  _Float16* along = p.tall ? ort_xt(p, b, p.cur) : ort_x(p, b);        // [rows][cols]
-  _Float16* turned = p.tall ? ort_x(p, b) : ort_xt(p, b, p.cur);       // [cols][rows]
-  const int c = threadIdx.x & 63;
-  const bool flat_a = p.flat && p.tall, flat_t = p.flat && !p.tall;   // X^T for a single step of hi alone
-  for (int y = threadIdx.x >> 6; y < 64; y += 4) {
-    const int gy = y0 + y, gx = x0 + c;
-    const float v = gy < p.m && gx < p.n ? (float)((double)lf(g[(size_t)gy * p.n + gx]) * f) : 0.0f;
-    tile[y][c] = v;
-    _Float16 h, l;
-    ort_split(v, h, l);
-    const size_t at = flat_a ? (size_t)gy * cols + gx : ort_at(gy, gx, cols);
-    along[at] = h;
-    if (!flat_a) along[at + 32] = l;
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    const bool in = y0 + 4 * q + w < p.m && x0 + lane < p.n;          // (padding stays zero where the norm is not finite)
+    tile[4 * q + w][lane] = in ? (float)((double)lf(v[q]) * f) : 0.0f;
   }
   __syncthreads();
-  for (int y = threadIdx.x >> 6; y < 64; y += 4) {
-    _Float16 h, l;
-    ort_split(tile[c][y], h, l);
-    const size_t at = flat_t ? (size_t)(x0 + y) * rows + y0 + c : ort_at(x0 + y, y0 + c, rows);
-    turned[at] = h;
-    if (!flat_t) turned[at + 32] = l;
+  _Float16* along = p.tall ? ort_xt(p, b, p.cur) : ort_x(p, b);        // [rows][cols]
+  _Float16* turned = p.tall ? ort_x(p, b) : ort_xt(p, b, p.cur);       // [cols][rows]
+  const bool flat_a = p.flat && p.tall, flat_t = p.flat && !p.tall;   // X^T for a single step of hi alone
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {                                       // eight of a row of either: 16 bytes of hi, 16 of lo
+    const int y = (q & 1) * 32 + threadIdx.x / 8, x = threadIdx.x % 8 * 8;
+    f16x8 h, l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      _Float16 hh, ll;
+      ort_split(q < 2 ? tile[y][x + e] : tile[x + e][y], hh, ll);
+      h[e] = hh;
+      l[e] = ll;
+    }
+    _Float16* to = q < 2 ? along : turned;
+    const int row = (q < 2 ? y0 : x0) + y, col = (q < 2 ? x0 : y0) + x, ld = q < 2 ? cols : rows;
+    const bool flat = q < 2 ? flat_a : flat_t;
+    const size_t at = flat ? (size_t)row * ld + col : ort_at(row, col, ld);
+    *(f16x8*)(to + at) = h;
+    if (!flat) *(f16x8*)(to + at + 32) = l;
   }
 }
 
