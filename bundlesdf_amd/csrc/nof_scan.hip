@@ -177,7 +177,7 @@ __device__ __forceinline__ void scan_fold(float (&A)[V], float (&B)[V], float (&
 // The composition of a whole segment.  BACK: of the recurrence of what positions hand to the one before, c[t-1] = a[t] (dh[t] + c[t]).
 // The segment's slots take equal stretches of it, so that the only barrier is the last composition's.
 template <typename TG, typename T, int V, bool PC, bool BACK>
-__global__ __launch_bounds__(64 * SCAN_MAXW, 4) void k_scan_segments(ScanArgs p) {
+__global__ __launch_bounds__(64 * SCAN_MAXW, PC && V == 2 && sizeof(TG) == 4 ? 3 : 4) void k_scan_segments(ScanArgs p) {
   __shared__ float2 sh[SCAN_MAXW * 64 * V];
   const ScanWhere q = scan_where<V>(p);
   const int seg = BACK ? blockIdx.y + 1 : blockIdx.y;               // nobody needs the forward's last or the backward's first
@@ -188,13 +188,19 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, 4) void k_scan_segments(ScanArgs p)
   float A[V], B[V], TA[V], TB[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) { A[v] = 1.0f; B[v] = 0.0f; }
-  for (int k = 0; k < p.chunks_per_seg; ++k) {
-    const int64_t i = i0 + (int64_t)(BACK ? p.chunks_per_seg - 1 - k : k) * SCAN_U;
-    if (i >= q.n) continue;
-    ScanRaw<TG, PC ? V : 1> a[SCAN_U];
-    ScanRaw<T, V> r[SCAN_U];
-    scan_fetch<TG, PC ? V : 1>(g, i, q.n, full, 1.0f, a);
-    scan_fetch<T, V>(x, i, q.n, full, 0.0f, r);
+  // two runs of positions in turn, the next one's loads under way while one is composed
+  ScanRaw<TG, PC ? V : 1> a[2][SCAN_U];
+  ScanRaw<T, V> r[2][SCAN_U];
+  auto place = [&](int k) { return i0 + (int64_t)(BACK ? p.chunks_per_seg - 1 - k : k) * SCAN_U; };
+  auto fetch = [&](int k, auto& to, auto& too) {
+    const int64_t i = place(k);
+    if (k < p.chunks_per_seg && i < q.n) {
+      scan_fetch<TG, PC ? V : 1>(g, i, q.n, full, 1.0f, to);
+      scan_fetch<T, V>(x, i, q.n, full, 0.0f, too);
+    }
+  };
+  auto compose = [&](int k, const auto& a, const auto& r) {
+    if (k >= p.chunks_per_seg || place(k) >= q.n) return;
 #pragma unroll
     for (int t = 0; t < SCAN_U; ++t) {
       const int u = BACK ? SCAN_U - 1 - t : t;
@@ -205,6 +211,13 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, 4) void k_scan_segments(ScanArgs p)
         A[v] *= av;
       }
     }
+  };
+  fetch(0, a[0], r[0]);
+  for (int k = 0; k < p.chunks_per_seg; k += 2) {
+    fetch(k + 1, a[1], r[1]);
+    compose(k, a[0], r[0]);
+    fetch(k + 2, a[0], r[0]);
+    compose(k + 1, a[1], r[1]);
   }
   scan_wave<V, BACK>(A, B, p.cs, sh);
   __syncthreads();
