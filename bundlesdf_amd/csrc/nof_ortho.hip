@@ -9,11 +9,12 @@
 // weight), products hi hi + hi lo + lo hi accumulate in binary32: as exact as a binary32 product at a third of the fp16 rate, which on
 // this card is some three times the binary32 rate.  One fp16 product instead would be off by 2^-12 per step, which small singular values
 // amplify by up to a^steps: 4 % for a matrix of rank 4 plus noise of 1e-4.  The norm is summed in 64 bits: an error of it is common to all
-// values and the polynomial amplifies it.
+// values and the polynomial amplifies it.  Of at most 64 rows, A A is formed more exactly (ort_square).
 //
 // Matrices of at most 128 x 128 take one workgroup and one launch (k_ortho_small): X lives in accumulator registers, operands in LDS.
-// Thin ones, of at most 128 on one side, take a launch a step (k_ortho_thin).  Larger ones are three launches a step over images of X, X^T, A, P in the workspace, every product C = L R^T with both operands'
-// rows along the summed index, so X is stored in both orientations.
+// Thin ones, of at most 128 on one side, take a launch a step (k_ortho_thin).  Larger ones are three launches a step over images of X, X^T,
+// A, P in the workspace (four where the Gram product is cut, ort_cuts), every product C = L R^T with both operands' rows along the summed
+// index, so X is stored in both orientations.
 #include "nof_learn_dev.h"
 #include "nof_mfma_dev.h"
 #include <type_traits>
@@ -53,27 +54,95 @@ __device__ __forceinline__ double ort_factor(double sumsq, float eps) {
   return d == 0.0 ? 0.0 : (double)ORT_SCALE / d;
 }
 
+// Few rows leave little to average: an error of A A is one of all of X, and up to four steps amplify it.  So in matrices of at most 64 rows
+// the sums of the large parts and of what the small ones add are kept apart (the many small terms then cost the large sum no rounding), and
+// A A is more exact than pairs would give it: of 33 to 64 rows as products of three fp16 parts (33 bits), of at most 32 on the binary64 matrix
+// cores.  Relative error against 64 bits, 24 random matrices each: 9 x 287 2.8e-7 (as pairs 8.5e-7, a binary32 computation 5.9e-7), 32 x 500
+// 6e-7 (2.2e-6, 2.7e-6), 33 x 128 1.3e-6 (2.0e-6, 1.4e-6), 64 x 500 1.2e-6 (1.8e-6, 1.6e-6); from 65 rows on pairs are no worse than
+// binary32 (128 x 1000: 7e-7 and 1.7e-6).  64 x 64 on the binary64 cores: 33 us, as three parts 20, as pairs 18.
+enum { ORT_PAIRS, ORT_THREE, ORT_WIDE };
+__host__ __device__ constexpr int ort_square(int rt) { return rt == 1 ? ORT_WIDE : rt == 2 ? ORT_THREE : ORT_PAIRS; }
+__host__ __device__ constexpr int ort_parts(int rt) { return ort_square(rt) == ORT_THREE ? 3 : 2; }        // planes of A's image
+__device__ __forceinline__ void ort_split(float x, float less, _Float16& hi, _Float16& mid, _Float16& lo) {       // of x + less
+  hi = (_Float16)x;
+  const float rest = (x - (float)hi) + less;
+  mid = (_Float16)rest;
+  lo = (_Float16)(rest - (float)mid);
+}
+
+// P = ca I + cb A + cc A A of at most 32 rows, 16 x 16 blocks on and above the diagonal shared by `waves`; A in rows of ORT_WIDE_ROW (whose
+// loads touch every bank equally), P as pairs
+#define ORT_WIDE_ROW 36
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void ort_poly64(const double* a, int r, int w, int waves, int lane, float ca, float cb, float cc, _Float16* hi, _Float16* lo, int pitch) {
+  const int blocks = (r + 15) / 16, l15 = lane & 15, l4 = lane >> 4;
+  for (int t = w; t < blocks * (blocks + 1) / 2; t += waves) {
+    const int bi = t == 2, bj = t > 0;
+    const double *L = a + (16 * bi + l15) * ORT_WIDE_ROW + l4, *R = a + (16 * bj + l15) * ORT_WIDE_ROW + l4;
+    f64x4 s = {};
+    for (int k = 0; k < r; k += 16) {
+#pragma unroll
+      for (int q = 0; q < 16; q += 4) s = __builtin_amdgcn_mfma_f64_16x16x4f64(L[k + q], R[k + q], s, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = 16 * bi + 4 * e + l4, j = 16 * bj + l15;
+      const double v = (i == j ? (double)ca : 0.0) + (double)cb * a[i * ORT_WIDE_ROW + j] + (double)cc * s[e];
+      _Float16 h, l;
+      ort_split((float)(v * ORT_SCALE), h, l);
+      hi[j * pitch + i] = h;
+      lo[j * pitch + i] = l;
+      if (bi != bj) { hi[i * pitch + j] = h; lo[i * pitch + j] = l; }
+    }
+  }
+}
+// (P's image where it has no block meets zeros of X, and has to be a number there)
+__device__ __forceinline__ void ort_clear(_Float16* image, int halves, int tid, int threads) {
+  const f16x8 z = {};
+  for (int q = tid * 8; q < halves; q += threads * 8) *(f16x8*)(image + q) = z;
+}
+__device__ __forceinline__ void ort_mma3(f16x8 lh, f16x8 ll, f16x8 rh, f16x8 rl, f32x16& large, f32x16& small) {
+  small = PrecF16::mma(lh, rl, small);
+  small = PrecF16::mma(ll, rh, small);
+  large = PrecF16::mma(lh, rh, large);
+}
+
+// 32 x 32 tile of L R^T over 16 n columns, three parts each, planes apart
+__device__ __forceinline__ void ort_mma6(const _Float16* L, const _Float16* R, int plane, int n, f32x16& large, f32x16& small) {
+#pragma unroll 2
+  for (int q = 0; q < n; ++q) {
+    const f16x8 lh = *(const f16x8*)(L + 16 * q), lm = *(const f16x8*)(L + plane + 16 * q), ll = *(const f16x8*)(L + 2 * plane + 16 * q);
+    const f16x8 rh = *(const f16x8*)(R + 16 * q), rm = *(const f16x8*)(R + plane + 16 * q), rl = *(const f16x8*)(R + 2 * plane + 16 * q);
+    small = PrecF16::mma(lh, rl, small);
+    small = PrecF16::mma(ll, rh, small);
+    small = PrecF16::mma(lm, rm, small);
+    ort_mma3(lh, lm, rh, rm, large, small);
+  }
+}
+
 // ---- one workgroup a matrix -------------------------------------------------------------------------------------------------------
 // One wave per 32 x 32 tile of X (r <= k after the turn; tiles rt x KT).  LDS: two pairs of images, rows of 32 KT + 8 halves (the pad
 // spreads a column's 16-byte reads over all banks; known at compile time, or sixteen row offsets per store stay live and spill).  The first holds X for the Gram product and X^T for the last one, the second A, then P: symmetric, so their tiles are stored
-// turned, four halves at a time.  Bound by the chain of products, barriers and LDS round trips: 1.7 us a step for 16 x 16, 2.5 for 64 x 64,
-// 7.7 for 128 x 128 (half of it the matrix cores); four waves of 2 x 2 tiles instead of sixteen of one read half as much LDS and take 1.4
+// turned, four halves at a time.  Bound by the chain of products, barriers and LDS round trips: 1.7 us a step for 16 x 16, 3.2 for 64 x 64,
+// 8 for 128 x 128 (half of it the matrix cores); four waves of 2 x 2 tiles instead of sixteen of one read half as much LDS and take 1.4
 // times as long.
 struct OrtCoef { float c[3 * ORT_MAX_STEPS]; };
 
-template <typename T, int KT>
-__global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restrict__ g, T* __restrict__ out, int m, int n, int steps, OrtCoef coef, float eps) {
+// RT: rows of tiles at most
+template <typename T, int KT, int RT>
+__global__ __launch_bounds__(64 * KT * RT) void k_ortho_small(const T* __restrict__ g, T* __restrict__ out, int m, int n, int steps, OrtCoef coef, float eps) {
   extern __shared__ __attribute__((aligned(16))) char ort_lds[];
-  __shared__ double red[16];
+  constexpr int square = ort_square(RT);
+  __shared__ double red[16], a64[square == ORT_WIDE ? 32 * ORT_WIDE_ROW : 1];
   const bool tall = m > n;
-  const int r = tall ? n : m, k = tall ? m : n, rt = (r + 31) / 32;
+  const int r = tall ? n : m, k = tall ? m : n, rt = square != ORT_PAIRS ? RT : (r + 31) / 32;
   int tid = threadIdx.x;
   int hi = (tid >> 5) & 1, l31 = tid & 31, w = __builtin_amdgcn_readfirstlane(tid >> 6), ti = w / KT, tj = w % KT;      // rt * KT waves
   constexpr int px = 32 * KT + 8;
   _Float16* xh = (_Float16*)ort_lds;
   _Float16* xl = xh + 32 * KT * px;
   _Float16* ah = xl + 32 * KT * px;
-  _Float16* al = ah + 32 * KT * px;
+  _Float16* al = ah + 32 * RT * px;
   g += (size_t)blockIdx.x * m * n;
   out += (size_t)blockIdx.x * m * n;
   int j = 32 * tj + l31;
@@ -86,6 +155,7 @@ __global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restric
     x[e] = i < r && j < k ? lf(g[i * si + j * sj]) : 0.0f;
     s += (double)x[e] * (double)x[e];
   }
+  if (square == ORT_WIDE) ort_clear(ah, 2 * 32 * RT * px, tid, 64 * KT * RT);
   const double f = ort_factor(ort_block_sum(s, red), eps);
 #pragma unroll
   for (int e = 0; e < 16; ++e) x[e] = (float)((double)x[e] * f);
@@ -111,34 +181,55 @@ __global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restric
       ort_split(x[e], xh[at], xl[at]);
     }
     __syncthreads();
-    f32x16 acc = {}, sq = {};
+    const int li = (32 * ti + l31) * px + 8 * hi, ri = (32 * tj + l31) * px + 8 * hi, own = j * px + 32 * ti + 4 * hi;
+    f32x16 acc = {}, sq = {}, acc2 = {}, sq2 = {};                    // (acc2, sq2: what the small parts add)
     if (gram) {
-      #pragma unroll 2
+#pragma unroll 2
       for (int q = 0; q < 2 * KT; ++q) {
-        const int lo = (32 * ti + l31) * px + 16 * q + 8 * hi, ro = (32 * tj + l31) * px + 16 * q + 8 * hi;
-        acc = ort_mma3(*(const f16x8*)(xh + lo), *(const f16x8*)(xl + lo), *(const f16x8*)(xh + ro), *(const f16x8*)(xl + ro), acc);
+        const f16x8 lh = *(const f16x8*)(xh + li + 16 * q), ll = *(const f16x8*)(xl + li + 16 * q), rh = *(const f16x8*)(xh + ri + 16 * q), rl = *(const f16x8*)(xl + ri + 16 * q);
+        if (square != ORT_PAIRS) ort_mma3(lh, ll, rh, rl, acc, acc2);
+        else acc = ort_mma3(lh, ll, rh, rl, acc);
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[e] *= 1.0f / ORT_SCALE;         // 4096 A
-      put(ah, al, acc);
+      for (int e = 0; e < 16; ++e) { acc[e] *= 1.0f / ORT_SCALE; acc2[e] *= 1.0f / ORT_SCALE; }     // 4096 A
+      if (square == ORT_WIDE) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) a64[l31 * ORT_WIDE_ROW + nloc(hi, e)] = ((double)acc[e] + (double)acc2[e]) * (1.0 / ORT_SCALE);
+      } else if (square == ORT_THREE) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          f16x4 h4, m4, l4;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { _Float16 h, m, l; ort_split(acc[4 * q + e], acc2[4 * q + e], h, m, l); h4[e] = h; m4[e] = m; l4[e] = l; }
+          *(f16x4*)(ah + own + 8 * q) = h4;
+          *(f16x4*)(al + own + 8 * q) = m4;
+          *(f16x4*)(al + 32 * RT * px + own + 8 * q) = l4;
+        }
+      } else {
+        put(ah, al, acc);
+      }
     }
     __syncthreads();                                                  // X has been read, A is there
     put(xh, xl, x);                                                   // X^T over X
-    if (gram) {
+    if (square == ORT_WIDE) {
+      ort_poly64(a64, r, w, KT, tid & 63, ca, cb, cc, ah, al, px);
+    } else {
+      if (square == ORT_THREE && gram) ort_mma6(ah + li, ah + ri, 32 * RT * px, 2 * rt, sq, sq2);
+      else if (gram) {
 #pragma unroll 2
-      for (int q = 0; q < 2 * rt; ++q) {
-        const int lo = (32 * ti + l31) * px + 16 * q + 8 * hi, ro = (32 * tj + l31) * px + 16 * q + 8 * hi;
-        sq = ort_mma3(*(const f16x8*)(ah + lo), *(const f16x8*)(al + lo), *(const f16x8*)(ah + ro), *(const f16x8*)(al + ro), sq);
+        for (int q = 0; q < 2 * rt; ++q)
+          sq = ort_mma3(*(const f16x8*)(ah + li + 16 * q), *(const f16x8*)(al + li + 16 * q), *(const f16x8*)(ah + ri + 16 * q), *(const f16x8*)(al + ri + 16 * q), sq);
       }
-    }
-    __syncthreads();                                                  // A has been read
-    if (gram) {
+      __syncthreads();                                                // A has been read
+      if (gram) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int i = 32 * ti + nloc(hi, e);
-        acc[e] = (i == j ? ca * ORT_SCALE : 0.0f) + cb * acc[e] + cc * (sq[e] * (1.0f / ORT_SCALE));
+        for (int e = 0; e < 16; ++e) {
+          const float one = 32 * ti + nloc(hi, e) == j ? ca * ORT_SCALE : 0.0f;
+          if (square == ORT_THREE) acc[e] = (one + cb * acc[e] + cc * (sq[e] * (1.0f / ORT_SCALE))) + (cb * acc2[e] + cc * (sq2[e] * (1.0f / ORT_SCALE)));
+          else acc[e] = one + cb * acc[e] + cc * (sq[e] * (1.0f / ORT_SCALE));
+        }
+        put(ah, al, acc);
       }
-      put(ah, al, acc);
     }
     __syncthreads();
     f32x16 y = {};
@@ -164,8 +255,8 @@ __global__ __launch_bounds__(64 * KT * KT) void k_ortho_small(const T* __restric
 // At most 128 on the shorter side, more on the longer: a launch a step instead of three.  A workgroup owns a stretch of X's columns, 128 at a
 // time through LDS, and knows the Gram matrix as the sum of all workgroups' parts of it, which the launch before left behind: it forms A and
 // P for itself, then X <- P X of its columns and the new part.  X stays in memory as the accumulators hold it.  Parts are added in the order
-// of the workgroups.  64 x 1000 fp32: 49 us (109 as tiles of the larger matrices, whose Gram product is one tile's chain over the long side),
-// 64 x 16384: 130 us (599), 128 x 4096: 141 us (222).
+// of the workgroups.  64 x 1000 fp32: 50 us (109 as tiles of the larger matrices, whose Gram product is one tile's chain over the long side),
+// 64 x 16384: 119 us (599), 128 x 4096: 141 us (222).
 struct OrtThin {
   const double* part; int n_part;
   float* x; const float* gram_in; float* gram_out;
@@ -199,7 +290,8 @@ __device__ __forceinline__ f32x16 ort_tile_product(const _Float16* L, int dl, co
 template <typename T, int RT, int MODE>
 __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g, T* __restrict__ out, OrtThin p) {
   extern __shared__ __attribute__((aligned(16))) char ort_lds[];
-  __shared__ double red[4 * RT];
+  constexpr int square = ort_square(RT);
+  __shared__ double red[4 * RT], a64[square == ORT_WIDE ? 32 * ORT_WIDE_ROW : 1];
   constexpr int PX = 136, PA = 32 * RT + 8, plane_x = 128 * PA > 32 * RT * PX ? 128 * PA : 32 * RT * PX, plane_a = 32 * RT * PA;
   _Float16* X = (_Float16*)ort_lds;                                   // X [32 RT][PX] or X^T [128][PA]
   _Float16* A = X + 2 * plane_x;                                      // A, then P, [32 RT][PA]
@@ -225,6 +317,66 @@ __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g
     double s = 0.0;
     for (int q = tid; q < p.n_part; q += 256 * RT) s += p.part[b * p.n_part + q];
     f = ort_factor(ort_block_sum(s, red), p.eps);
+  } else if constexpr (square != ORT_PAIRS) {
+    double a[4 * RT];                                                 // a tile of A by 4 / RT waves
+#pragma unroll
+    for (int e = 0; e < 4 * RT; ++e) a[e] = 0.0;
+    const int tile = w * RT / 4, first = w * RT % 4;
+    const float* in = p.gram_in + ((size_t)b * p.blocks * RT * RT + tile) * 1024 + first * 256 + lane * 4;
+#pragma unroll 2
+    for (int q = 0; q < p.blocks; q += 4) {                           // four in binary32: conversions to 64 bits are slow (64 x 16384: 119 us, 182 without)
+#pragma unroll
+      for (int c = 0; c < RT; ++c) {
+        float4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = q + u < p.blocks ? *(const float4*)(in + (size_t)(q + u) * RT * RT * 1024 + c * 256) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        a[4 * c] += (double)((v[0].x + v[1].x) + (v[2].x + v[3].x));
+        a[4 * c + 1] += (double)((v[0].y + v[1].y) + (v[2].y + v[3].y));
+        a[4 * c + 2] += (double)((v[0].z + v[1].z) + (v[2].z + v[3].z));
+        a[4 * c + 3] += (double)((v[0].w + v[1].w) + (v[2].w + v[3].w));
+      }
+    }
+    if constexpr (square == ORT_WIDE) {
+      ort_clear(A, 2 * plane_a, tid, 256 * RT);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a64[l31 * ORT_WIDE_ROW + nloc(hi, 4 * w + e)] = a[e] * (1.0 / ORT_SCALE);
+      __syncthreads();
+      ort_poly64(a64, p.r, w, 4, lane, p.ca, p.cb, p.cc, A, A + plane_a, PA);
+    } else {
+#pragma unroll
+      for (int c = 0; c < RT; ++c) {
+        f16x4 h4, m4, l4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = (float)a[4 * c + e];
+          _Float16 h, m, l;
+          ort_split(x, (float)(a[4 * c + e] - (double)x), h, m, l);
+          h4[e] = h; m4[e] = m; l4[e] = l;
+        }
+        _Float16* at = A + (tile % RT * 32 + l31) * PA + tile / RT * 32 + 8 * (first + c) + 4 * hi;
+        *(f16x4*)at = h4;
+        *(f16x4*)(at + plane_a) = m4;
+        *(f16x4*)(at + 2 * plane_a) = l4;
+      }
+      __syncthreads();
+      f32x16 sq = {}, sq2 = {}, pp;
+      if (gram) {
+        ort_mma6(A + (32 * ti + l31) * PA + 8 * hi, A + (32 * tj + l31) * PA + 8 * hi, plane_a, 2 * RT, sq, sq2);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const _Float16* at = A + (32 * tj + l31) * PA + 32 * ti + 8 * q + 4 * hi;
+          const f16x4 h4 = *(const f16x4*)at, m4 = *(const f16x4*)(at + plane_a), l4 = *(const f16x4*)(at + 2 * plane_a);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float one = 32 * ti + nloc(hi, 4 * q + e) == 32 * tj + l31 ? p.ca * ORT_SCALE : 0.0f;
+            pp[4 * q + e] = (one + p.cb * (float)h4[e] + p.cc * (sq[4 * q + e] * (1.0f / ORT_SCALE))) +
+                          (p.cb * ((float)m4[e] + (float)l4[e]) + p.cc * (sq2[4 * q + e] * (1.0f / ORT_SCALE)));
+          }
+        }
+      }
+      __syncthreads();                                                  // A has been read
+      if (gram) put(A, plane_a, 32 * tj + l31, pp);
+    }
   } else {
     float a[16];
     f32x16 sq = {};
@@ -251,7 +403,7 @@ __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g
       put(A, plane_a, 32 * tj + l31, a);
     }
   }
-  f32x16 part = {};
+  f32x16 part = {}, less = {};                                        // (what the small parts add, by itself but for ORT_PAIRS)
   for (int c = 0; c < p.chunks; ++c) {
     asm volatile("" : "+v"(tid));                                     // (no instruction: lane places are formed in the loop, not before it and spilled)
     lane = tid & 63; hi = lane >> 5; l31 = lane & 31;
@@ -288,13 +440,20 @@ __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g
 #pragma unroll
       for (int e = 0; e < 16; ++e) ort_split(x[e], to[nloc(0, e) * PX], to[plane_x + nloc(0, e) * PX]);
       __syncthreads();
-      if (gram) part = ort_tile_product(X + (32 * ti + l31) * PX + 8 * hi, plane_x, X + (32 * tj + l31) * PX + 8 * hi, plane_x, 8, part);
+      if (square != ORT_PAIRS && gram) {
+        const _Float16 *L = X + (32 * ti + l31) * PX + 8 * hi, *R = X + (32 * tj + l31) * PX + 8 * hi;
+#pragma unroll 2
+        for (int q = 0; q < 8; ++q)
+          ort_mma3(*(const f16x8*)(L + 16 * q), *(const f16x8*)(L + plane_x + 16 * q), *(const f16x8*)(R + 16 * q), *(const f16x8*)(R + plane_x + 16 * q), part, less);
+      } else if (gram) {
+        part = ort_tile_product(X + (32 * ti + l31) * PX + 8 * hi, plane_x, X + (32 * tj + l31) * PX + 8 * hi, plane_x, 8, part);
+      }
       __syncthreads();
     }
   }
   if (MODE != ORT_FINAL && gram) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) part[e] *= 1.0f / ORT_SCALE;         // 4096 of A
+    for (int e = 0; e < 16; ++e) part[e] = (square != ORT_PAIRS ? part[e] + less[e] : part[e]) * (1.0f / ORT_SCALE);         // 4096 of A
     ort_tile_store(p.gram_out + (((size_t)b * p.blocks + block) * RT * RT + ti * RT + tj) * 1024, lane, part);
   }
 }
@@ -710,7 +869,7 @@ typedef OrtShape<2, 2, 1, 1, 2, 1> OrtSingle;                          // the jo
 // Five steps of 200 x 4096: 255 us uncut, 153 cut; 600 x 2900: 282 and 241; 333 x 1001, 3 of them: 174 and 170.  Below 1024 the join costs
 // more than the parts save (512 x 512: 146 and 154), and so it does with many tiles of a middling length (1024 x 1024: 209 and 221;
 // 1024 x 2048: 285 either way; 1024 x 4096: 435 and 424).  Parts of four stages gain nothing (200 x 4096: 171).
-static int ort_split(int64_t batch, int64_t rp, int64_t kp) {
+static int ort_cuts(int64_t batch, int64_t rp, int64_t kp) {
   const int64_t n = rp / 64, tiles = batch * n * (n + 1) / 2, most = kp / 256, want = 512 / tiles;
   if (kp < 1024 || want < 2 || kp * want < 6144) return 1;
   return (int)(want < most ? want : most);
@@ -737,18 +896,18 @@ extern "C" int64_t nof_orthogonalize_workspace_bytes(int64_t batch, int64_t m, i
     return learn_align(batch * ORT_NORM_BLOCKS * 8) + batch * blocks * (chunks * rt * 4 + 2 * rt * rt) * 4096;
   }
   const int64_t r = m < n ? m : n, k = m < n ? n : m, unit = ort_unit(batch, r, k), rp = ort_up(r, unit), kp = ort_up(k, unit);
-  const int64_t split = ort_split(batch, rp, kp), side = rp / 64;
+  const int64_t split = ort_cuts(batch, rp, kp), side = rp / 64;
   return learn_align(batch * ORT_NORM_BLOCKS * 8) + batch * (6 * rp * kp + 4 * rp * rp) * 2 + (split > 1 ? batch * side * (side + 1) / 2 * split * 64 * 64 * 4 : 0);
 }
 
-template <typename T, int KT>
+template <typename T, int KT, int RT>
 static void ort_launch_small(const void* g, void* out, int64_t batch, int64_t m, int64_t n, int32_t steps, const float* coef, float eps, hipStream_t st) {
   OrtCoef c = {};
   for (int i = 0; i < 3 * steps; ++i) c.c[i] = coef[i];
   const int rt = (int)nof_div_up(m < n ? m : n, 32);
-  constexpr size_t lds = (size_t)4 * 2 * 32 * KT * (32 * KT + 8);    // 136 KiB for KT = 4
-  if (lds > 64 << 10) (void)hipFuncSetAttribute((const void*)&k_ortho_small<T, KT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  hipLaunchKernelGGL((k_ortho_small<T, KT>), dim3((unsigned)batch), dim3(64 * rt * KT), lds, st, (const T*)g, (T*)out, (int)m, (int)n, steps, c, eps);
+  constexpr size_t lds = (size_t)2 * 32 * (2 * KT + ort_parts(RT) * RT) * (32 * KT + 8);      // 136 KiB for KT = RT = 4
+  if (lds > 64 << 10) (void)hipFuncSetAttribute((const void*)&k_ortho_small<T, KT, RT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  hipLaunchKernelGGL((k_ortho_small<T, KT, RT>), dim3((unsigned)batch), dim3(64 * rt * KT), lds, st, (const T*)g, (T*)out, (int)m, (int)n, steps, c, eps);
 }
 
 template <int MODE, typename S> static int64_t ort_tiles(const OrtArgs& p) {
@@ -789,7 +948,7 @@ static int ort_launch_norm(const void* g, double* part, int64_t batch, int64_t m
 template <typename T, int RT, int MODE>
 static void ort_thin_step(const void* g, void* out, const OrtThin& p, int64_t batch, hipStream_t st) {
   constexpr int px = 128 * (32 * RT + 8) > 32 * RT * 136 ? 128 * (32 * RT + 8) : 32 * RT * 136;
-  constexpr size_t lds = 2 * 2 * (size_t)(px + 32 * RT * (32 * RT + 8));                              // 136 KiB for RT = 4
+  constexpr size_t lds = 2 * (size_t)(2 * px + ort_parts(RT) * 32 * RT * (32 * RT + 8));                              // 136 KiB for RT = 4
   if (lds > 64 << 10) (void)hipFuncSetAttribute((const void*)&k_ortho_thin<T, RT, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   hipLaunchKernelGGL((k_ortho_thin<T, RT, MODE>), dim3((unsigned)(batch * p.blocks)), dim3(256 * RT), lds, st, (const T*)g, (T*)out, p);
 }
@@ -822,10 +981,10 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
   const int64_t r = m < n ? m : n, k = m < n ? n : m;
   if (ort_is_small(m, n)) {
     const int kt = (int)nof_div_up(k, 32);
-    if (kt == 1) ort_launch_small<T, 1>(g, out, batch, m, n, steps, coef, eps, st);
-    else if (kt == 2) ort_launch_small<T, 2>(g, out, batch, m, n, steps, coef, eps, st);
-    else if (kt == 3) ort_launch_small<T, 3>(g, out, batch, m, n, steps, coef, eps, st);
-    else ort_launch_small<T, 4>(g, out, batch, m, n, steps, coef, eps, st);
+    auto small = r > 64 ? (kt == 3 ? ort_launch_small<T, 3, 3> : ort_launch_small<T, 4, 4>)
+               : r > 32 ? (kt == 2 ? ort_launch_small<T, 2, 2> : kt == 3 ? ort_launch_small<T, 3, 2> : ort_launch_small<T, 4, 2>)
+               : kt == 1 ? ort_launch_small<T, 1, 1> : kt == 2 ? ort_launch_small<T, 2, 1> : kt == 3 ? ort_launch_small<T, 3, 1> : ort_launch_small<T, 4, 1>;
+    small(g, out, batch, m, n, steps, coef, eps, st);
     return;
   }
   if (ort_is_thin(m, n)) {
@@ -845,7 +1004,7 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
   p.flat = light && steps == 1;
   double* part = (double*)workspace;
   p.ws = (_Float16*)((char*)workspace + learn_align(batch * ORT_NORM_BLOCKS * 8));
-  p.split = ort_split(batch, p.rp, p.kp);
+  p.split = ort_cuts(batch, p.rp, p.kp);
   p.parts = (float*)(p.ws + batch * p.per);
   const unsigned nb = (unsigned)batch;
   const int n_part = ort_launch_norm<T>(g, part, batch, m, n, st);
