@@ -33,7 +33,7 @@ template <int SIZE> struct EmbAt;
 template <> struct EmbAt<2> { typedef emb_u4 t __attribute__((aligned(2))); };
 template <> struct EmbAt<4> { typedef emb_u4 t __attribute__((aligned(4))); };
 template <typename T> using EmbBits = typename EmbAt<sizeof(T)>::t;
-// ONCE: past the caches, for what is read only here (the gradient's rows: the table's stay, a lookup behind it takes 60 us instead of 84)
+// ONCE: past the caches, for what is read only here and is too large to lie in them from its making (the gradient's rows: emb_launch_sums)
 template <typename T, int V, bool ONCE>
 __device__ __forceinline__ void emb_load(const T* __restrict__ p, int n, float (&f)[V]) {
   if (n >= V) {
@@ -279,7 +279,7 @@ __device__ __forceinline__ void emb_put(T* __restrict__ grad, int64_t row, int D
 }
 
 // part [chunk][2][DP], DP = D up to a multiple of 8: the sum of the id that a run inherits from the run before it, and of the one that it starts and hands on
-template <typename T>
+template <typename T, bool ONCE>
 __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ dout, int64_t stride, const uint32_t* __restrict__ key,
                                                         const uint32_t* __restrict__ pos, uint32_t N, uint32_t rows, int D, float scale,
                                                         T* __restrict__ grad, float* __restrict__ part, int ls, int C, uint32_t n_red) {
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       kk[u] = i + u < hi ? key[i + u] : rows;
-      if (kk[u] < rows) emb_load<T, V, true>(dout + (int64_t)pos[i + u] * stride + col, D - col, x[u]);
+      if (kk[u] < rows) emb_load<T, V, ONCE>(dout + (int64_t)pos[i + u] * stride + col, D - col, x[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -458,8 +458,11 @@ static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* ke
   const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
   const unsigned cols = (unsigned)nof_div_up(nv, (int64_t)1 << ls), n_red = (unsigned)nof_div_up(p.chunks, EMB_T >> ls);
   const unsigned n_zero = (unsigned)nof_div_up(p.s.rows, EMB_ZROWS);
-  hipLaunchKernelGGL(k_embed_reduce<T>, dim3(n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N,
-                     (uint32_t)p.s.rows, D, scale, (T*)grad, part, ls, p.C, n_red);
+  // dout past the caches from half of the last one (256 MB) on.  65536 x 2048 bf16: the table's rows stay, a lookup behind it takes 60 us
+  // instead of 84; 8192 x 1024: the launch takes 30 us so, 20 through the caches, where dout still lies.
+  auto reduce = (int64_t)p.s.N * D * (int64_t)sizeof(T) >= (int64_t)128 << 20 ? k_embed_reduce<T, true> : k_embed_reduce<T, false>;
+  hipLaunchKernelGGL(reduce, dim3(n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N, (uint32_t)p.s.rows, D, scale,
+                     (T*)grad, part, ls, p.C, n_red);
   if (p.chunks > 1) {
     const int64_t jv = nof_div_up(D, 4);
     const int jl = learn_log2_up(jv < 64 ? jv : 64);
