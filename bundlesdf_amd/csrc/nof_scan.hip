@@ -108,16 +108,16 @@ template <typename T, int V> __device__ __forceinline__ ScanRaw<T, V> scan_fill(
 }
 
 // SCAN_U positions from i0 on of n > 0; positions from n on are `fill` (their loads go to the last row: a branch per row, or a predicate
-// per row and array, costs the compiler its registers)
+// per row and array, costs the compiler its registers).  The choice is each slot's: made for a whole segment, 24 x 1777 x 520 of uneven
+// lengths took 18 us to compose, 12 so.
 template <typename T, int V>
-__device__ __forceinline__ void scan_fetch(const ScanRows<const T>& x, int64_t i0, int64_t n, bool full, float fill, ScanRaw<T, V> (&r)[SCAN_U]) {
+__device__ __forceinline__ void scan_fetch(const ScanRows<const T>& x, int64_t i0, int64_t n, float fill, ScanRaw<T, V> (&r)[SCAN_U]) {
   const T* p = x.at(i0);
-  const int64_t st = x.stride();
-  if (full) {
+  const int64_t st = x.stride(), left = n - i0;
+  if (left >= SCAN_U) {
 #pragma unroll
     for (int u = 0; u < SCAN_U; ++u) r[u] = *reinterpret_cast<const ScanRaw<T, V>*>(p + u * st);
   } else {
-    const int64_t left = n - i0;
 #pragma unroll
     for (int u = 0; u < SCAN_U; ++u) {
       const ScanRaw<T, V> in = *reinterpret_cast<const ScanRaw<T, V>*>(p + (u < left ? u : left - 1) * st), out = scan_fill<T, V>(fill);
@@ -184,7 +184,6 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, PC && V == 2 && sizeof(TG) == 4 ? 3
   const ScanRows<const TG> g((const TG*)p.gate + q.b * p.gate_sb + (PC ? q.ch : q.ch / p.P), p.gate_st, p, q.n);
   const ScanRows<const T> x(BACK ? (const T*)p.dh + q.b * p.dh_sb + q.ch : (const T*)p.value + q.b * p.value_sb + q.ch, BACK ? p.dh_st : p.value_st, p, q.n);
   const int64_t seg0 = (int64_t)seg * p.chunks_per_seg * p.chunk, each = (int64_t)p.chunks_per_seg * SCAN_U, i0 = seg0 + q.slot * each;
-  const bool full = seg0 + (int64_t)p.chunks_per_seg * p.chunk <= q.n;
   float A[V], B[V], TA[V], TB[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) { A[v] = 1.0f; B[v] = 0.0f; }
@@ -195,8 +194,8 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, PC && V == 2 && sizeof(TG) == 4 ? 3
   auto fetch = [&](int k, auto& to, auto& too) {
     const int64_t i = place(k);
     if (k < p.chunks_per_seg && i < q.n) {
-      scan_fetch<TG, PC ? V : 1>(g, i, q.n, full, 1.0f, to);
-      scan_fetch<T, V>(x, i, q.n, full, 0.0f, too);
+      scan_fetch<TG, PC ? V : 1>(g, i, q.n, 1.0f, to);
+      scan_fetch<T, V>(x, i, q.n, 0.0f, too);
     }
   };
   auto compose = [&](int k, const auto& a, const auto& r) {
@@ -278,13 +277,13 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, 3) void k_scan_fwd(ScanArgs p) {
   ScanRaw<T, V> r[SCAN_U];
   const int64_t at0 = (int64_t)c0 * p.chunk;
   if (at0 < q.n) {
-    scan_fetch<TG, PC ? V : 1>(g, at0 + q.slot * SCAN_U, q.n, at0 + p.chunk <= q.n, 1.0f, a);
-    scan_fetch<T, V>(x, at0 + q.slot * SCAN_U, q.n, at0 + p.chunk <= q.n, 0.0f, r);
+    scan_fetch<TG, PC ? V : 1>(g, at0 + q.slot * SCAN_U, q.n, 1.0f, a);
+    scan_fetch<T, V>(x, at0 + q.slot * SCAN_U, q.n, 0.0f, r);
   }
   scan_over<V>(p, q, 0, 1, seg, S, sh[0]);
   for (int c = c0; c < c1; ++c) {
     const int64_t at = (int64_t)c * p.chunk, i0 = at + q.slot * SCAN_U;
-    const bool full = at + p.chunk <= q.n;
+    const bool full = i0 + SCAN_U <= q.n;
     if (at < q.n) {
       float A[V], B[V], TA[V], TB[V], s[V];
 #pragma unroll
@@ -321,8 +320,8 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, 3) void k_scan_fwd(ScanArgs p) {
       // (positions behind the end keep the state)
       if (p.last && q.on && i0 < q.n && i0 + SCAN_U >= q.n) lstore<float, V>(p.last + (int64_t)q.b * p.D + q.ch, s);
       if (c + 1 < c1 && at + p.chunk < q.n) {
-        scan_fetch<TG, PC ? V : 1>(g, i0 + p.chunk, q.n, at + 2 * p.chunk <= q.n, 1.0f, a);
-        scan_fetch<T, V>(x, i0 + p.chunk, q.n, at + 2 * p.chunk <= q.n, 0.0f, r);
+        scan_fetch<TG, PC ? V : 1>(g, i0 + p.chunk, q.n, 1.0f, a);
+        scan_fetch<T, V>(x, i0 + p.chunk, q.n, 0.0f, r);
       }
     }
     if (h0 && q.on && !full) {                                        // rows behind the sequence's end
@@ -381,14 +380,14 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, PC || V == 1 ? 3 : 2) void k_scan_b
   scan_over<V>(p, q, p.segs - 1, -1, p.segs - 1 - seg, R, sh[0][0]);
   for (int c = c1 - 1; c >= c0; --c) {
     const int64_t at = (int64_t)c * p.chunk, i0 = at + q.slot * SCAN_U;
-    const bool full = at + p.chunk <= q.n;
+    const bool full = i0 + SCAN_U <= q.n;
     if (at < q.n) {
       ScanRaw<TG, PC ? V : 1> a[SCAN_U];
       ScanRaw<T, V> r[SCAN_U], d[SCAN_U];
       float A[V], B[V], A2[V], B2[V], TA[V], TB[V], m[V], s[V], hp[SCAN_U][V];
-      scan_fetch<TG, PC ? V : 1>(g, i0, q.n, full, 1.0f, a);
-      scan_fetch<T, V>(x, i0, q.n, full, 0.0f, r);
-      scan_fetch<T, V>(y, i0, q.n, full, 0.0f, d);
+      scan_fetch<TG, PC ? V : 1>(g, i0, q.n, 1.0f, a);
+      scan_fetch<T, V>(x, i0, q.n, 0.0f, r);
+      scan_fetch<T, V>(y, i0, q.n, 0.0f, d);
       lload<float, V>(p.marks + ((int64_t)q.b * p.n_marks + c) * p.D + q.ch, m);
 #pragma unroll
       for (int v = 0; v < V; ++v) { A[v] = 1.0f; B[v] = 0.0f; B2[v] = 0.0f; }
