@@ -48,7 +48,7 @@ __device__ __forceinline__ void emb_load(const T* __restrict__ p, int n, float (
   }
 }
 // a store past the caches: nothing here reads it again, and the rows that are read stay (65536 x 2048 bf16 looked up: 59 us, 91 without;
-// the gradient of a 131072-row table by them 222 us, 248 without)
+// the gradient of a 131072-row table by them 227 us, 248 without)
 template <typename T, int V>
 __device__ __forceinline__ void emb_store(T* __restrict__ p, int n, const float (&f)[V]) {
   if (n >= V) {
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
 
 // The run in which a cut id starts adds what the runs behind it inherited: a workgroup per run and slice of at most 64 x V columns, whose
 // groups of lanes each add a stretch of the runs; their sums meet in LDS, neighbours first.  (One group for all of an id that many runs hold
-// is a chain of loads: 17 us of the 222 above, 8 so.)
+// is a chain of loads: 17 us of the large table's 227, 8 so.)
 template <typename T>
 __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict__ key, uint32_t N, uint32_t rows, int D, float scale,
                                                       T* __restrict__ grad, const float* __restrict__ part, int ls, int C) {

@@ -508,8 +508,8 @@ __global__ __launch_bounds__(256) void k_scan_step(const TG* __restrict__ gate, 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 // Everything here depends on the sizes alone, so that the forward's marks fit the backward.
 // Segments: from one wave per SIMD (1024 waves) on, a workgroup's own look-ahead keeps the memory busy and a second pass over the inputs
-// would cost more than it gives; below, two waves per SIMD, of two chunks at least.  4 x 16384 x 1024 bf16, forward + backward: 114 + 185 us
-// so, 122 + 198 with four waves per SIMD, 162 + 231 with one.
+// would cost more than it gives; below, two waves per SIMD, of two chunks at least.  4 x 16384 x 1024 bf16, forward + backward: 111 + 177 us
+// so, 123 + 192 with four waves per SIMD, 154 + 209 with one.
 static void scan_layout(ScanArgs& p, int span, int v) {
   p.span = span;
   const int nv = span / v;
