@@ -10,6 +10,7 @@
 //      them and writes the sum of every id that lies within the run; an id cut by the run's ends leaves a partial sum.  Further
 //      workgroups of the same launch write the zeros of the rows that no id names -- most of the bytes of a large table;
 //   3. k_embed_join: the partial sums of a cut id, in the order of their runs.
+// Few positions of few rows take one launch instead (k_embed_few).
 #include "nof_learn_dev.h"
 
 #define EMB_T 256                       // threads of the streaming kernels
@@ -19,6 +20,7 @@
 #define EMB_SORT_W (EMB_SORT_T / 64)
 #define EMB_BITS 10                     // widest digit of the many-workgroup sort
 #define EMB_MAX_BLOCKS 128
+#define EMB_FEW_N 4096                  // positions that k_embed_few lists
 
 // ---- lookup -----------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ int64_t emb_id(const void* __restrict__ ids, int ids64, int64_t i) {
@@ -399,6 +401,71 @@ __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict
   }
 }
 
+// ---- few rows, few positions ------------------------------------------------------------------------------------------------------
+// One launch, no sort: a workgroup per table row and slice of the columns looks all ids over -- its waves a stretch each, keeping the
+// positions that name the row in their order --, then its groups of lanes add a stretch of them each and their sums meet in LDS.  64 rows,
+// 4096 positions of 16 fp32: 9 us, where the sort, its sums and their join take 18.
+template <typename T>
+__global__ __launch_bounds__(EMB_T) void k_embed_few(const T* __restrict__ dout, int64_t stride, const void* __restrict__ ids, int ids64, int N, int D,
+                                                     float scale, T* __restrict__ grad, int ls) {
+  constexpr int V = EmbVec<T>::V, W = EMB_T / 64;
+  __shared__ uint16_t list[EMB_FEW_N + 64 * W];
+  __shared__ int counts[W];
+  __shared__ float sums[EMB_T * V];
+  const int row = blockIdx.x, w = threadIdx.x >> 6, l64 = threadIdx.x & 63;
+  const int per_wave = (N + EMB_T - 1) / EMB_T * 64, lo = w * per_wave, hi = lo + per_wave < N ? lo + per_wave : N;
+  int count = 0;
+#pragma unroll 8
+  for (int base = lo; base < hi; base += 64) {
+    const int i = base + l64;
+    const bool mine = i < hi && emb_id(ids, ids64, i) == row;
+    const uint64_t all = __ballot(mine);
+    if (mine) list[lo + count + __popcll(all & (((uint64_t)1 << l64) - 1))] = (uint16_t)i;
+    count += __popcll(all);
+  }
+  if (l64 == 0) counts[w] = count;
+  __syncthreads();
+  int total = 0, ends[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) { total += counts[k]; ends[k] = total; }
+  const int lane = threadIdx.x & ((1 << ls) - 1), group = threadIdx.x >> ls, groups = EMB_T >> ls;
+  const int col = (((int)blockIdx.y << ls) + lane) * V;
+  const int each = (total + groups - 1) / groups, m0 = group * each, m1 = m0 + each < total ? m0 + each : total;
+  float acc[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+  if (col < D) {
+    constexpr int U = 8;                                              // rows in flight per group
+    for (int m = m0; m < m1; m += U) {
+      float x[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int q = m + u < m1 ? m + u : m1 - 1;
+        int at = q;                                                   // of the concatenated lists
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k)
+          if (q >= ends[k]) at = q - ends[k] + (k + 1) * per_wave;
+        emb_load<T, V, false>(dout + (int64_t)list[at] * stride + col, D - col, x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] += m + u < m1 ? x[u][k] : 0.0f;
+    }
+  }
+  for (int o = 1; o < groups && o <= total; o *= 2) {                 // (groups behind the last position hold zeros)
+#pragma unroll
+    for (int k = 0; k < V; ++k) sums[threadIdx.x * V + k] = acc[k];
+    __syncthreads();
+    if ((group & (2 * o - 1)) == 0 && group + o < groups) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] += sums[(threadIdx.x + (o << ls)) * V + k];
+    }
+    __syncthreads();
+  }
+  if (group == 0 && col < D) emb_put<T, V>(grad, row, D, col, scale, acc);
+}
+
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 // sorted positions per run: long where there is work for every compute unit anyway, short where a run is the critical path
 static int emb_chunk(int64_t N, int32_t D) {
@@ -406,14 +473,24 @@ static int emb_chunk(int64_t N, int32_t D) {
   return e >= (int64_t)1 << 26 ? 64 : e >= (int64_t)1 << 24 ? 32 : e >= (int64_t)1 << 22 ? 16 : 8;
 }
 
-struct EmbPlan { EmbSort s; bool small; int64_t key[2], pos[2], hist, part, bytes; int C; uint32_t chunks; };
+struct EmbPlan { EmbSort s; bool few, small; int64_t key[2], pos[2], hist, part, bytes; int C; uint32_t chunks; };
+
+// k_embed_few: every row's workgroups look all ids over, so few positions and rows x slices.  Against the sort: 4096 positions, 64 rows of 16
+// fp32 9 us and 18 (15 and 21 if all name one row), 4096 rows of 32 16 and 24, 8000 of 16 25 and 24; 256 positions, 16000 rows 13 and 16;
+// 8192 positions of 64 fp32 in 2 rows 32 and 22.
+static bool emb_few(int64_t N, int64_t rows, int32_t D) { return N <= EMB_FEW_N && rows * nof_div_up(D, 32) * (N + 1024) <= (int64_t)20 << 20; }
 
 static EmbPlan emb_plan(int64_t N, int64_t rows, int32_t D) {
   EmbPlan p = {};
   const int bits = learn_log2_up(rows + 1) > 0 ? learn_log2_up(rows + 1) : 1;
-  p.small = N <= EMB_SMALL;
   p.s.N = (uint32_t)N;
   p.s.rows = rows;
+  p.few = emb_few(N, rows, D);
+  if (p.few) {
+    p.bytes = N > 0 ? 256 : 0;                                        // unused; a caller passes a workspace whatever the sizes
+    return p;
+  }
+  p.small = N <= EMB_SMALL;
   if (p.small) {
     p.s.passes = (bits + 7) / 8;
   } else {
@@ -471,6 +548,15 @@ static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* ke
   }
 }
 
+// at most eight lanes a row, so that a frequent id is many groups' work
+template <typename T>
+static void emb_launch_few(const void* dout, int64_t stride, const void* ids, int ids64, float scale, void* grad, const EmbPlan& p, int32_t D, hipStream_t st) {
+  const int64_t nv = nof_div_up(D, EmbVec<T>::V);
+  const int ls = learn_log2_up(nv < 8 ? nv : 8);
+  hipLaunchKernelGGL(k_embed_few<T>, dim3((unsigned)p.s.rows, (unsigned)nof_div_up(nv, (int64_t)1 << ls)), dim3(EMB_T), 0, st, (const T*)dout, stride, ids,
+                     ids64, (int)p.s.N, D, scale, (T*)grad, ls);
+}
+
 extern "C" int nof_embed_fwd(const void* table, int64_t table_stride, int32_t type, const void* ids, int32_t ids64, float scale, void* out,
                              int64_t N, int64_t V, int32_t D, void* stream) {
   NOF_ARG(learn_type_ok(type) && (ids64 == 0 || ids64 == 1));
@@ -499,6 +585,13 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
   NOF_ARG(N == 0 || workspace_bytes >= p.bytes);
   NOF_ARG(N == 0 || ((uintptr_t)workspace & 255) == 0);
   hipStream_t st = (hipStream_t)stream;
+  if (p.few) {
+    if (type == NOF_TYPE_F32) emb_launch_few<float>(dout, dout_stride, ids, ids64, scale, grad_table, p, D, st);
+    else if (type == NOF_TYPE_BF16) emb_launch_few<__bf16>(dout, dout_stride, ids, ids64, scale, grad_table, p, D, st);
+    else emb_launch_few<_Float16>(dout, dout_stride, ids, ids64, scale, grad_table, p, D, st);
+    NOF_LAUNCH_OK();
+    return 0;
+  }
   char* ws = (char*)workspace;
   uint32_t *key[2] = {nullptr, nullptr}, *pos[2] = {nullptr, nullptr};
   float* part = nullptr;

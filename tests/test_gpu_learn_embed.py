@@ -158,3 +158,47 @@ def test_offsets_past_32_bits(nof):
     assert torch.equal(grad[V - 1], (rows[0].float() + rows[4].float()).to(torch.bfloat16)) and torch.equal(grad[V - 2], rows[2])
     grad[ids[:4]] = 0
     assert all(int(torch.count_nonzero(part)) == 0 for part in grad.split(1 << 17))
+
+
+def big_of(V, D, N, dtype, seed):
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    return torch.randn(N, D, device='cuda', generator=gen).to(dtype), gen
+
+
+@pytest.mark.parametrize('N,V,D', [(4096, 4096, 32), (4096, 4097, 32), (4096, 64, 33), (4097, 64, 16), (257, 300, 9), (1, 19000, 33), (63, 5, 1001), (2049, 2, 24),
+                                   (1000, 40000, 16), (4000, 90000, 40)])
+@pytest.mark.parametrize('kind', ['same', 'random', 'skewed', 'absent'])
+def test_the_gradient_on_either_side_of_one_launch(nof, N, V, D, kind):
+    """few positions of few rows are added in one launch, others sorted: either side of the border, at odd sizes, rows apart, ids and dout not finite"""
+    from bundlesdf_amd import learn_ops as L
+    rng = np.random.default_rng(N * 3 + V + D)
+    for q, dtype in enumerate(TYPES):
+        ids = make_ids(kind, N, V, (torch.int32, torch.int64)[(q + N) % 2], rng).cuda()
+        dout, _ = big_of(V, D + 3, N, dtype, q)
+        for d in (dout[:, 3:], dout[:1, :D].expand(N, D)):
+            grad = L.embed_lookup_grad(d, ids, V, -0.3)
+            check_grad(grad, d, ids, V, -0.3)
+            assert torch.equal(grad, L.embed_lookup_grad(d.clone(), ids, V, -0.3))
+        inside = ids.long().clamp(-1, V)
+        dout[N // 2, :] = float('nan')
+        grad = L.embed_lookup_grad(dout[:, :D], ids, V)
+        hit = torch.zeros(V + 2, dtype=torch.bool, device='cuda')
+        hit[inside[N // 2] + 1] = True
+        assert torch.equal(grad.isnan().any(1), hit[1:V + 1])                      # in the row that it is added to, and there alone
+
+
+def test_one_launch_captured(nof):
+    from bundlesdf_amd import learn_ops as L
+    dout, gen = big_of(40, 20, 700, torch.bfloat16, 3)
+    ids = torch.randint(-1, 41, (700,), device='cuda', generator=gen)
+    L.embed_lookup_grad(dout, ids, 40)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        grad = L.embed_lookup_grad(dout, ids, 40, 2.0)
+    for _ in range(4):
+        ids.copy_(torch.randint(-1, 41, (700,), device='cuda', generator=gen))
+        dout.normal_(generator=gen)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, L.embed_lookup_grad(dout, ids, 40, 2.0))
+        check_grad(grad, dout, ids, 40, 2.0)
