@@ -138,3 +138,36 @@ def test_stream_and_graph(nof):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], L.orthogonalize(a)) and torch.equal(out[1], L.orthogonalize(b))
+
+
+@pytest.mark.parametrize('m,n', [(9, 20), (20, 9), (31, 128), (9, 300), (32, 2100), (300, 17), (40, 64), (33, 100), (128, 50), (64, 300), (700, 41), (100, 100), (90, 300),
+                                 (140, 300), (140, 2300), (1100, 333)])
+@pytest.mark.parametrize('dtype', TYPES)
+def test_every_way_of_computing_it(nof, m, n, dtype):
+    """one, two and five steps, in place, a zero matrix and one that is not finite between others, and captured: replays with the program's own calls between"""
+    from bundlesdf_amd import learn_ops as L
+    u = make('noise', (4, m, n), dtype, m + n)
+    for steps in (1, 2):
+        check(L.orthogonalize(u, steps=steps), u, steps=steps)
+    want = L.orthogonalize(u)
+    check(want, u)
+    v = u.clone()
+    assert L.orthogonalize(v, out=v) is v and torch.equal(v, want)
+    v = u.clone()
+    v[1] = 0.0
+    v[2, m // 2, n // 2] = float('nan')
+    got = L.orthogonalize(v)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[3], want[3]) and (got[1] == 0).all() and got[2].isnan().all()
+    v[2, m // 2, n // 2] = float('-inf')
+    got = L.orthogonalize(v)
+    assert torch.equal(got[3], want[3]) and got[2].isnan().all()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = L.orthogonalize(v)
+    for seed in range(3):
+        v.copy_(make('decay', (4, m, n), dtype, seed))
+        g.replay()
+        eager = L.orthogonalize(v)
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+    check(out, v)
