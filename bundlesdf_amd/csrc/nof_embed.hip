@@ -8,13 +8,18 @@
 //   1. a stable radix sort of (id, position): one k_embed_hist + k_embed_scatter per digit, or k_embed_sort_small as one workgroup;
 //   2. k_embed_reduce: a group of lanes owns a run of C sorted positions and one slice of the columns, reads the rows of dout behind
 //      them and writes the sum of every id that lies within the run; an id cut by the run's ends leaves a partial sum.  Further
-//      workgroups of the same launch write the zeros of the rows that no id names -- most of the bytes of a large table;
+//      workgroups of the same launch write the zeros of the rows that no id names -- most of the bytes of a large table -- where the
+//      sort's launches have not done so;
 //   3. k_embed_join: the partial sums of a cut id, in the order of their runs.
 // Few positions of few rows take one launch instead (k_embed_few).
 #include "nof_learn_dev.h"
 
 #define EMB_T 256                       // threads of the streaming kernels
 #define EMB_ZROWS 32                    // table rows per workgroup of the zero role
+#define EMB_ZBYTES 65536                // of the sort's zero role per workgroup
+#define EMB_ZHIST ((int64_t)12 << 20)     // bytes of zeros that ride in one launch of the sort
+#define EMB_ZSCATTER ((int64_t)32 << 20)
+#define EMB_ZSMALL ((int64_t)48 << 20)
 #define EMB_SMALL 4096                  // positions that the one-workgroup sort holds in LDS
 #define EMB_SORT_T 512
 #define EMB_SORT_W (EMB_SORT_T / 64)
@@ -50,7 +55,7 @@ __device__ __forceinline__ void emb_load(const T* __restrict__ p, int n, float (
   }
 }
 // a store past the caches: nothing here reads it again, and the rows that are read stay (65536 x 2048 bf16 looked up: 59 us, 91 without;
-// the gradient of a 131072-row table by them 227 us, 248 without)
+// the gradient of a 131072-row table by them: 26 us less)
 template <typename T, int V>
 __device__ __forceinline__ void emb_store(T* __restrict__ p, int n, const float (&f)[V]) {
   if (n >= V) {
@@ -106,6 +111,17 @@ __device__ __forceinline__ uint64_t emb_match(uint32_t digit, int bits, bool in)
   return m;
 }
 
+// Zeros for the gradient's first rows, written by workgroups that ride behind the sort's own: those few leave the chip idle for as long as
+// the memory takes for tens of megabytes (named rows are overwritten later).  131072 x 2048 bf16 196 us without, 190 so; 200000 x 64 fp32 by
+// 2000 positions 32 and 25, a million by 100000 x 64 bf16 159 and 146.
+struct EmbZero { char* at; uint64_t bytes; };                         // any border, whole elements
+__device__ __forceinline__ void emb_zero(const EmbZero& z, uint32_t block, uint32_t threads) {
+  const uint64_t lo = (uint64_t)block * EMB_ZBYTES, hi = lo + EMB_ZBYTES < z.bytes ? lo + EMB_ZBYTES : z.bytes, whole = lo + (hi - lo) / 16 * 16;
+  const emb_u4 none = {0, 0, 0, 0};
+  for (uint64_t i = lo + threadIdx.x * 16; i < whole; i += (uint64_t)threads * 16) __builtin_nontemporal_store(none, reinterpret_cast<EmbAt<2>::t*>(z.at + i));
+  for (uint64_t i = whole + threadIdx.x * 2; i < hi; i += (uint64_t)threads * 2) *reinterpret_cast<uint16_t*>(z.at + i) = 0;
+}
+
 struct EmbSort {
   const void* ids; int ids64; int64_t rows;
   uint32_t N, per;                      // positions; positions per workgroup (a multiple of EMB_SORT_T)
@@ -114,7 +130,8 @@ struct EmbSort {
 
 // hist[block][digit] of a pass.  (Counted with atomics by the scatter before instead, an id that many positions hold is one address:
 // 15 us for 8192 positions against 8 + 3.)
-__global__ __launch_bounds__(EMB_SORT_T) void k_embed_hist(EmbSort s, int pass, const uint32_t* __restrict__ key_in, uint32_t* __restrict__ hist) {
+__global__ __launch_bounds__(EMB_SORT_T) void k_embed_hist(EmbSort s, int pass, const uint32_t* __restrict__ key_in, uint32_t* __restrict__ hist, EmbZero z) {
+  if ((int)blockIdx.x >= s.n_blocks) return emb_zero(z, blockIdx.x - s.n_blocks, EMB_SORT_T);
   __shared__ uint32_t cnt[1 << EMB_BITS];
   const int bins = 1 << s.bits, shift = pass * s.bits;
   for (int d = threadIdx.x; d < bins; d += EMB_SORT_T) cnt[d] = 0;
@@ -132,7 +149,8 @@ __global__ __launch_bounds__(EMB_SORT_T) void k_embed_hist(EmbSort s, int pass, 
 // wave from the counts of the waves before it, a lane from its rank among the equal digits of its wave: no order is left to chance.
 __global__ __launch_bounds__(EMB_SORT_T) void k_embed_scatter(EmbSort s, int pass, const uint32_t* __restrict__ key_in,
                                                               const uint32_t* __restrict__ pos_in, uint32_t* __restrict__ key_out,
-                                                              uint32_t* __restrict__ pos_out, const uint32_t* __restrict__ hist) {
+                                                              uint32_t* __restrict__ pos_out, const uint32_t* __restrict__ hist, EmbZero z) {
+  if ((int)blockIdx.x >= s.n_blocks) return emb_zero(z, blockIdx.x - s.n_blocks, EMB_SORT_T);
   __shared__ uint32_t cnt[EMB_SORT_W][1 << EMB_BITS];
   __shared__ uint32_t wsum[EMB_SORT_W];
   const int bins = 1 << s.bits, shift = pass * s.bits, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -201,7 +219,8 @@ __global__ __launch_bounds__(EMB_SORT_T) void k_embed_scatter(EmbSort s, int pas
 
 // The whole sort as one workgroup of sixteen waves, 8 bits a digit, keys and positions in LDS (56 KiB).
 __global__ __launch_bounds__(1024) void k_embed_sort_small(const void* __restrict__ ids, int ids64, int64_t rows, int N, int passes,
-                                                           uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out) {
+                                                           uint32_t* __restrict__ key_out, uint32_t* __restrict__ pos_out, EmbZero z) {
+  if (blockIdx.x > 0) return emb_zero(z, blockIdx.x - 1, 1024);
   __shared__ uint32_t key[2][EMB_SMALL];
   __shared__ uint16_t pos[2][EMB_SMALL];
   __shared__ uint32_t cnt[16][128];                                  // two digits a word: counts stay below 2^16
@@ -284,14 +303,14 @@ __device__ __forceinline__ void emb_put(T* __restrict__ grad, int64_t row, int D
 template <typename T, bool ONCE>
 __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ dout, int64_t stride, const uint32_t* __restrict__ key,
                                                         const uint32_t* __restrict__ pos, uint32_t N, uint32_t rows, int D, float scale,
-                                                        T* __restrict__ grad, float* __restrict__ part, int ls, int C, uint32_t n_red) {
+                                                        T* __restrict__ grad, float* __restrict__ part, int ls, int C, uint32_t n_red, uint32_t zeroed) {
   constexpr int V = EmbVec<T>::V;
   const int DP = (D + 7) & ~7;
   const int lane = threadIdx.x & ((1 << ls) - 1);
   const int col = (((int)blockIdx.y << ls) + lane) * V;
   if (blockIdx.x >= n_red) {                                          // the zero role
     __shared__ uint8_t named[EMB_ZROWS];
-    const uint32_t v0 = (blockIdx.x - n_red) * EMB_ZROWS;
+    const uint32_t v0 = zeroed + (blockIdx.x - n_red) * EMB_ZROWS;
     if (threadIdx.x < EMB_ZROWS) {
       const uint32_t v = v0 + threadIdx.x;
       const uint32_t at = v < rows ? emb_lower(key, N, v) : 0;
@@ -317,14 +336,24 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
 #pragma unroll
   for (int k = 0; k < V; ++k) acc[k] = 0.0f;
   constexpr int U = 8;                                                // rows in flight per group
+  uint32_t next_key[U], next_pos[U];                                  // (keys and positions a turn ahead: rows wait for one load, not for three)
+  auto ahead = [&](uint32_t i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      next_key[u] = i + u < hi ? key[i + u] : rows;
+      next_pos[u] = i + u < hi ? pos[i + u] : 0;
+    }
+  };
+  ahead(lo);
   for (uint32_t i = lo; i < hi; i += U) {
     uint32_t kk[U];
     float x[U][V];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      kk[u] = i + u < hi ? key[i + u] : rows;
-      if (kk[u] < rows) emb_load<T, V, ONCE>(dout + (int64_t)pos[i + u] * stride + col, D - col, x[u]);
+      kk[u] = next_key[u];
+      if (kk[u] < rows) emb_load<T, V, ONCE>(dout + (int64_t)next_pos[u] * stride + col, D - col, x[u]);
     }
+    ahead(i + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (kk[u] != cur) {                                             // an id ends here (or the run does: `rows`)
@@ -352,7 +381,7 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
 
 // The run in which a cut id starts adds what the runs behind it inherited: a workgroup per run and slice of at most 64 x V columns, whose
 // groups of lanes each add a stretch of the runs; their sums meet in LDS, neighbours first.  (One group for all of an id that many runs hold
-// is a chain of loads: 17 us of the large table's 227, 8 so.)
+// is a chain of loads: 17 us for the large table, 8 so.)
 template <typename T>
 __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict__ key, uint32_t N, uint32_t rows, int D, float scale,
                                                       T* __restrict__ grad, const float* __restrict__ part, int ls, int C) {
@@ -467,20 +496,24 @@ __global__ __launch_bounds__(EMB_T) void k_embed_few(const T* __restrict__ dout,
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
-// sorted positions per run: long where there is work for every compute unit anyway, short where a run is the critical path
-static int emb_chunk(int64_t N, int32_t D) {
-  const int64_t e = N * D;
-  return e >= (int64_t)1 << 26 ? 64 : e >= (int64_t)1 << 24 ? 32 : e >= (int64_t)1 << 22 ? 16 : 8;
+// Sorted positions per run: as many as leave 2048 waves (two per SIMD).  A shorter run is more partial sums, a longer one a longer chain of
+// loads.  Gradient alone, 8 / 16 / 32 / 64 positions: 8192 x 1024 bf16 40.7 / 41.5 / 46.6 / 57.8 us, 65536 x 256 fp32 57 / 43 / 37.7 / 39.1,
+// 65536 x 2048 bf16 234 / 214 / 197 / 190.
+static int emb_chunk(int64_t N, int32_t D, int size) {
+  const int64_t nv = nof_div_up(D, 16 / size), waves = (N << learn_log2_up(nv < EMB_T ? nv : EMB_T)) * nof_div_up(nv, EMB_T) / 64;
+  int c = 8;
+  while (c < 64 && waves / (2 * c) >= 2048) c *= 2;
+  return c;
 }
 
-struct EmbPlan { EmbSort s; bool few, small; int64_t key[2], pos[2], hist, part, bytes; int C; uint32_t chunks; };
+struct EmbPlan { EmbSort s; bool few, small; int64_t key[2], pos[2], hist, part, bytes, zeroed; int C; uint32_t chunks; };       // zeroed: rows that the sort's launches clear
 
 // k_embed_few: every row's workgroups look all ids over, so few positions and rows x slices.  Against the sort: 4096 positions, 64 rows of 16
 // fp32 9 us and 18 (15 and 21 if all name one row), 4096 rows of 32 16 and 24, 8000 of 16 25 and 24; 256 positions, 16000 rows 13 and 16;
 // 8192 positions of 64 fp32 in 2 rows 32 and 22.
 static bool emb_few(int64_t N, int64_t rows, int32_t D) { return N <= EMB_FEW_N && rows * nof_div_up(D, 32) * (N + 1024) <= (int64_t)20 << 20; }
 
-static EmbPlan emb_plan(int64_t N, int64_t rows, int32_t D) {
+static EmbPlan emb_plan(int64_t N, int64_t rows, int32_t D, int size) {
   EmbPlan p = {};
   const int bits = learn_log2_up(rows + 1) > 0 ? learn_log2_up(rows + 1) : 1;
   p.s.N = (uint32_t)N;
@@ -501,7 +534,7 @@ static EmbPlan emb_plan(int64_t N, int64_t rows, int32_t D) {
     p.s.per = (uint32_t)(nof_div_up(per, EMB_SORT_T) * EMB_SORT_T);
     p.s.n_blocks = (int)nof_div_up(N, p.s.per);
   }
-  p.C = emb_chunk(N, D);
+  p.C = emb_chunk(N, D, size);
   p.chunks = (uint32_t)nof_div_up(N, p.C);
   int64_t at = 0;
   for (int k = 0; k < 2; ++k) {
@@ -534,12 +567,12 @@ static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* ke
   const int64_t nv = nof_div_up(D, EmbVec<T>::V);
   const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
   const unsigned cols = (unsigned)nof_div_up(nv, (int64_t)1 << ls), n_red = (unsigned)nof_div_up(p.chunks, EMB_T >> ls);
-  const unsigned n_zero = (unsigned)nof_div_up(p.s.rows, EMB_ZROWS);
+  const unsigned n_zero = (unsigned)nof_div_up(p.s.rows - p.zeroed, EMB_ZROWS);
   // dout past the caches from half of the last one (256 MB) on.  65536 x 2048 bf16: the table's rows stay, a lookup behind it takes 60 us
   // instead of 84; 8192 x 1024: the launch takes 30 us so, 20 through the caches, where dout still lies.
   auto reduce = (int64_t)p.s.N * D * (int64_t)sizeof(T) >= (int64_t)128 << 20 ? k_embed_reduce<T, true> : k_embed_reduce<T, false>;
   hipLaunchKernelGGL(reduce, dim3(n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N, (uint32_t)p.s.rows, D, scale,
-                     (T*)grad, part, ls, p.C, n_red);
+                     (T*)grad, part, ls, p.C, n_red, (uint32_t)p.zeroed);
   if (p.chunks > 1) {
     const int64_t jv = nof_div_up(D, 4);
     const int jl = learn_log2_up(jv < 64 ? jv : 64);
@@ -572,7 +605,9 @@ extern "C" int nof_embed_fwd(const void* table, int64_t table_stride, int32_t ty
 }
 
 extern "C" int64_t nof_embed_bwd_workspace_bytes(int64_t N, int64_t V, int32_t D) {
-  return emb_sizes_ok(N, V, D) ? emb_plan(N, V, D).bytes : -1;
+  if (!emb_sizes_ok(N, V, D)) return -1;
+  const int64_t a = emb_plan(N, V, D, 2).bytes, b = emb_plan(N, V, D, 4).bytes;        // (of any type)
+  return a > b ? a : b;
 }
 
 extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type, const void* ids, int32_t ids64, float scale,
@@ -581,7 +616,7 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
   NOF_ARG(emb_sizes_ok(N, V, D) && dout_stride >= 0);
   if (V == 0 || D == 0) return 0;
   NOF_ARG(grad_table && (N == 0 || (dout && ids && workspace)));
-  EmbPlan p = emb_plan(N, V, D);
+  EmbPlan p = emb_plan(N, V, D, (int)learn_type_size(type));
   NOF_ARG(N == 0 || workspace_bytes >= p.bytes);
   NOF_ARG(N == 0 || ((uintptr_t)workspace & 255) == 0);
   hipStream_t st = (hipStream_t)stream;
@@ -602,13 +637,27 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
     uint32_t* hist = (uint32_t*)(ws + p.hist);
     p.s.ids = ids;
     p.s.ids64 = ids64;
+    // what the launches of the sort have time for
+    const int64_t row = D * learn_type_size(type), room = p.small ? EMB_ZSMALL : p.s.passes * (EMB_ZHIST + EMB_ZSCATTER);
+    p.zeroed = room / row < V ? room / row : V;
+    EmbZero z = {(char*)grad_table, 0};
+    int64_t left = p.zeroed * row;
+    auto share = [&](int64_t most) {                                  // the next stretch; its workgroups
+      z.at += z.bytes;
+      z.bytes = (uint64_t)(left < most ? left : most);
+      left -= (int64_t)z.bytes;
+      return (unsigned)nof_div_up((int64_t)z.bytes, EMB_ZBYTES);
+    };
     if (p.small) {
-      hipLaunchKernelGGL(k_embed_sort_small, dim3(1), dim3(1024), 0, st, ids, (int)ids64, V, (int)N, p.s.passes, key[0], pos[0]);
+      const unsigned more = share(left);
+      hipLaunchKernelGGL(k_embed_sort_small, dim3(1 + more), dim3(1024), 0, st, ids, (int)ids64, V, (int)N, p.s.passes, key[0], pos[0], z);
     } else {
       for (int pass = 0; pass < p.s.passes; ++pass, cur ^= 1) {
-        hipLaunchKernelGGL(k_embed_hist, dim3(p.s.n_blocks), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur], hist);
-        hipLaunchKernelGGL(k_embed_scatter, dim3(p.s.n_blocks), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur],
-                           (const uint32_t*)pos[cur], key[cur ^ 1], pos[cur ^ 1], (const uint32_t*)hist);
+        unsigned more = share(EMB_ZHIST);
+        hipLaunchKernelGGL(k_embed_hist, dim3(p.s.n_blocks + more), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur], hist, z);
+        more = share(EMB_ZSCATTER);
+        hipLaunchKernelGGL(k_embed_scatter, dim3(p.s.n_blocks + more), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur],
+                           (const uint32_t*)pos[cur], key[cur ^ 1], pos[cur ^ 1], (const uint32_t*)hist, z);
       }
     }
     NOF_LAUNCH_OK();

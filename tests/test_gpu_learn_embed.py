@@ -202,3 +202,21 @@ def test_one_launch_captured(nof):
         torch.cuda.synchronize()
         assert torch.equal(grad, L.embed_lookup_grad(dout, ids, 40, 2.0))
         check_grad(grad, dout, ids, 40, 2.0)
+
+
+@pytest.mark.parametrize('N,V,D', [(5000, 60000, 1000), (300, 30000, 1001), (4999, 131000, 7)])
+def test_rows_that_nobody_names_are_zeros_wherever_they_lie(nof, N, V, D):
+    """a table larger than the stretch that the sort's launches clear, over memory that held something else"""
+    from bundlesdf_amd import learn_ops as L
+    for q, dtype in enumerate(TYPES):
+        dout, gen = big_of(V, D, N, dtype, 7 + q)
+        ids = torch.randint(-1, V, (N,), device='cuda', generator=gen)
+        ids[:N // 3] = V - 1
+        stale = torch.full((V, D), float('nan'), dtype=dtype, device='cuda')
+        del stale
+        grad = L.embed_lookup_grad(dout, ids, V, 0.5)
+        named = torch.zeros(V, dtype=torch.bool, device='cuda')
+        named[ids[ids >= 0]] = True
+        assert not grad[~named].any() and not grad.isnan().any()
+        rows = torch.unique(ids[ids >= 0])
+        check_grad(grad[rows], dout[ids >= 0], torch.searchsorted(rows, ids[ids >= 0]), len(rows), 0.5)
