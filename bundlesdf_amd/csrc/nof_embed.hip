@@ -391,13 +391,14 @@ __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict
   const uint32_t chunk = blockIdx.x;
   const uint64_t first = (uint64_t)chunk * C, end = first + C;
   if (end >= N) return;
-  const uint32_t lo = (uint32_t)first, id = key[end - 1];
-  if (id >= rows || key[end] != id) return;                           // nothing handed on
-  if (key[lo] == id && lo > 0 && key[lo - 1] == id) return;           // nor started here
-  uint32_t last = chunk + 1, step = 1;                                // the last run that starts with the id: doubling steps, then halving
-  while (((uint64_t)last + step) * C < N && key[((uint64_t)last + step) * C] == id) { last += step; step *= 2; }
-  for (step /= 2; step > 0; step /= 2)
-    if (((uint64_t)last + step) * C < N && key[((uint64_t)last + step) * C] == id) last += step;
+  const uint32_t lo = (uint32_t)first, id = key[end - 1], after = key[end], start = key[lo], before = key[lo > 0 ? lo - 1 : 0];
+  if (id >= rows || after != id) return;                              // nothing handed on
+  if (start == id && lo > 0 && before == id) return;                  // nor started here
+  uint32_t last = chunk;                                              // the last run that starts with the id, as many runs at a time as threads
+  for (int more = EMB_T; more == EMB_T; last += more) {
+    const uint64_t at = ((uint64_t)last + 1 + threadIdx.x) * C;
+    more = __syncthreads_count(at < N && key[at] == id);
+  }
   const int lane = threadIdx.x & ((1 << ls) - 1), group = threadIdx.x >> ls, groups = EMB_T >> ls;
   const int col = (((int)blockIdx.y << ls) + lane) * V;
   const uint32_t each = (last - chunk + groups - 1) / groups, c0 = chunk + 1 + group * each, c1 = c0 + each <= last ? c0 + each : last + 1;
