@@ -923,11 +923,14 @@ static void ort_gemm(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
 template <int MODE, typename T, bool PAIRS>
 static void ort_product(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
   const int64_t wide = p.rp % 128 == 0 && p.kp % 128 == 0 ? batch * ort_tiles<MODE, OrtWide>(p) : 0;
-  if (MODE == ORT_GRAM && p.split > 1) {
-    if (batch * ort_tiles<MODE, OrtNarrow>(p) * p.split > 256) ort_gemm<MODE, T, OrtNarrow, PAIRS>(p, out, batch, st);
-    else ort_gemm<MODE, T, OrtNarrowDeep, PAIRS>(p, out, batch, st);
-    ort_gemm<ORT_JOIN, T, OrtSingle, PAIRS>(p, out, batch, st);
-  } else if (wide > 256) ort_gemm<MODE, T, OrtWide, PAIRS>(p, out, batch, st);
+  if constexpr (MODE == ORT_GRAM) {
+    if (p.split > 1) {
+      if (batch * ort_tiles<MODE, OrtNarrow>(p) * p.split > 256) ort_gemm<MODE, T, OrtNarrow, PAIRS>(p, out, batch, st);
+      else ort_gemm<MODE, T, OrtNarrowDeep, PAIRS>(p, out, batch, st);
+      return ort_gemm<ORT_JOIN, T, OrtSingle, PAIRS>(p, out, batch, st);
+    }
+  }
+  if (wide > 256) ort_gemm<MODE, T, OrtWide, PAIRS>(p, out, batch, st);
   else if (ort_wide(wide)) ort_gemm<MODE, T, OrtWideDeep, PAIRS>(p, out, batch, st);
   else if (batch * ort_tiles<MODE, OrtNarrow>(p) > 256) ort_gemm<MODE, T, OrtNarrow, PAIRS>(p, out, batch, st);
   else ort_gemm<MODE, T, OrtNarrowDeep, PAIRS>(p, out, batch, st);
