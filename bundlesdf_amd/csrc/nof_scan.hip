@@ -510,10 +510,14 @@ __global__ __launch_bounds__(256) void k_scan_step(const TG* __restrict__ gate, 
 // Segments: from one wave per SIMD (1024 waves) on, a workgroup's own look-ahead keeps the memory busy and a second pass over the inputs
 // would cost more than it gives; below, two waves per SIMD, of two chunks at least.  4 x 16384 x 1024 bf16, forward + backward: 111 + 177 us
 // so, 123 + 192 with four waves per SIMD, 154 + 209 with one.
+// Tiles narrower than a wave where that leaves a fifth fewer lanes without a channel: 65 channels a group (24 x 1777 x 520, eight gates)
+// backward 84 us, 115 as 64 + 1.
 static void scan_layout(ScanArgs& p, int span, int v) {
   p.span = span;
   const int nv = span / v;
   p.cs = learn_log2_up(nv < 64 ? nv : 64);
+  for (int cs = 5; nv > 64 && cs >= 4; --cs)                          // (one tile a span stays one: another means sums to join)
+    if (5 * (nof_div_up(nv, (int64_t)1 << cs) << cs) <= 4 * (nof_div_up(nv, (int64_t)1 << p.cs) << p.cs)) p.cs = cs;
   p.tiles_per_span = (int)nof_div_up(nv, (int64_t)1 << p.cs);
   p.tiles = p.D / span * p.tiles_per_span;
   const int64_t slots = nof_div_up(p.T, SCAN_U), per_wave = 64 >> p.cs, need = nof_div_up(slots, per_wave);
