@@ -121,9 +121,10 @@ __device__ __forceinline__ void ort_mma6(const _Float16* L, const _Float16* R, i
 }
 
 // ---- one workgroup a matrix -------------------------------------------------------------------------------------------------------
-// One wave per 32 x 32 tile of X (r <= k after the turn; tiles rt x KT).  LDS: two pairs of images, rows of 32 KT + 8 halves (the pad
-// spreads a column's 16-byte reads over all banks; known at compile time, or sixteen row offsets per store stay live and spill).  The first holds X for the Gram product and X^T for the last one, the second A, then P: symmetric, so their tiles are stored
-// turned, four halves at a time.  Bound by the chain of products, barriers and LDS round trips: 1.7 us a step for 16 x 16, 3.2 for 64 x 64,
+// One wave per 32 x 32 tile of X (r <= k after the turn; tiles rt x KT).  LDS: images of hi and lo, rows of 32 KT + 8 halves (the pad
+// spreads a column's 16-byte reads over all banks; known at compile time, or sixteen row offsets per store stay live and spill).  The first
+// pair holds X for the Gram product and X^T for the last one, the second A, then P: symmetric, so their tiles are stored turned, four
+// halves at a time.  Bound by the chain of products, barriers and LDS round trips: 1.7 us a step for 16 x 16, 3.2 for 64 x 64,
 // 8 for 128 x 128 (half of it the matrix cores); four waves of 2 x 2 tiles instead of sixteen of one read half as much LDS and take 1.4
 // times as long.
 struct OrtCoef { float c[3 * ORT_MAX_STEPS]; };
@@ -186,7 +187,8 @@ __global__ __launch_bounds__(64 * KT * RT) void k_ortho_small(const T* __restric
     if (gram) {
 #pragma unroll 2
       for (int q = 0; q < 2 * KT; ++q) {
-        const f16x8 lh = *(const f16x8*)(xh + li + 16 * q), ll = *(const f16x8*)(xl + li + 16 * q), rh = *(const f16x8*)(xh + ri + 16 * q), rl = *(const f16x8*)(xl + ri + 16 * q);
+        const f16x8 lh = *(const f16x8*)(xh + li + 16 * q), ll = *(const f16x8*)(xl + li + 16 * q);
+        const f16x8 rh = *(const f16x8*)(xh + ri + 16 * q), rl = *(const f16x8*)(xl + ri + 16 * q);
         if (square != ORT_PAIRS) ort_mma3(lh, ll, rh, rl, acc, acc2);
         else acc = ort_mma3(lh, ll, rh, rl, acc);
       }
@@ -649,7 +651,8 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
     }
   };
   f32x16 acc[S::ti][S::tj] = {};
-  const int wi = (w / S::wn) * S::ti * 32, wj = (w % S::wn) * S::tj * 32, n_stages = s1 - s0, rounds = (n_stages + S::kg - 1) / S::kg, stages = (n_stages - kg + S::kg - 1) / S::kg;      // this group's stages
+  const int wi = (w / S::wn) * S::ti * 32, wj = (w % S::wn) * S::tj * 32;
+  const int n_stages = s1 - s0, rounds = (n_stages + S::kg - 1) / S::kg, stages = (n_stages - kg + S::kg - 1) / S::kg;      // this group's stages
 #pragma unroll
   for (int q = 0; q < S::ns - 1; ++q)
     if (q < stages) load(q);

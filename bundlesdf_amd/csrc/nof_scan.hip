@@ -297,7 +297,8 @@ __global__ __launch_bounds__(64 * SCAN_MAXW, 3) void k_scan_fwd(ScanArgs p) {
       scan_fold<V, false>(A, B, TA, TB, p.cs, p.waves, sh[c & 1]);
 #pragma unroll
       for (int v = 0; v < V; ++v) { s[v] = A[v] * S[v] + B[v]; S[v] = TA[v] * S[v] + TB[v]; }
-      if (p.marks && q.on && i0 < q.n && (uint32_t)i0 % (uint32_t)p.mark == 0) lstore<float, V>(p.marks + ((int64_t)q.b * p.n_marks + (uint32_t)i0 / (uint32_t)p.mark) * p.D + q.ch, s);
+      if (p.marks && q.on && i0 < q.n && (uint32_t)i0 % (uint32_t)p.mark == 0)
+        lstore<float, V>(p.marks + ((int64_t)q.b * p.n_marks + (uint32_t)i0 / (uint32_t)p.mark) * p.D + q.ch, s);
       T* o = h.at(i0);
       const int64_t ost = h.stride();
       const int64_t left = q.n - i0;
