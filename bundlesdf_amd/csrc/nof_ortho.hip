@@ -17,7 +17,6 @@
 // index, so X is stored in both orientations.
 #include "nof_learn_dev.h"
 #include "nof_mfma_dev.h"
-#include <type_traits>
 
 #define ORT_SCALE 4096.0f               // operands hold 4096 times their value: |P| <= 15, |X| <= 2 stay below 65504
 #define ORT_SMALL 128
@@ -463,7 +462,7 @@ __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g
 // ---- larger matrices --------------------------------------------------------------------------------------------------------------
 // images of one matrix, in halves: X [rp][kp], X^T [kp][rp] twice (the last product reads one while it writes the other), A and P
 // [rp][rp].  32 hi of a row lie next to their 32 lo, a cache line that one stage of a product reads whole (as planes, lines of which a
-// stage read half, L2 held the products at 10 TB/s of useful and as much useless traffic); an image that is read for hi alone is a hi plane.
+// stage read half, L2 held the products at 10 TB/s of useful and as much useless traffic).
 // rp, kp: r and k up to whole tiles, zeros in between.
 struct OrtArgs {
   _Float16* ws; size_t per;             // halves per matrix
@@ -472,7 +471,6 @@ struct OrtArgs {
   int cur;                              // which X^T holds X
   int tiles;                            // of a matrix in this launch
   int split; float* parts;              // the Gram product's long axis in `split` parts, joined by a launch of its own
-  int flat;                             // this launch's P or X^T is read for hi alone
 };
 __device__ __forceinline__ _Float16* ort_x(const OrtArgs& p, int b) { return p.ws + b * p.per; }
 __device__ __forceinline__ _Float16* ort_xt(const OrtArgs& p, int b, int which) { return p.ws + b * p.per + (size_t)(1 + which) * 2 * p.rp * p.kp; }
@@ -526,7 +524,6 @@ __global__ __launch_bounds__(256) void k_ortho_split(const T* __restrict__ g, co
   __syncthreads();
   _Float16* along = p.tall ? ort_xt(p, b, p.cur) : ort_x(p, b);        // [rows][cols]
   _Float16* turned = p.tall ? ort_x(p, b) : ort_xt(p, b, p.cur);       // [cols][rows]
-  const bool flat_a = p.flat && p.tall, flat_t = p.flat && !p.tall;   // X^T for a single step of hi alone
 #pragma unroll
   for (int q = 0; q < 4; ++q) {                                       // eight of a row of either: 16 bytes of hi, 16 of lo
     const int y = (q & 1) * 32 + threadIdx.x / 8, x = threadIdx.x % 8 * 8;
@@ -540,10 +537,9 @@ __global__ __launch_bounds__(256) void k_ortho_split(const T* __restrict__ g, co
     }
     _Float16* to = q < 2 ? along : turned;
     const int row = (q < 2 ? y0 : x0) + y, col = (q < 2 ? x0 : y0) + x, ld = q < 2 ? cols : rows;
-    const bool flat = q < 2 ? flat_a : flat_t;
-    const size_t at = flat ? (size_t)row * ld + col : ort_at(row, col, ld);
+    const size_t at = ort_at(row, col, ld);
     *(f16x8*)(to + at) = h;
-    if (!flat) *(f16x8*)(to + at + 32) = l;
+    *(f16x8*)(to + at + 32) = l;
   }
 }
 
@@ -553,15 +549,15 @@ __global__ __launch_bounds__(256) void k_ortho_split(const T* __restrict__ g, co
 #define ORT_LAST 3
 #define ORT_JOIN 4                      // the Gram product's parts, added in order
 
-// A stage is 64 halves of every row: 32 of the summed index as hi and lo, or 64 of it as hi alone.  16-byte piece c of row `row`
+// A stage is 64 halves of every row: 32 of the summed index as hi and lo.  16-byte piece c of row `row`
 // sits at piece c ^ ort_swizzle(row): a fragment's reads (one piece of 32 consecutive rows) then touch every bank equally, for eight lanes
 // of 128 bytes and for sixteen of 256
 __device__ __forceinline__ int ort_swizzle(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
 // C = L R^T.  A workgroup is WM x WN waves of TI x TJ tiles of 32 x 32; a stage is 64 halves of every row, NS stages a ring in
-// LDS that direct loads fill NS - 1 stages ahead, one barrier a stage.  PAIRS: operands are hi + lo (three products), else hi alone: what the last
-// product of a bfloat16 result takes, off by at most 2^-10 of it beside the rounding's 2^-8 (in any other product, an error of hi alone would
-// be amplified by the steps that follow: up to 1 % for a multiple of the identity).
+// LDS that direct loads fill NS - 1 stages ahead, one barrier a stage.  Operands are pairs in every product, the last one of a 16-bit result
+// too: of hi alone, bfloat16 results lay beyond the rounding's half step by 4.3e-4 of their norm (1024 x 1024 of rank 16), and so they would more
+with a larger first coefficient (P's diagonal is 4096 a, which fp16 steps by 8 and up).
 // KG groups of such waves take the stages in turn, so that few tiles still give every SIMD several waves; their sums meet in LDS.
 template <int WM, int WN, int TI, int TJ, int NS, int KG> struct OrtShape {
   static constexpr int wm = WM, wn = WN, ti = TI, tj = TJ, ns = NS, kg = KG, M = WM * TI * 32, N = WN * TJ * 32, group = WM * WN * 64, threads = group * KG;
@@ -577,7 +573,7 @@ __device__ __forceinline__ void ort_wave_sync() {
   asm volatile("" ::: "memory");
 }
 
-template <int MODE, typename T, typename S, bool PAIRS>
+template <int MODE, typename T, typename S>
 __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::stage <= 40960 ? 2 : 1)) void k_ortho_gemm(OrtArgs p, T* __restrict__ out) {
   __shared__ __attribute__((aligned(16))) _Float16 lds[S::ns * S::kg * S::stage];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, l31 = lane & 31;
@@ -626,14 +622,14 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
   if (MODE == ORT_GRAM || MODE == ORT_JOIN) { L = R = ort_x(p, b); K = p.kp; }
   else if (MODE == ORT_POLY) { L = R = ort_a(p, b); K = p.rp; }
   else { L = ort_p(p, b); R = ort_xt(p, b, p.cur); K = p.rp; }
-  constexpr int kstep = PAIRS ? 32 : 64;
+  constexpr int kstep = 32;
   int s0 = 0, s1 = MODE == ORT_JOIN ? 0 : K / kstep;                  // the stages of this part
   if (MODE == ORT_GRAM && p.split > 1) {
     const unsigned n = s1;                                            // (at most 512, in at most 64 parts)
     s0 = n * slice / p.split;
     s1 = n * (slice + 1) / p.split;
   }
-  const size_t pitch = PAIRS ? 2 * (size_t)K : (size_t)K;
+  const size_t pitch = 2 * (size_t)K;
   // where this thread's pieces of a stage come from: L's rows, then R's
   const _Float16* src[S::loads];
 #pragma unroll
@@ -676,13 +672,13 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
         for (int t = 0; t < S::ti; ++t) {
           const int row = wi + 32 * t + l31, o = row * 64, z = ort_swizzle(row);
           lh[kk][t] = *(const f16x8*)(st + o + (c ^ z) * 8);
-          if (PAIRS) ll[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
+          ll[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
         }
 #pragma unroll
         for (int t = 0; t < S::tj; ++t) {
           const int row = wj + 32 * t + l31, o = (S::M + row) * 64, z = ort_swizzle(row);
           rh[kk][t] = *(const f16x8*)(st + o + (c ^ z) * 8);
-          if (PAIRS) rl[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
+          rl[kk][t] = *(const f16x8*)(st + o + ((c + 4) ^ z) * 8);
         }
       }
 #pragma unroll
@@ -691,7 +687,7 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
         for (int i = 0; i < S::ti; ++i)
 #pragma unroll
           for (int j = 0; j < S::tj; ++j)
-            acc[i][j] = PAIRS ? ort_mma3(lh[kk][i], ll[kk][i], rh[kk][j], rl[kk][j], acc[i][j]) : PrecF16::mma(lh[kk][i], rh[kk][j], acc[i][j]);
+            acc[i][j] = ort_mma3(lh[kk][i], ll[kk][i], rh[kk][j], rl[kk][j], acc[i][j]);
     }
     }
     slot = slot + 1 == S::ns ? 0 : slot + 1;
@@ -807,7 +803,6 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
   _Float16* band = lds + w * 32 * wmax;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    if (MODE == ORT_POLY && p.flat && half) break;
     if (MODE == ORT_APPLY || bi != bj) {                              // as computed; a tile on the diagonal is its own mirror image
 #pragma unroll
       for (int i = 0; i < S::ti; ++i) {
@@ -823,7 +818,7 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
 #pragma unroll
         for (int q = 0; q < 2 * S::tj; ++q) {
           const int piece = q * 64 + lane, row = piece / (4 * S::tj), at = piece % (4 * S::tj) * 8;
-          const size_t to = MODE == ORT_POLY && p.flat ? (size_t)(i0 + 32 * i + row) * ld + j0 + at : ort_at(i0 + 32 * i + row, j0 + at, ld) + 32 * half;
+          const size_t to = ort_at(i0 + 32 * i + row, j0 + at, ld) + 32 * half;
           *(f16x8*)(c + to) = *(const f16x8*)(band + row * wmax + at);
         }
         ort_wave_sync();
@@ -831,7 +826,6 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
     }
 #pragma unroll
     for (int j = 0; j < S::tj; ++j) {                                 // and turned
-      if (p.flat && half) break;
 #pragma unroll
       for (int i = 0; i < S::ti; ++i)
 #pragma unroll
@@ -849,7 +843,7 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
 #pragma unroll
       for (int q = 0; q < 2 * S::ti; ++q) {
         const int piece = q * 64 + lane, row = piece / (4 * S::ti), at = piece % (4 * S::ti) * 8;
-        const size_t to = p.flat ? (size_t)(j0 + 32 * j + row) * p.rp + i0 + at : ort_at(j0 + 32 * j + row, i0 + at, p.rp) + 32 * half;
+        const size_t to = ort_at(j0 + 32 * j + row, i0 + at, p.rp) + 32 * half;
         *(f16x8*)(ct + to) = *(const f16x8*)(band + row * wmax + at);
       }
       ort_wave_sync();
@@ -917,26 +911,26 @@ template <int MODE, typename S> static int64_t ort_tiles(const OrtArgs& p) {
   const int64_t ni = p.rp / S::M, nj = p.kp / S::N;
   return MODE == ORT_GRAM || MODE == ORT_POLY || MODE == ORT_JOIN ? ni * (ni + 1) / 2 : ni * nj;
 }
-template <int MODE, typename T, typename S, bool PAIRS>
+template <int MODE, typename T, typename S>
 static void ort_gemm(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
   p.tiles = (int)ort_tiles<MODE, S>(p);
   const int64_t parts = MODE == ORT_GRAM ? p.split : 1;
-  hipLaunchKernelGGL((k_ortho_gemm<MODE, T, S, PAIRS>), dim3((unsigned)(p.tiles * batch * parts)), dim3(S::threads), 0, st, p, out);
+  hipLaunchKernelGGL((k_ortho_gemm<MODE, T, S>), dim3((unsigned)(p.tiles * batch * parts)), dim3(S::threads), 0, st, p, out);
 }
-template <int MODE, typename T, bool PAIRS>
+template <int MODE, typename T>
 static void ort_product(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
   const int64_t wide = p.rp % 128 == 0 && p.kp % 128 == 0 ? batch * ort_tiles<MODE, OrtWide>(p) : 0;
   if constexpr (MODE == ORT_GRAM) {
     if (p.split > 1) {
-      if (batch * ort_tiles<MODE, OrtNarrow>(p) * p.split > 256) ort_gemm<MODE, T, OrtNarrow, PAIRS>(p, out, batch, st);
-      else ort_gemm<MODE, T, OrtNarrowDeep, PAIRS>(p, out, batch, st);
-      return ort_gemm<ORT_JOIN, T, OrtSingle, PAIRS>(p, out, batch, st);
+      if (batch * ort_tiles<MODE, OrtNarrow>(p) * p.split > 256) ort_gemm<MODE, T, OrtNarrow>(p, out, batch, st);
+      else ort_gemm<MODE, T, OrtNarrowDeep>(p, out, batch, st);
+      return ort_gemm<ORT_JOIN, T, OrtSingle>(p, out, batch, st);
     }
   }
-  if (wide > 256) ort_gemm<MODE, T, OrtWide, PAIRS>(p, out, batch, st);
-  else if (ort_wide(wide)) ort_gemm<MODE, T, OrtWideDeep, PAIRS>(p, out, batch, st);
-  else if (batch * ort_tiles<MODE, OrtNarrow>(p) > 256) ort_gemm<MODE, T, OrtNarrow, PAIRS>(p, out, batch, st);
-  else ort_gemm<MODE, T, OrtNarrowDeep, PAIRS>(p, out, batch, st);
+  if (wide > 256) ort_gemm<MODE, T, OrtWide>(p, out, batch, st);
+  else if (ort_wide(wide)) ort_gemm<MODE, T, OrtWideDeep>(p, out, batch, st);
+  else if (batch * ort_tiles<MODE, OrtNarrow>(p) > 256) ort_gemm<MODE, T, OrtNarrow>(p, out, batch, st);
+  else ort_gemm<MODE, T, OrtNarrowDeep>(p, out, batch, st);
 }
 
 // the sums of squares, as many as it says
@@ -1006,8 +1000,6 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
   p.r = (int)r; p.k = (int)k; p.rp = (int)ort_up(r, unit); p.kp = (int)ort_up(k, unit);
   p.m = (int)m; p.n = (int)n; p.tall = m > n;
   p.per = (size_t)6 * p.rp * p.kp + (size_t)4 * p.rp * p.rp;
-  constexpr bool light = std::is_same<T, __bf16>::value;             // the last product of hi alone (k_ortho_gemm)
-  p.flat = light && steps == 1;
   double* part = (double*)workspace;
   p.ws = (_Float16*)((char*)workspace + learn_align(batch * ORT_NORM_BLOCKS * 8));
   p.split = ort_cuts(batch, p.rp, p.kp);
@@ -1018,13 +1010,10 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
                      (const double*)part, n_part, p, eps);
   for (int s = 0; s < steps; ++s, p.cur ^= 1) {
     p.ca = coef[3 * s]; p.cb = coef[3 * s + 1]; p.cc = coef[3 * s + 2];
-    p.flat = 0;
-    ort_product<ORT_GRAM, float, true>(p, nullptr, batch, st);
-    p.flat = light && s + 1 == steps;
-    ort_product<ORT_POLY, float, true>(p, nullptr, batch, st);
-    p.flat = light && s + 2 == steps;
-    if (s + 1 < steps) ort_product<ORT_APPLY, float, true>(p, nullptr, batch, st);
-    else ort_product<ORT_LAST, T, !light>(p, (T*)out, batch, st);
+    ort_product<ORT_GRAM, float>(p, nullptr, batch, st);
+    ort_product<ORT_POLY, float>(p, nullptr, batch, st);
+    if (s + 1 < steps) ort_product<ORT_APPLY, float>(p, nullptr, batch, st);
+    else ort_product<ORT_LAST, T>(p, (T*)out, batch, st);
   }
 }
 
