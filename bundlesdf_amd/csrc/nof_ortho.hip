@@ -557,7 +557,7 @@ __device__ __forceinline__ int ort_swizzle(int row) { return (row & 7) ^ ((row >
 // C = L R^T.  A workgroup is WM x WN waves of TI x TJ tiles of 32 x 32; a stage is 64 halves of every row, NS stages a ring in
 // LDS that direct loads fill NS - 1 stages ahead, one barrier a stage.  Operands are pairs in every product, the last one of a 16-bit result
 // too: of hi alone, bfloat16 results lay beyond the rounding's half step by 4.3e-4 of their norm (1024 x 1024 of rank 16), and so they would more
-with a larger first coefficient (P's diagonal is 4096 a, which fp16 steps by 8 and up).
+// with a larger first coefficient (P's diagonal is 4096 a, which fp16 steps by 8 and up).
 // KG groups of such waves take the stages in turn, so that few tiles still give every SIMD several waves; their sums meet in LDS.
 template <int WM, int WN, int TI, int TJ, int NS, int KG> struct OrtShape {
   static constexpr int wm = WM, wn = WN, ti = TI, tj = TJ, ns = NS, kg = KG, M = WM * TI * 32, N = WN * TJ * 32, group = WM * WN * 64, threads = group * KG;
