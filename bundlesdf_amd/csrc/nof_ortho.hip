@@ -5,10 +5,11 @@
 // so a singular value s of X goes to a s + b s^3 + c s^5 and the singular vectors stay.
 //
 // Bound by the matrix cores.  A and A A are symmetric: only the tiles on and above the diagonal are computed, each is stored twice.
-// Operands are fp16 pairs hi + lo of 4096 times the value (rounding of lo: 2^-23 of the value, subnormals out of reach for what carries
-// weight), products hi hi + hi lo + lo hi accumulate in binary32: as exact as a binary32 product at a third of the fp16 rate, which on
-// this card is some three times the binary32 rate.  One fp16 product instead would be off by 2^-12 per step, which small singular values
-// amplify by up to a^steps: 4 % for a matrix of rank 4 plus noise of 1e-4.  The norm is summed in 64 bits: an error of it is common to all
+// Operands are fp16 pairs hi + lo / 2048 of 4096 times the value: off by 2^-23 of the value, or by 2^-48 where that is more (hi is subnormal
+// below 2^-26 and lo takes what it leaves; with lo as it is, it would be subnormal below 2^-15 already: rows of 1e-5 of the largest were off by
+// 1e-4 so, and steps that lift them made them most of the result).  Products hi hi + (hi lo + lo hi) / 2048 accumulate in binary32, large and
+// small apart: as exact as a binary32 product at a third of the fp16 rate, which on this card is some three times the binary32 rate.  One fp16
+// product instead would be off by 2^-12 per step, which small singular values amplify by up to a^steps: 4 % for a matrix of rank 4 plus noise of 1e-4.  The norm is summed in 64 bits: an error of it is common to all
 // values and the polynomial amplifies it.  Of at most 64 rows, A A is formed more exactly (ort_square).
 //
 // Matrices of at most 128 x 128 take one workgroup and one launch (k_ortho_small): X lives in accumulator registers, operands in LDS.
@@ -19,6 +20,7 @@
 #include "nof_mfma_dev.h"
 
 #define ORT_SCALE 4096.0f               // operands hold 4096 times their value: |P| <= 15, |X| <= 2 stay below 65504
+#define ORT_LESS 2048.0f                // and their small parts 2048 times theirs
 #define ORT_SMALL 128
 #define ORT_NORM_BLOCKS 512             // at most
 #define ORT_MAX_STEPS 32
@@ -27,13 +29,14 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ void ort_split(float x, _Float16& hi, _Float16& lo) {
   hi = (_Float16)x;
-  lo = (_Float16)(x - (float)hi);
+  lo = (_Float16)((x - (float)hi) * ORT_LESS);
 }
 
-__device__ __forceinline__ f32x16 ort_mma3(f16x8 lh, f16x8 ll, f16x8 rh, f16x8 rl, f32x16 c) {
-  c = PrecF16::mma(lh, rl, c);
-  c = PrecF16::mma(ll, rh, c);
-  return PrecF16::mma(lh, rh, c);
+// a product is large + small / 2048
+__device__ __forceinline__ void ort_mma3(f16x8 lh, f16x8 ll, f16x8 rh, f16x8 rl, f32x16& large, f32x16& small) {
+  small = PrecF16::mma(lh, rl, small);
+  small = PrecF16::mma(ll, rh, small);
+  large = PrecF16::mma(lh, rh, large);
 }
 
 // sum over the workgroup's threads in a fixed order, given to all
@@ -64,9 +67,9 @@ __host__ __device__ constexpr int ort_square(int rt) { return rt == 1 ? ORT_WIDE
 __host__ __device__ constexpr int ort_parts(int rt) { return ort_square(rt) == ORT_THREE ? 3 : 2; }        // planes of A's image
 __device__ __forceinline__ void ort_split(float x, float less, _Float16& hi, _Float16& mid, _Float16& lo) {       // of x + less
   hi = (_Float16)x;
-  const float rest = (x - (float)hi) + less;
+  const float rest = ((x - (float)hi) + less) * ORT_LESS;
   mid = (_Float16)rest;
-  lo = (_Float16)(rest - (float)mid);
+  lo = (_Float16)((rest - (float)mid) * ORT_LESS);
 }
 
 // P = ca I + cb A + cc A A of at most 32 rows, 16 x 16 blocks on and above the diagonal shared by `waves`; A in rows of ORT_WIDE_ROW (whose
@@ -100,23 +103,21 @@ __device__ __forceinline__ void ort_clear(_Float16* image, int halves, int tid, 
   const f16x8 z = {};
   for (int q = tid * 8; q < halves; q += threads * 8) *(f16x8*)(image + q) = z;
 }
-__device__ __forceinline__ void ort_mma3(f16x8 lh, f16x8 ll, f16x8 rh, f16x8 rl, f32x16& large, f32x16& small) {
-  small = PrecF16::mma(lh, rl, small);
-  small = PrecF16::mma(ll, rh, small);
-  large = PrecF16::mma(lh, rh, large);
-}
 
 // 32 x 32 tile of L R^T over 16 n columns, three parts each, planes apart
 __device__ __forceinline__ void ort_mma6(const _Float16* L, const _Float16* R, int plane, int n, f32x16& large, f32x16& small) {
+  f32x16 least = {};
 #pragma unroll 2
   for (int q = 0; q < n; ++q) {
     const f16x8 lh = *(const f16x8*)(L + 16 * q), lm = *(const f16x8*)(L + plane + 16 * q), ll = *(const f16x8*)(L + 2 * plane + 16 * q);
     const f16x8 rh = *(const f16x8*)(R + 16 * q), rm = *(const f16x8*)(R + plane + 16 * q), rl = *(const f16x8*)(R + 2 * plane + 16 * q);
-    small = PrecF16::mma(lh, rl, small);
-    small = PrecF16::mma(ll, rh, small);
-    small = PrecF16::mma(lm, rm, small);
+    least = PrecF16::mma(lh, rl, least);
+    least = PrecF16::mma(ll, rh, least);
+    least = PrecF16::mma(lm, rm, least);
     ort_mma3(lh, lm, rh, rm, large, small);
   }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) small[e] += least[e] * (1.0f / ORT_LESS);
 }
 
 // ---- one workgroup a matrix -------------------------------------------------------------------------------------------------------
@@ -188,11 +189,10 @@ __global__ __launch_bounds__(64 * KT * RT) void k_ortho_small(const T* __restric
       for (int q = 0; q < 2 * KT; ++q) {
         const f16x8 lh = *(const f16x8*)(xh + li + 16 * q), ll = *(const f16x8*)(xl + li + 16 * q);
         const f16x8 rh = *(const f16x8*)(xh + ri + 16 * q), rl = *(const f16x8*)(xl + ri + 16 * q);
-        if (square != ORT_PAIRS) ort_mma3(lh, ll, rh, rl, acc, acc2);
-        else acc = ort_mma3(lh, ll, rh, rl, acc);
+        ort_mma3(lh, ll, rh, rl, acc, acc2);
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) { acc[e] *= 1.0f / ORT_SCALE; acc2[e] *= 1.0f / ORT_SCALE; }     // 4096 A
+      for (int e = 0; e < 16; ++e) { acc[e] *= 1.0f / ORT_SCALE; acc2[e] *= 1.0f / (ORT_SCALE * ORT_LESS); }         // 4096 A
       if (square == ORT_WIDE) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) a64[l31 * ORT_WIDE_ROW + nloc(hi, e)] = ((double)acc[e] + (double)acc2[e]) * (1.0 / ORT_SCALE);
@@ -207,6 +207,8 @@ __global__ __launch_bounds__(64 * KT * RT) void k_ortho_small(const T* __restric
           *(f16x4*)(al + 32 * RT * px + own + 8 * q) = l4;
         }
       } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[e] += acc2[e];
         put(ah, al, acc);
       }
     }
@@ -219,28 +221,28 @@ __global__ __launch_bounds__(64 * KT * RT) void k_ortho_small(const T* __restric
       else if (gram) {
 #pragma unroll 2
         for (int q = 0; q < 2 * rt; ++q)
-          sq = ort_mma3(*(const f16x8*)(ah + li + 16 * q), *(const f16x8*)(al + li + 16 * q), *(const f16x8*)(ah + ri + 16 * q), *(const f16x8*)(al + ri + 16 * q), sq);
+          ort_mma3(*(const f16x8*)(ah + li + 16 * q), *(const f16x8*)(al + li + 16 * q), *(const f16x8*)(ah + ri + 16 * q), *(const f16x8*)(al + ri + 16 * q), sq, sq2);
       }
       __syncthreads();                                                // A has been read
       if (gram) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float one = 32 * ti + nloc(hi, e) == j ? ca * ORT_SCALE : 0.0f;
-          if (square == ORT_THREE) acc[e] = (one + cb * acc[e] + cc * (sq[e] * (1.0f / ORT_SCALE))) + (cb * acc2[e] + cc * (sq2[e] * (1.0f / ORT_SCALE)));
-          else acc[e] = one + cb * acc[e] + cc * (sq[e] * (1.0f / ORT_SCALE));
+          const float one = 32 * ti + nloc(hi, e) == j ? ca * ORT_SCALE : 0.0f, s2 = sq2[e] * (1.0f / (ORT_SCALE * ORT_LESS));
+          if (square == ORT_THREE) acc[e] = (one + cb * acc[e] + cc * (sq[e] * (1.0f / ORT_SCALE))) + (cb * acc2[e] + cc * s2);
+          else acc[e] = one + cb * acc[e] + cc * (sq[e] * (1.0f / ORT_SCALE) + s2);
         }
         put(ah, al, acc);
       }
     }
     __syncthreads();
-    f32x16 y = {};
+    f32x16 y = {}, y2 = {};
 #pragma unroll 2
     for (int q = 0; q < 2 * rt; ++q) {
       const int lo = (32 * ti + l31) * px + 16 * q + 8 * hi, ro = (32 * tj + l31) * px + 16 * q + 8 * hi;
-      y = ort_mma3(*(const f16x8*)(ah + lo), *(const f16x8*)(al + lo), *(const f16x8*)(xh + ro), *(const f16x8*)(xl + ro), y);
+      ort_mma3(*(const f16x8*)(ah + lo), *(const f16x8*)(al + lo), *(const f16x8*)(xh + ro), *(const f16x8*)(xl + ro), y, y2);
     }
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] = y[e] * (1.0f / ORT_SCALE);
+    for (int e = 0; e < 16; ++e) x[e] = (y[e] + y2[e] * (1.0f / ORT_LESS)) * (1.0f / ORT_SCALE);
     __syncthreads();
   }
   asm volatile("" : "+v"(tid));
@@ -280,12 +282,11 @@ template <typename A> __device__ __forceinline__ void ort_tile_store(float* p, i
 #pragma unroll
   for (int q = 0; q < 4; ++q) *(float4*)(p + q * 256 + lane * 4) = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
 }
-// 32 x 32 tile of L R^T over 16 n columns; rows of `pl`, `pr` halves, lo planes dl, dr halves behind
-__device__ __forceinline__ f32x16 ort_tile_product(const _Float16* L, int dl, const _Float16* R, int dr, int n, f32x16 acc) {
+// 32 x 32 tile of L R^T over 16 n columns; lo planes dl, dr halves behind
+__device__ __forceinline__ void ort_tile_product(const _Float16* L, int dl, const _Float16* R, int dr, int n, f32x16& large, f32x16& small) {
 #pragma unroll 2
   for (int q = 0; q < n; ++q)
-    acc = ort_mma3(*(const f16x8*)(L + 16 * q), *(const f16x8*)(L + dl + 16 * q), *(const f16x8*)(R + 16 * q), *(const f16x8*)(R + dr + 16 * q), acc);
-  return acc;
+    ort_mma3(*(const f16x8*)(L + 16 * q), *(const f16x8*)(L + dl + 16 * q), *(const f16x8*)(R + 16 * q), *(const f16x8*)(R + dr + 16 * q), large, small);
 }
 
 template <typename T, int RT, int MODE>
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g
           for (int e = 0; e < 4; ++e) {
             const float one = 32 * ti + nloc(hi, 4 * q + e) == 32 * tj + l31 ? p.ca * ORT_SCALE : 0.0f;
             pp[4 * q + e] = (one + p.cb * (float)h4[e] + p.cc * (sq[4 * q + e] * (1.0f / ORT_SCALE))) +
-                          (p.cb * ((float)m4[e] + (float)l4[e]) + p.cc * (sq2[4 * q + e] * (1.0f / ORT_SCALE)));
+                          (p.cb * (((float)m4[e] + (float)l4[e] * (1.0f / ORT_LESS)) * (1.0f / ORT_LESS)) + p.cc * (sq2[4 * q + e] * (1.0f / (ORT_SCALE * ORT_LESS))));
           }
         }
       }
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g
     }
   } else {
     float a[16];
-    f32x16 sq = {};
+    f32x16 sq = {}, sq2 = {};
     if (gram) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) a[e] = 0.0f;
@@ -395,16 +396,16 @@ __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g
       put(A, plane_a, 32 * tj + l31, a);
     }
     __syncthreads();
-    if (gram) sq = ort_tile_product(A + (32 * ti + l31) * PA + 8 * hi, plane_a, A + (32 * tj + l31) * PA + 8 * hi, plane_a, 2 * RT, sq);
+    if (gram) ort_tile_product(A + (32 * ti + l31) * PA + 8 * hi, plane_a, A + (32 * tj + l31) * PA + 8 * hi, plane_a, 2 * RT, sq, sq2);
     __syncthreads();
     if (gram) {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        a[e] = (32 * ti + nloc(hi, e) == 32 * tj + l31 ? p.ca * ORT_SCALE : 0.0f) + p.cb * a[e] + p.cc * (sq[e] * (1.0f / ORT_SCALE));
+        a[e] = (32 * ti + nloc(hi, e) == 32 * tj + l31 ? p.ca * ORT_SCALE : 0.0f) + p.cb * a[e] + p.cc * ((sq[e] + sq2[e] * (1.0f / ORT_LESS)) * (1.0f / ORT_SCALE));
       put(A, plane_a, 32 * tj + l31, a);
     }
   }
-  f32x16 part = {}, less = {};                                        // (what the small parts add, by itself but for ORT_PAIRS)
+  f32x16 part = {}, less = {};
   for (int c = 0; c < p.chunks; ++c) {
     asm volatile("" : "+v"(tid));                                     // (no instruction: lane places are formed in the loop, not before it and spilled)
     lane = tid & 63; hi = lane >> 5; l31 = lane & 31;
@@ -422,10 +423,10 @@ __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g
       ort_tile_load(at, lane, x);
       put(X, plane_x, 32 * tj + l31, x);
       __syncthreads();                                                // X^T is there (and P)
-      f32x16 y = {};
-      y = ort_tile_product(A + (32 * ti + l31) * PA + 8 * hi, plane_a, X + (32 * tj + l31) * PA + 8 * hi, plane_x, 2 * RT, y);
+      f32x16 y = {}, y2 = {};
+      ort_tile_product(A + (32 * ti + l31) * PA + 8 * hi, plane_a, X + (32 * tj + l31) * PA + 8 * hi, plane_x, 2 * RT, y, y2);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = y[e] * (1.0f / ORT_SCALE);
+      for (int e = 0; e < 16; ++e) x[e] = (y[e] + y2[e] * (1.0f / ORT_LESS)) * (1.0f / ORT_SCALE);
     }
     if (MODE == ORT_FINAL) {
 #pragma unroll
@@ -441,20 +442,13 @@ __global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g
 #pragma unroll
       for (int e = 0; e < 16; ++e) ort_split(x[e], to[nloc(0, e) * PX], to[plane_x + nloc(0, e) * PX]);
       __syncthreads();
-      if (square != ORT_PAIRS && gram) {
-        const _Float16 *L = X + (32 * ti + l31) * PX + 8 * hi, *R = X + (32 * tj + l31) * PX + 8 * hi;
-#pragma unroll 2
-        for (int q = 0; q < 8; ++q)
-          ort_mma3(*(const f16x8*)(L + 16 * q), *(const f16x8*)(L + plane_x + 16 * q), *(const f16x8*)(R + 16 * q), *(const f16x8*)(R + plane_x + 16 * q), part, less);
-      } else if (gram) {
-        part = ort_tile_product(X + (32 * ti + l31) * PX + 8 * hi, plane_x, X + (32 * tj + l31) * PX + 8 * hi, plane_x, 8, part);
-      }
+      if (gram) ort_tile_product(X + (32 * ti + l31) * PX + 8 * hi, plane_x, X + (32 * tj + l31) * PX + 8 * hi, plane_x, 8, part, less);
       __syncthreads();
     }
   }
   if (MODE != ORT_FINAL && gram) {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) part[e] = (square != ORT_PAIRS ? part[e] + less[e] : part[e]) * (1.0f / ORT_SCALE);         // 4096 of A
+    for (int e = 0; e < 16; ++e) part[e] = (part[e] + less[e] * (1.0f / ORT_LESS)) * (1.0f / ORT_SCALE);         // 4096 of A
     ort_tile_store(p.gram_out + (((size_t)b * p.blocks + block) * RT * RT + ti * RT + tj) * 1024, lane, part);
   }
 }
@@ -646,7 +640,7 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
       src[q] += S::kg * 64;
     }
   };
-  f32x16 acc[S::ti][S::tj] = {};
+  f32x16 acc[S::ti][S::tj] = {}, less[S::ti][S::tj] = {};
   const int wi = (w / S::wn) * S::ti * 32, wj = (w % S::wn) * S::tj * 32;
   const int n_stages = s1 - s0, rounds = (n_stages + S::kg - 1) / S::kg, stages = (n_stages - kg + S::kg - 1) / S::kg;      // this group's stages
 #pragma unroll
@@ -687,12 +681,18 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
         for (int i = 0; i < S::ti; ++i)
 #pragma unroll
           for (int j = 0; j < S::tj; ++j)
-            acc[i][j] = ort_mma3(lh[kk][i], ll[kk][i], rh[kk][j], rl[kk][j], acc[i][j]);
+            ort_mma3(lh[kk][i], ll[kk][i], rh[kk][j], rl[kk][j], acc[i][j], less[i][j]);
     }
     }
     slot = slot + 1 == S::ns ? 0 : slot + 1;
     fill = fill + 1 == S::ns ? 0 : fill + 1;
   }
+#pragma unroll
+  for (int i = 0; i < S::ti; ++i)
+#pragma unroll
+    for (int j = 0; j < S::tj; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] += less[i][j][e] * (1.0f / ORT_LESS);
   // Results leave through LDS, a band of 32 rows of the wave's tile at a time, so that global stores are 16 bytes a lane and whole rows of
   // the tile: stored from the accumulators they were 2 bytes a lane, and 8 in the other orientation.
   constexpr int wmax = 32 * (S::ti > S::tj ? S::ti : S::tj) + 8;
@@ -789,7 +789,7 @@ __global__ __launch_bounds__(S::threads, S::threads / 256 * (S::ns * S::kg * S::
           const f16x4 h4 = *(const f16x4*)(a + 8 * q), l4 = *(const f16x4*)(a + 32 + 8 * q);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            v[4 * q + e] = (row0 + 8 * q + e == col ? p.ca * ORT_SCALE : 0.0f) + p.cb * ((float)h4[e] + (float)l4[e]) +
+            v[4 * q + e] = (row0 + 8 * q + e == col ? p.ca * ORT_SCALE : 0.0f) + p.cb * ((float)h4[e] + (float)l4[e] * (1.0f / ORT_LESS)) +
                            p.cc * (v[4 * q + e] * (1.0f / ORT_SCALE));
         }
       } else {

@@ -45,3 +45,44 @@ def test_sixteen_bits_are_the_binary32_result_rounded_once(nof, dtype, m, n, ran
         got, want = L.orthogonalize(u, steps=steps, coefficients=coef), L.orthogonalize(u.float(), steps=steps, coefficients=coef).double()
         beyond = ((got.double() - want).abs() - half_step(want, dtype)).clamp_min(0.0)
         assert got.dtype == dtype and float(beyond.norm()) <= 2.0 ** -13, (steps, coef, float(beyond.norm()), float(want.norm()))
+
+
+# Beside a binary32 computation of the same products.  There a product of two elements is rounded once, 2^-24 of it; here its operands are held to
+# 2^-23 each and lo lo, at most 2^-24 (2^-12 of either), is left out: five times as much.  The sums are binary32's in both.  So an error is at most five
+# times the binary32 computation's -- of a row, or a column, where those differ in size --, as long as what carries it lies above the smallest
+# that pairs hold, 2^-48 of the norm: P (|a| + |b| + |c| = s of magnitudes, r elements a row) and X bring s (1 + sqrt(r)) of those to a row of size `size`.
+def check_beside_binary32(got, u, steps, dim, coef=QUINTIC):
+    x = normalised(u)
+    want = iterate(x, steps, coef)
+    plain = iterate(x.float(), steps, coef).double()
+    size = x.norm(dim=dim).clamp_min(1e-300)
+    floor = 2.0 ** -48 * sum(abs(c) for c in coef) * (1 + min(u.shape[-2:]) ** 0.5) / size
+    off, ref = ((y - want).norm(dim=dim) / want.norm(dim=dim).clamp_min(1e-300) for y in (got.double(), plain))
+    bad = off > 5 * ref.amax(-1, keepdim=True) + floor
+    assert not bad.any(), (u.shape, steps, int(bad.sum()), float((off / (5 * ref.amax(-1, keepdim=True) + floor)).max()), float(off.max()), float(ref.max()))
+
+
+SHAPES = [(8, 4096), (8, 100), (40, 96), (64, 1000), (100, 120), (96, 96), (90, 700), (200, 400), (333, 1001), (130, 2300), (1024, 4096)]
+
+
+@pytest.mark.parametrize('m,n', SHAPES + [(n, m) for m, n in SHAPES])
+def test_rows_and_columns_of_very_different_size(nof, m, n):
+    """an embedding's seldom rows, units that are almost dead: 1e-5, 1e-7 of the others, and so many steps that they become part of the result"""
+    from bundlesdf_amd import learn_ops as L
+    for small in (1e-3, 1e-5, 1e-7):
+        rows, cols = randn(2, m, n, seed=m + n), randn(2, m, n, seed=m + n + 1)
+        rows[:, ::2] *= small
+        cols[:, :, 1::2] *= small
+        for steps in (5, 12):
+            check_beside_binary32(L.orthogonalize(rows, steps=steps), rows, steps, -1)
+            check_beside_binary32(L.orthogonalize(cols, steps=steps), cols, steps, -2)
+
+
+@pytest.mark.parametrize('m,n', [(8, 8), (50, 50), (120, 120), (20, 300), (150, 150), (300, 200)])
+def test_single_values_down_to_1e_9(nof, m, n):
+    from bundlesdf_amd import learn_ops as L
+    u = torch.zeros(m, n, device='cuda')
+    k = min(m, n)
+    u[torch.arange(k), torch.arange(k)] = torch.logspace(0, -9, k, device='cuda')
+    for steps in (5, 12):
+        check_beside_binary32(L.orthogonalize(u, steps=steps)[:k, :k], u[:k, :k], steps, -1)
