@@ -856,7 +856,10 @@ static bool ort_sizes_ok(int64_t batch, int64_t m, int64_t n) {
   return batch >= 0 && batch < 65536 && m >= 0 && m <= 16384 && n >= 0 && n <= 16384;
 }
 static bool ort_is_small(int64_t m, int64_t n) { return m <= ORT_SMALL && n <= ORT_SMALL; }
-// The tile of a product: 128 x 128 where that gives a workgroup per compute unit, else 64 x 64.  Images are padded to whole tiles.
+// The tile of a product: 128 x 128 where that occupies more than half of the 256 compute units, else 64 x 64; up to one tile a compute unit by
+// eight waves of it.  Images are padded to whole tiles.  Five steps as 64 x 64 and as 128 x 128, by X's tiles of 128 x 128: 2048 x 1024 (128) 290
+// and 314 us, 2500 x 1024 (160) 341 and 334, 3500 x 1024 (224) 396 and 370, 1920 x 2048 (240) 706 and 646; A and P of 2048 x 2048 (136)
+// 836 and 790 of the whole.  As eight waves and as four: 1920 x 2048 646 and 661, 2048 x 2048 (256) 790 and 822.
 typedef OrtShape<2, 2, 2, 2, 2, 1> OrtWide;
 typedef OrtShape<2, 2, 2, 2, 2, 2> OrtWideDeep;                        // one workgroup per compute unit at most: all of LDS is its ring
 typedef OrtShape<2, 2, 1, 1, 2, 2> OrtNarrow;
@@ -871,7 +874,7 @@ static int ort_cuts(int64_t batch, int64_t rp, int64_t kp) {
   if (kp < 1024 || want < 2 || kp * want < 6144) return 1;
   return (int)(want < most ? want : most);
 }
-static bool ort_wide(int64_t tiles_of_128) { return tiles_of_128 >= 256; }
+static bool ort_wide(int64_t tiles_of_128) { return tiles_of_128 > 128; }
 static int64_t ort_up(int64_t x, int64_t unit) { return nof_div_up(x, unit) * unit; }
 static int64_t ort_unit(int64_t batch, int64_t r, int64_t k) { return ort_wide(batch * nof_div_up(r, 128) * nof_div_up(k, 128)) ? 128 : 64; }
 
