@@ -86,3 +86,57 @@ def test_single_values_down_to_1e_9(nof, m, n):
     u[torch.arange(k), torch.arange(k)] = torch.logspace(0, -9, k, device='cuda')
     for steps in (5, 12):
         check_beside_binary32(L.orthogonalize(u, steps=steps)[:k, :k], u[:k, :k], steps, -1)
+
+
+@pytest.mark.parametrize('m,n', SHAPES + [(2048, 2048), (4001, 1100)])
+def test_low_rank_and_noise(nof, m, n):
+    """few strong directions over weak ones, which the steps lift: where single fp16 products are off by percents"""
+    from bundlesdf_amd import learn_ops as L
+    for noise in (0.0, 1e-4, 1e-2):
+        u = randn(m, 4, seed=m) @ randn(4, n, seed=n) + noise * randn(m, n, seed=m + n)
+        for steps in (1, 5):
+            x = normalised(u)
+            want = iterate(x, steps)
+            got, plain = L.orthogonalize(u, steps=steps).double(), iterate(x.float(), steps).double()
+            assert float((got - want).norm()) <= 5 * float((plain - want).norm()), (noise, steps, float((got - want).norm()), float((plain - want).norm()))
+
+
+# A multiple of the identity has one singular value, 1 / sqrt(k), and every product one term: the error is no average.  Of the value s, with
+# eta = 5 * 2^-24 a product, A is off by eta s^2 and A A by 4 eta s^4 at most (its two factors, itself, its storing), b A by 2, P by its storing and
+# its product with X: eta s (2 |b| s^2 + 4 |c| s^4 + 2 (|a| + |b| s^2 + |c| s^4)); a former error is multiplied by the slope.
+@pytest.mark.parametrize('k', [5, 30, 64, 100, 128, 200, 333, 1024, 2048])
+def test_multiple_of_the_identity(nof, k):
+    from bundlesdf_amd import learn_ops as L
+    a, b, c = QUINTIC
+    for steps in (1, 2, 5):
+        s, tol, eta = k ** -0.5, k ** -0.5 * 2.0 ** -22, 5 * 2.0 ** -24
+        for _ in range(steps):
+            tol = abs(a + 3 * b * s ** 2 + 5 * c * s ** 4) * tol * 1.01 + eta * s * (2 * abs(b) * s ** 2 + 4 * abs(c) * s ** 4 + 2 * abs(a) + 2 * abs(b) * s ** 2 + 2 * abs(c) * s ** 4)
+            s = s * (a + s ** 2 * (b + c * s ** 2))
+        got = L.orthogonalize(torch.eye(k, device='cuda') * 0.37, steps=steps).double()
+        assert float((got.diagonal() - s).abs().max()) <= tol, (steps, float((got.diagonal() - s).abs().max()), tol)
+        assert float((got - torch.diag(got.diagonal())).abs().max()) == 0.0
+
+
+# The products by tiles of 128 x 128: of X one tile a compute unit at most (2500 x 1024, 2048 x 2048 and its A and P), more (4001 x 1100; the last
+# two, of whose A and P too), of either orientation; padded to whole tiles or not; one matrix and several.
+@pytest.mark.parametrize('batch,m,n', [(1, 2500, 1024), (1, 1024, 2500), (1, 2048, 2048), (1, 4096, 1024), (1, 1024, 4096), (4, 1024, 1024), (1, 4001, 1100),
+                                       (1, 1100, 4001), (3, 1153, 1400), (9, 600, 900), (2, 2048, 2048), (1, 2950, 2900)])
+def test_large_tiles(nof, batch, m, n):
+    from bundlesdf_amd import learn_ops as L
+    u = randn(batch, m, n, seed=m + n) + randn(batch, m, 4, seed=m) @ randn(batch, 4, n, seed=n)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        v = u.to(dtype)
+        for steps in (1, 2, 5):
+            x = normalised(v)
+            want = iterate(x, steps)
+            off = (iterate(x.float(), steps).double() - want).flatten(1).norm(dim=1)
+            got = L.orthogonalize(v, steps=steps)
+            err = (got.double() - want).abs()
+            if dtype != torch.float32:                                # (beyond half a step at most twice what there was before the rounding)
+                err, off = (err - half_step(want, dtype)).clamp_min(0.0), 2 * off
+            assert (err.flatten(1).norm(dim=1) <= 5 * off).all(), (dtype, steps, err.flatten(1).norm(dim=1).tolist(), off.tolist())
+            assert torch.equal(got, L.orthogonalize(v, steps=steps))
+            w = v.clone()
+            L.orthogonalize(w, steps=steps, out=w)
+            assert torch.equal(got, w)
