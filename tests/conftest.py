@@ -30,9 +30,25 @@ _ORDER = ['test_gpu_erratum', 'test_gpu_ops', 'test_gpu_tiles', 'test_gpu_rays',
 _LAST = ['test_gpu_fullsize', 'test_gpu_dp']
 
 
+# These pass addresses that are none to the C entry points and expect each call to be refused before a launch: on a machine with a GPU, a check
+# that is missing would be a memory fault there instead of a failed test.
+_HOST_ONLY = ['test_learn_ops_host', 'test_learn_ops_limits']
+
+
+def _module(item):
+    return os.path.splitext(os.path.basename(str(item.fspath)))[0]
+
+
 def pytest_collection_modifyitems(session, config, items):
+    host_only = [item for item in items if _module(item) in _HOST_ONLY]
+    if host_only:
+        import torch
+        if torch.cuda.is_available():
+            for item in host_only:
+                item.add_marker(pytest.mark.skip(reason='passes addresses that are none: not on a machine with a GPU'))
+
     def key(item):
-        mod = os.path.splitext(os.path.basename(str(item.fspath)))[0]
+        mod = _module(item)
         if mod in _ORDER:
             return (0, _ORDER.index(mod))
         if mod in _LAST:
