@@ -27,3 +27,9 @@ def test_host_only_tests_do_not_meet_a_gpu(monkeypatch, gpu):
     items = collect(Item('test_learn_ops_host'), Item('test_learn_ops_limits'), Item('test_mesh'))
     assert {(i.fspath.split(os.sep)[-1], tuple(i.marks)) for i in items} == {
         ('test_learn_ops_host.py', ('skip',) if gpu else ()), ('test_learn_ops_limits.py', ('skip',) if gpu else ()), ('test_mesh.py', ())}
+
+
+def test_what_needs_files_from_outside_runs_last():
+    names = [i.name for i in collect(Item('test_gpu_chain', 'test_oracle_is_pinned_on_this_box'), Item('test_gpu_fullsize', 'a'), Item('test_gpu_learn_scan', 'b'),
+                                     Item('test_gpu_ops', 'c'))]
+    assert names == ['c', 'b', 'a', 'test_oracle_is_pinned_on_this_box']
