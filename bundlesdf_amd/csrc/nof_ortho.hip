@@ -1020,24 +1020,51 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
   }
 }
 
+// Where the singular values go: they start in [0, 1], and operands hold 4096 times |p| <= 15, |x| <= 2 without leaving fp16.  A step takes an
+// interval to an interval, whose ends lie at the old ends or where the polynomial is level.  The first step (from 1 on) that leaves, or 0.
+static int ort_leaves(const float* coef, int steps) {
+  double lo = 0.0, hi = 1.0;
+  for (int q = 0; q < steps; ++q) {
+    const double a = coef[3 * q], b = coef[3 * q + 1], c = coef[3 * q + 2], was[2] = {lo, hi};
+    double worst = 0.0;                                               // of |p|, at the squares' ends or where it is level
+    bool first = true;
+    auto at = [&](double s) {
+      const double l = s * s, p = a + l * (b + l * c), y = s * p;
+      if (!(fabs(p) <= worst)) worst = fabs(p);
+      if (first || !(y >= lo)) lo = y;
+      if (first || !(y <= hi)) hi = y;
+      first = false;
+    };
+    auto inside = [&](double l) {                                     // s = sqrt(l) and -sqrt(l), where they lie in the interval
+      if (!(l >= 0.0)) return;
+      const double s = sqrt(l);
+      if (s >= was[0] && s <= was[1]) at(s);
+      if (-s >= was[0] && -s <= was[1]) at(-s);
+    };
+    at(was[0]);
+    at(was[1]);
+    inside(0.0);
+    if (c != 0.0) inside(-b / (2.0 * c));
+    // a + 3 b l + 5 c l^2 = 0
+    const double d = 9.0 * b * b - 20.0 * a * c;
+    if (d >= 0.0) {
+      const double t = -0.5 * (3.0 * b + (b < 0.0 ? -sqrt(d) : sqrt(d)));
+      if (c != 0.0) inside(t / (5.0 * c));
+      if (t != 0.0) inside(a / t);
+    }
+    if (!(worst <= 15.0 && lo >= -2.0 && hi <= 2.0)) return q + 1;
+  }
+  return 0;
+}
+
 extern "C" int nof_orthogonalize(const void* update, void* out, int32_t type, int32_t steps, const float* h_coef, float eps, void* workspace,
                                  int64_t workspace_bytes, int64_t batch, int64_t m, int64_t n, void* stream) {
   NOF_ARG(learn_type_ok(type));
   NOF_ARG(ort_sizes_ok(batch, m, n));
   NOF_ARG(steps >= 1 && steps <= ORT_MAX_STEPS && h_coef && eps >= 0.0f && eps <= 3.0e38f);
   if (batch == 0 || m == 0 || n == 0) return 0;
-  // where the singular values go: they start in [0, 1], and operands hold 4096 times |p| <= 15, |x| <= 2 without leaving fp16
-  {
-    double s[129];
-    for (int i = 0; i <= 128; ++i) s[i] = i / 128.0;
-    for (int q = 0; q < steps; ++q)
-      for (int i = 0; i <= 128; ++i) {
-        const double l = s[i] * s[i], f = (double)h_coef[3 * q] + l * ((double)h_coef[3 * q + 1] + l * (double)h_coef[3 * q + 2]);
-        s[i] *= f;
-        if (!(fabs(f) <= 15.0 && fabs(s[i]) <= 2.0))
-          return nof_set_error(-1, "%s: argument check failed: these coefficients take singular values out of [0, 2] (step %d)", __func__, q);
-      }
-  }
+  if (const int q = ort_leaves(h_coef, steps))
+    return nof_set_error(-1, "%s: argument check failed: these coefficients take singular values out of [0, 2] (step %d)", __func__, q - 1);
   NOF_ARG(update && out);
   const int64_t need = nof_orthogonalize_workspace_bytes(batch, m, n);
   NOF_ARG(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need));

@@ -1,0 +1,55 @@
+"""Borders of what the learning operators take (bundlesdf_amd/learn_ops.py, the last section of include/nof_hip.h), on the host: what lies behind them is
+refused before anything is launched.  Never on a GPU: the addresses are none (tests/conftest.py)."""
+import ctypes as C
+
+import pytest
+
+from bundlesdf_amd import lib
+
+PTR = C.c_void_p(256)                                            # never dereferenced
+
+
+def refuses(rc):
+    return rc < 0 and b'argument check' in lib.load().nof_last_error()
+
+
+def orthogonalize(*triples):
+    """200 x 6 without a workspace: refused in any case, for the coefficients or for that"""
+    coef = (C.c_float * (3 * len(triples)))(*[x for t in triples for x in t])
+    return lib.load().nof_orthogonalize(PTR, PTR, 0, len(triples), coef, 1e-30, None, 0, 2, 200, 6, None)
+
+
+def leaves(*triples):
+    """in 64 bits, on a grid that is fine enough for the cases below"""
+    import numpy as np
+    s = np.linspace(0.0, 1.0, 1 << 18)
+    with np.errstate(invalid='ignore'):
+        for a, b, c in np.float32(triples).astype(float):
+            p = a + s * s * (b + s * s * c)
+            s = s * p
+            if not (np.abs(p).max() <= 15.0 and np.abs(s).max() <= 2.0):
+                return True
+    return False
+
+
+def test_coefficients_are_judged_between_any_grid_of_values():
+    # 3 / t (s - s^3 / (3 t^2)) has its largest value, 2, at t: here a little more, and less than 2 at every multiple of 1/128
+    t = 0.5 + 1 / 256
+    peak = (3.0 / t * 1.00002, -1.0 / t ** 3 * 1.00002, 0.0)
+    grid = [k / 128 * (peak[0] + (k / 128) ** 2 * peak[1]) for k in range(129)]
+    assert max(grid) < 2.0 and leaves(peak)
+    so = lib.load()
+    assert refuses(orthogonalize(peak)) and b'[0, 2]' in so.nof_last_error()
+    lower = (peak[0] * 0.9999, peak[1] * 0.9999, 0.0)
+    assert not leaves(lower) and refuses(orthogonalize(lower)) and b'workspace' in so.nof_last_error()      # taken: what is refused is the workspace
+
+
+@pytest.mark.parametrize('triples', [((3.4445, -4.7750, 2.0315),) * 32, ((1.5, -0.5, 0.0),) * 4, ((3.0, -3.2, 1.2), (2.0, -1.5, 0.5), (1.5, -0.5, 0.0)),
+                                     ((0.0, 0.0, 0.0), (15.0, 0.0, 0.0)), ((1.0, 0.0, 0.0),), ((-1.0, 0.0, 0.0), (1.5, -0.5, 0.0)), ((5.0, -20.0, 16.0),) * 6,
+                                     ((0.0, 2.0, 0.0),), ((0.0, 0.0, 2.0), (0.5, 0.0, 0.0)), ((8.2872, -23.5959, 17.3004), (4.1071, -2.9478, 0.5448)),
+                                     ((2.1, 0.0, 0.0),), ((15.5, -15.0, 0.0),), ((0.0, -2.5, 0.0),), ((1.9, 0.0, 0.0), (0.0, 0.0, 1.0)), ((14.0, -40.0, 27.0),),
+                                     ((-1.5, 0.0, 0.0), (1.6, 0.0, 0.0)), ((float('inf'), 0.0, 0.0),), ((1.0, float('nan'), 0.0),), ((1.0, 0.0, float('-inf')),)])
+def test_coefficients(triples):
+    so = lib.load()
+    assert refuses(orthogonalize(*triples))
+    assert (b'[0, 2]' in so.nof_last_error()) == leaves(*triples), so.nof_last_error()
