@@ -15,7 +15,7 @@
 #include "nof_learn_dev.h"
 
 #define EMB_T 256                       // threads of the streaming kernels
-#define EMB_ZROWS 32                    // table rows per workgroup of the zero role
+#define EMB_ZROWS 32                    // table rows per workgroup of the zero role at a time
 #define EMB_ZBYTES 65536                // of the sort's zero role per workgroup
 #define EMB_ZHIST ((int64_t)12 << 20)     // bytes of zeros that ride in one launch of the sort
 #define EMB_ZSCATTER ((int64_t)32 << 20)
@@ -25,6 +25,7 @@
 #define EMB_SORT_W (EMB_SORT_T / 64)
 #define EMB_BITS 10                     // widest digit of the many-workgroup sort
 #define EMB_MAX_BLOCKS 128
+#define EMB_MAX_GRID (1 << 22)          // workgroups of a role whose work has no such limit: a launch has less than 2^32 threads on an axis
 #define EMB_FEW_N 4096                  // positions that k_embed_few lists
 
 // ---- lookup -----------------------------------------------------------------------------------------------------------------------
@@ -310,19 +311,21 @@ __global__ __launch_bounds__(EMB_T) void k_embed_reduce(const T* __restrict__ do
   const int col = (((int)blockIdx.y << ls) + lane) * V;
   if (blockIdx.x >= n_red) {                                          // the zero role
     __shared__ uint8_t named[EMB_ZROWS];
-    const uint32_t v0 = zeroed + (blockIdx.x - n_red) * EMB_ZROWS;
-    if (threadIdx.x < EMB_ZROWS) {
-      const uint32_t v = v0 + threadIdx.x;
-      const uint32_t at = v < rows ? emb_lower(key, N, v) : 0;
-      named[threadIdx.x] = v >= rows || (at < N && key[at] == v);
-    }
-    __syncthreads();
     float z[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) z[k] = 0.0f;
-    if (col < D)
-      for (int r = threadIdx.x >> ls; r < EMB_ZROWS; r += EMB_T >> ls)
-        if (!named[r]) emb_store<T, V>(grad + (int64_t)(v0 + r) * D + col, D - col, z);
+    for (uint32_t v0 = zeroed + (blockIdx.x - n_red) * EMB_ZROWS; v0 < rows; v0 += (gridDim.x - n_red) * EMB_ZROWS) {        // (rows < 2^30: no overflow)
+      if (threadIdx.x < EMB_ZROWS) {
+        const uint32_t v = v0 + threadIdx.x;
+        const uint32_t at = v < rows ? emb_lower(key, N, v) : 0;
+        named[threadIdx.x] = v >= rows || (at < N && key[at] == v);
+      }
+      __syncthreads();
+      if (col < D)
+        for (int r = threadIdx.x >> ls; r < EMB_ZROWS; r += EMB_T >> ls)
+          if (!named[r]) emb_store<T, V>(grad + (int64_t)(v0 + r) * D + col, D - col, z);
+      __syncthreads();
+    }
     return;
   }
   const uint32_t chunk = blockIdx.x * (EMB_T >> ls) + (threadIdx.x >> ls);
@@ -568,7 +571,8 @@ static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* ke
   const int64_t nv = nof_div_up(D, EmbVec<T>::V);
   const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
   const unsigned cols = (unsigned)nof_div_up(nv, (int64_t)1 << ls), n_red = (unsigned)nof_div_up(p.chunks, EMB_T >> ls);
-  const unsigned n_zero = (unsigned)nof_div_up(p.s.rows - p.zeroed, EMB_ZROWS);
+  const int64_t zeros = nof_div_up(p.s.rows - p.zeroed, EMB_ZROWS);
+  const unsigned n_zero = (unsigned)(zeros < EMB_MAX_GRID ? zeros : EMB_MAX_GRID);
   // dout past the caches from half of the last one (256 MB) on.  65536 x 2048 bf16: the table's rows stay, a lookup behind it takes 60 us
   // instead of 84; 8192 x 1024: the launch takes 30 us so, 20 through the caches, where dout still lies.
   auto reduce = (int64_t)p.s.N * D * (int64_t)sizeof(T) >= (int64_t)128 << 20 ? k_embed_reduce<T, true> : k_embed_reduce<T, false>;

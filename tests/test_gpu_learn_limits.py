@@ -1,0 +1,30 @@
+"""The learning operators (bundlesdf_amd/learn_ops.py) at the far end of the sizes that they take."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def poisoned(*shape, dtype):
+    """the next tensor of this size lies where this one of NaN lay"""
+    x = torch.full(shape, float('nan'), dtype=dtype, device='cuda')
+    torch.cuda.synchronize()
+    del x
+
+
+@pytest.mark.parametrize('N', [0, 3000, 5000])
+def test_gradient_of_the_largest_table(nof, N):
+    """2^30 - 1 rows: every row that no id names is zero"""
+    from bundlesdf_amd import learn_ops as L
+    V = (1 << 30) - 1
+    gen = torch.Generator(device='cuda').manual_seed(N)
+    ids = torch.randint(0, V, (N,), device='cuda', generator=gen, dtype=torch.int64)
+    if N:
+        ids[:4] = torch.tensor([0, V - 1, V - 1, V // 2], device='cuda')
+    dout = torch.randint(1, 9, (N, 1), device='cuda', generator=gen).to(torch.bfloat16)
+    poisoned(V, 1, dtype=torch.bfloat16)
+    grad = L.embed_lookup_grad(dout, ids, V)
+    unique, where = torch.unique(ids, return_inverse=True)
+    want = torch.zeros(unique.numel(), device='cuda').index_add_(0, where, dout[:, 0].float())       # whole numbers of at most 8 bits: exact
+    assert torch.equal(grad[unique, 0].float(), want)
+    assert int(torch.count_nonzero(grad)) == unique.numel()
