@@ -391,46 +391,47 @@ __global__ __launch_bounds__(EMB_T) void k_embed_join(const uint32_t* __restrict
   constexpr int V = 4;
   const int DP = (D + 7) & ~7;
   __shared__ float sums[EMB_T * V];
-  const uint32_t chunk = blockIdx.x;
-  const uint64_t first = (uint64_t)chunk * C, end = first + C;
-  if (end >= N) return;
-  const uint32_t lo = (uint32_t)first, id = key[end - 1], after = key[end], start = key[lo], before = key[lo > 0 ? lo - 1 : 0];
-  if (id >= rows || after != id) return;                              // nothing handed on
-  if (start == id && lo > 0 && before == id) return;                  // nor started here
-  uint32_t last = chunk;                                              // the last run that starts with the id, as many runs at a time as threads
-  for (int more = EMB_T; more == EMB_T; last += more) {
-    const uint64_t at = ((uint64_t)last + 1 + threadIdx.x) * C;
-    more = __syncthreads_count(at < N && key[at] == id);
-  }
   const int lane = threadIdx.x & ((1 << ls) - 1), group = threadIdx.x >> ls, groups = EMB_T >> ls;
   const int col = (((int)blockIdx.y << ls) + lane) * V;
-  const uint32_t each = (last - chunk + groups - 1) / groups, c0 = chunk + 1 + group * each, c1 = c0 + each <= last ? c0 + each : last + 1;
-  float acc[V], x[V];
+  for (uint32_t chunk = blockIdx.x;; chunk += gridDim.x) {              // (at most 2^28 runs: no overflow)
+    const uint64_t first = (uint64_t)chunk * C, end = first + C;
+    if (end >= N) return;
+    const uint32_t lo = (uint32_t)first, id = key[end - 1], after = key[end], start = key[lo], before = key[lo > 0 ? lo - 1 : 0];
+    if (id >= rows || after != id) continue;                            // nothing handed on
+    if (start == id && lo > 0 && before == id) continue;                // nor started here
+    uint32_t last = chunk;                                              // the last run that starts with the id, as many runs at a time as threads
+    for (int more = EMB_T; more == EMB_T; last += more) {
+      const uint64_t at = ((uint64_t)last + 1 + threadIdx.x) * C;
+      more = __syncthreads_count(at < N && key[at] == id);
+    }
+    const uint32_t each = (last - chunk + groups - 1) / groups, c0 = chunk + 1 + group * each, c1 = c0 + each <= last ? c0 + each : last + 1;
+    float acc[V], x[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) acc[k] = 0.0f;
-  if (col < D) {
-    if (group == 0) lload<float, V>(part + ((size_t)chunk * 2 + 1) * DP + col, acc);
+    for (int k = 0; k < V; ++k) acc[k] = 0.0f;
+    if (col < D) {
+      if (group == 0) lload<float, V>(part + ((size_t)chunk * 2 + 1) * DP + col, acc);
 #pragma unroll 4
-    for (uint32_t c = c0; c < c1; ++c) {
-      lload<float, V>(part + ((size_t)c * 2) * DP + col, x);
+      for (uint32_t c = c0; c < c1; ++c) {
+        lload<float, V>(part + ((size_t)c * 2) * DP + col, x);
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] += x[k];
+        for (int k = 0; k < V; ++k) acc[k] += x[k];
+      }
     }
-  }
-  for (int o = 1; o < groups && o <= (int)(last - chunk - 1); o *= 2) {
+    for (int o = 1; o < groups && o <= (int)(last - chunk - 1); o *= 2) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) sums[threadIdx.x * V + k] = acc[k];
-    __syncthreads();
-    if ((group & (2 * o - 1)) == 0 && group + o < groups) {
+      for (int k = 0; k < V; ++k) sums[threadIdx.x * V + k] = acc[k];
+      __syncthreads();
+      if ((group & (2 * o - 1)) == 0 && group + o < groups) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] += sums[(threadIdx.x + (o << ls)) * V + k];
+        for (int k = 0; k < V; ++k) acc[k] += sums[(threadIdx.x + (o << ls)) * V + k];
+      }
+      __syncthreads();
     }
-    __syncthreads();
-  }
-  if (group == 0 && col < D) {
+    if (group == 0 && col < D) {
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (col + k < D) grad[(int64_t)id * D + col + k] = lt<T>(acc[k] * scale);
+      for (int k = 0; k < V; ++k)
+        if (col + k < D) grad[(int64_t)id * D + col + k] = lt<T>(acc[k] * scale);
+    }
   }
 }
 
@@ -581,7 +582,7 @@ static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* ke
   if (p.chunks > 1) {
     const int64_t jv = nof_div_up(D, 4);
     const int jl = learn_log2_up(jv < 64 ? jv : 64);
-    hipLaunchKernelGGL(k_embed_join<T>, dim3(p.chunks, (unsigned)nof_div_up(jv, (int64_t)1 << jl)), dim3(EMB_T), 0, st, key, p.s.N,
+    hipLaunchKernelGGL(k_embed_join<T>, dim3(p.chunks < EMB_MAX_GRID ? p.chunks : EMB_MAX_GRID, (unsigned)nof_div_up(jv, (int64_t)1 << jl)), dim3(EMB_T), 0, st, key, p.s.N,
                        (uint32_t)p.s.rows, D, scale, (T*)grad, (const float*)part, jl, p.C);
   }
 }

@@ -28,3 +28,21 @@ def test_gradient_of_the_largest_table(nof, N):
     want = torch.zeros(unique.numel(), device='cuda').index_add_(0, where, dout[:, 0].float())       # whole numbers of at most 8 bits: exact
     assert torch.equal(grad[unique, 0].float(), want)
     assert int(torch.count_nonzero(grad)) == unique.numel()
+
+
+def test_gradient_of_more_than_2_30_positions(nof):
+    """every id holds some thousand positions: runs up to the last are joined"""
+    from bundlesdf_amd import learn_ops as L
+    N, V = (1 << 30) + 70001, 1 << 20
+    ids, dout = torch.empty(N, dtype=torch.int32, device='cuda'), torch.empty(N, 1, device='cuda')
+    for lo in range(0, N, 1 << 27):
+        i = torch.arange(lo, min(lo + (1 << 27), N), device='cuda')
+        ids[lo:lo + (1 << 27)] = i % V
+        dout[lo:lo + (1 << 27), 0] = (i // V + i) % 7
+    poisoned(V, 1, dtype=torch.float32)
+    grad = L.embed_lookup_grad(dout, ids, V)
+    v = torch.arange(V, device='cuda')
+    want = torch.zeros(V, dtype=torch.int64, device='cuda')
+    for k in range(-(-N // V)):
+        want += torch.where(k * V + v < N, (k + k * V + v) % 7, 0)
+    assert torch.equal(grad[:, 0].long(), want)                       # whole numbers below 2^24: exact in any order
