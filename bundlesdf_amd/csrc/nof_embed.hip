@@ -511,7 +511,13 @@ static int emb_chunk(int64_t N, int32_t D, int size) {
   return c;
 }
 
-struct EmbPlan { EmbSort s; bool few, small; int64_t key[2], pos[2], hist, part, bytes, zeroed; int C; uint32_t chunks; };       // zeroed: rows that the sort's launches clear
+struct EmbPlan {
+  EmbSort s;
+  bool few, small;
+  int64_t key[2], pos[2], hist, part, bytes, zeroed;                  // zeroed: rows that the sort's launches clear
+  int C, ls;                                                          // positions a run; 2^ls lanes a row
+  uint32_t chunks, n_red;                                             // runs; workgroups that add them
+};
 
 // k_embed_few: every row's workgroups look all ids over, so few positions and rows x slices.  Against the sort: 4096 positions, 64 rows of 16
 // fp32 9 us and 18 (15 and 21 if all name one row), 4096 rows of 32 16 and 24, 8000 of 16 25 and 24; 256 positions, 16000 rows 13 and 16;
@@ -539,8 +545,11 @@ static EmbPlan emb_plan(int64_t N, int64_t rows, int32_t D, int size) {
     p.s.per = (uint32_t)(nof_div_up(per, EMB_SORT_T) * EMB_SORT_T);
     p.s.n_blocks = (int)nof_div_up(N, p.s.per);
   }
+  const int64_t nv = nof_div_up(D, 16 / size);
+  p.ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
   p.C = emb_chunk(N, D, size);
   p.chunks = (uint32_t)nof_div_up(N, p.C);
+  p.n_red = (uint32_t)nof_div_up(p.chunks, EMB_T >> p.ls);
   int64_t at = 0;
   for (int k = 0; k < 2; ++k) {
     p.key[k] = at; at += learn_align(4 * N);
@@ -551,6 +560,9 @@ static EmbPlan emb_plan(int64_t N, int64_t rows, int32_t D, int size) {
   p.bytes = at;
   return p;
 }
+
+// whether the sums and the zero role fit a launch (less than 2^32 threads)
+static bool emb_launches(const EmbPlan& p) { return (int64_t)p.n_red + EMB_MAX_GRID < (int64_t)1 << 24; }
 
 static bool emb_sizes_ok(int64_t N, int64_t V, int32_t D) {
   return N >= 0 && N < ((int64_t)1 << 31) - 65536 && V >= 0 && V < (int64_t)1 << 30 && D >= 0 && D <= 1 << 20;
@@ -569,16 +581,14 @@ static void emb_launch_fwd(const void* table, int64_t stride, const void* ids, i
 template <typename T>
 static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* key, const uint32_t* pos, float scale, void* grad, float* part,
                             const EmbPlan& p, int32_t D, hipStream_t st) {
-  const int64_t nv = nof_div_up(D, EmbVec<T>::V);
-  const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
-  const unsigned cols = (unsigned)nof_div_up(nv, (int64_t)1 << ls), n_red = (unsigned)nof_div_up(p.chunks, EMB_T >> ls);
+  const unsigned cols = (unsigned)nof_div_up(nof_div_up(D, EmbVec<T>::V), (int64_t)1 << p.ls);
   const int64_t zeros = nof_div_up(p.s.rows - p.zeroed, EMB_ZROWS);
   const unsigned n_zero = (unsigned)(zeros < EMB_MAX_GRID ? zeros : EMB_MAX_GRID);
   // dout past the caches from half of the last one (256 MB) on.  65536 x 2048 bf16: the table's rows stay, a lookup behind it takes 60 us
   // instead of 84; 8192 x 1024: the launch takes 30 us so, 20 through the caches, where dout still lies.
   auto reduce = (int64_t)p.s.N * D * (int64_t)sizeof(T) >= (int64_t)128 << 20 ? k_embed_reduce<T, true> : k_embed_reduce<T, false>;
-  hipLaunchKernelGGL(reduce, dim3(n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N, (uint32_t)p.s.rows, D, scale,
-                     (T*)grad, part, ls, p.C, n_red, (uint32_t)p.zeroed);
+  hipLaunchKernelGGL(reduce, dim3(p.n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N, (uint32_t)p.s.rows, D, scale,
+                     (T*)grad, part, p.ls, p.C, p.n_red, (uint32_t)p.zeroed);
   if (p.chunks > 1) {
     const int64_t jv = nof_div_up(D, 4);
     const int jl = learn_log2_up(jv < 64 ? jv : 64);
@@ -612,8 +622,9 @@ extern "C" int nof_embed_fwd(const void* table, int64_t table_stride, int32_t ty
 
 extern "C" int64_t nof_embed_bwd_workspace_bytes(int64_t N, int64_t V, int32_t D) {
   if (!emb_sizes_ok(N, V, D)) return -1;
-  const int64_t a = emb_plan(N, V, D, 2).bytes, b = emb_plan(N, V, D, 4).bytes;        // (of any type)
-  return a > b ? a : b;
+  const EmbPlan a = emb_plan(N, V, D, 2), b = emb_plan(N, V, D, 4);    // (of any type)
+  if (!emb_launches(a)) return -1;                                    // (wider rows take more)
+  return emb_launches(b) && b.bytes > a.bytes ? b.bytes : a.bytes;
 }
 
 extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type, const void* ids, int32_t ids64, float scale,
@@ -623,6 +634,7 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
   if (V == 0 || D == 0) return 0;
   NOF_ARG(grad_table && (N == 0 || (dout && ids && workspace)));
   EmbPlan p = emb_plan(N, V, D, (int)learn_type_size(type));
+  NOF_ARG(emb_launches(p));
   NOF_ARG(N == 0 || workspace_bytes >= p.bytes);
   NOF_ARG(N == 0 || ((uintptr_t)workspace & 255) == 0);
   hipStream_t st = (hipStream_t)stream;

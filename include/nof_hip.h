@@ -564,7 +564,8 @@ int nof_grad_check(const float* grad, int64_t n, int32_t* flags, void* stream);
 int nof_embed_fwd(const void* table, int64_t table_stride, int32_t type, const void* ids, int32_t ids64, float scale, void* out,
                   int64_t N, int64_t V, int32_t D, void* stream);
 /* grad_table [V,D], overwritten, = scale * the sum of the rows of dout [N,D] (row stride `dout_stride`) whose id names the row; ids
- * outside [0, V) contribute nothing.  Sums in binary32, in the order of the positions: equal inputs give equal bits. */
+ * outside [0, V) contribute nothing.  Sums in binary32, in an order that the ids give: equal inputs give equal bits.  Rows of more than 1024
+ * bytes: N < 3 * 2^29, of more than 2048: N < 3 * 2^28. */
 int64_t nof_embed_bwd_workspace_bytes(int64_t N, int64_t V, int32_t D);
 int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type, const void* ids, int32_t ids64, float scale, void* grad_table,
                   void* workspace, int64_t workspace_bytes, int64_t N, int64_t V, int32_t D, void* stream);

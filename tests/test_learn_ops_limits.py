@@ -53,3 +53,18 @@ def test_coefficients(triples):
     so = lib.load()
     assert refuses(orthogonalize(*triples))
     assert (b'[0, 2]' in so.nof_last_error()) == leaves(*triples), so.nof_last_error()
+
+
+def test_embed_gradient_of_more_runs_than_a_launch_holds():
+    so = lib.load()
+
+    def bwd(type, N, D):
+        return so.nof_embed_bwd(PTR, D, type, PTR, 0, 1.0, PTR, PTR, 1 << 50, N, 4, D, None)
+
+    # bytes of a row: workgroups of the sums, 64 positions a run, 256 threads; a launch holds less than 2^24 of them, 2^22 are the zero role's
+    for D, N in ((257, 3 << 29), (512, 3 << 29), (513, 3 << 28), (1 << 20, 3 << 28)):
+        assert refuses(bwd(0, N, D)) and b'launches' in so.nof_last_error(), (D, N)
+        assert refuses(bwd(1, N, 2 * D)) if 2 * D <= 1 << 20 else True
+        assert so.nof_embed_bwd_workspace_bytes(N, 4, 2 * D if 2 * D <= 1 << 20 else D) == -1
+        assert so.nof_embed_bwd_workspace_bytes(N - 64, 4, D) > 16 * N
+    assert so.nof_embed_bwd_workspace_bytes((1 << 31) - 65537, 4, 256) > 16 << 31
