@@ -538,7 +538,7 @@ static bool scan_plan(ScanArgs& p, int64_t B, int64_t T, int32_t D, int32_t G, i
   p.mark = p.chunk;
   p.n_marks = p.n_chunks;
   if (!back) scan_layout(p, D, v);
-  return B * p.tiles < (int64_t)1 << 31;
+  return B * p.tiles * p.waves * 64 < (int64_t)1 << 32;               // (threads of a launch)
 }
 
 // two 16-bit channels a lane where a group is even
@@ -599,7 +599,7 @@ extern "C" int64_t nof_gated_scan_workspace_bytes(int64_t B, int64_t T, int32_t 
   ScanArgs p = {};
   if (!scan_plan(p, B, T, D, G, scan_vec(type, D, G), false)) return -1;
   const int64_t fwd = scan_seg_bytes(p);
-  if (!scan_plan(p, B, T, D, G, scan_vec(type, D, G), true)) return -1;
+  if (!scan_plan(p, B, T, D, G, scan_vec(type, D, G), true)) return fwd;                 // (a backward call of these sizes is refused)
   const int64_t bwd = scan_seg_bytes(p) + scan_gpart_bytes(p);
   return fwd > bwd ? fwd : bwd;
 }

@@ -576,7 +576,8 @@ int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type, const voi
  * the others are not read, their rows of h, dgate, dvalue are zeros.  reverse = 1: the recurrence runs from row lengths[b] - 1 down to 0.
  * Positions compose in parallel, so products of gates over a run of positions must stay within binary32 (|gate| <= 1 always does).
  * 16-bit types with an even number of channels per group: pointers and strides (a shared gate's aside) are multiples of two elements.
- * B < 2^24, T < 2^31, D <= 2^20. */
+ * B < 2^24, T < 2^31, D <= 2^20.  A launch holds less than 2^32 threads: B D < 2^24 always fits (and far more where rows are wide), what does
+ * not is refused; the workspace query answers for the forward where only the backward does not. */
 int64_t nof_gated_scan_marks_bytes(int64_t B, int64_t T, int32_t D, int32_t G, int32_t type);
 int64_t nof_gated_scan_workspace_bytes(int64_t B, int64_t T, int32_t D, int32_t G, int32_t type);
 int nof_gated_scan_fwd(const void* gate, int64_t gate_sb, int64_t gate_st, int32_t gate_type, const void* value, int64_t value_sb,

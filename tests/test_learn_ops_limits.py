@@ -68,3 +68,23 @@ def test_embed_gradient_of_more_runs_than_a_launch_holds():
         assert so.nof_embed_bwd_workspace_bytes(N, 4, 2 * D if 2 * D <= 1 << 20 else D) == -1
         assert so.nof_embed_bwd_workspace_bytes(N - 64, 4, D) > 16 * N
     assert so.nof_embed_bwd_workspace_bytes((1 << 31) - 65537, 4, 256) > 16 << 31
+
+
+def test_scans_of_more_threads_than_a_launch_holds():
+    so = lib.load()
+    null = C.c_void_p(None)
+
+    def fwd(t, B, T, D, G):
+        return so.nof_gated_scan_fwd(PTR, T * G, G, t, PTR, T * D, D, t, null, null, 0, PTR, PTR, null, PTR, 1 << 50, B, T, D, G, None)
+
+    def bwd(t, B, T, D, G):
+        return so.nof_gated_scan_bwd(PTR, T * G, G, t, PTR, T * D, D, t, PTR, T * D, D, null, PTR, null, 0, PTR, PTR, PTR, PTR, 1 << 50, B, T, D, G, None)
+
+    # (type, B, T, D, G): tiles of 64 channels (of two in 16 bits) by one wave; by four; in the backward, a group of two channels is a tile
+    for t, B, T, D, G in ((0, 1 << 23, 1, 512, 512), (1, 1 << 23, 1, 1024, 1024), (0, 1 << 21, 64, 512, 1), (0, 1 << 22, 1, 1024, 1024), (2, 1 << 21, 64, 1024, 2)):
+        size = so.nof_gated_scan_workspace_bytes
+        assert refuses(fwd(t, B, T, D, G)) and refuses(bwd(t, B, T, D, G)), (t, B, T, D, G)
+        assert size(B, T, D, G, t) == -1 and so.nof_gated_scan_marks_bytes(B, T, D, G, t) == -1
+        assert size(B - 1, T, D, G, t) >= 0
+    assert refuses(bwd(1, 1 << 17, 1, 1024, 512)) and so.nof_gated_scan_workspace_bytes(1 << 17, 1, 1024, 512, 1) == 0      # (the forward's)
+    assert so.nof_gated_scan_workspace_bytes((1 << 24) - 1, 100000, 1, 1, 0) >= 0                # 256 threads for every B x D: the most
