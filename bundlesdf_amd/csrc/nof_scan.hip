@@ -682,10 +682,10 @@ extern "C" int nof_gated_scan_step(const void* gate, int64_t gate_sb, int32_t ga
                                    const float* state, float* new_state, void* h, int64_t B, int32_t D, int32_t G, void* stream) {
   NOF_ARG(scan_types_ok(type, gate_type));
   NOF_ARG(scan_sizes_ok(B, 1, D, G) && gate_sb >= 0 && value_sb >= 0);
-  NOF_ARG(B * nof_div_up(D, 256) < (int64_t)1 << 31);
   if (B == 0 || D == 0) return 0;
   NOF_ARG(gate && value && state && new_state && h);
   const int v = scan_vec(type, D, G), size = (int)learn_type_size(type);
+  NOF_ARG(B * nof_div_up(D, 256 * v) < (int64_t)1 << 24);             // (less than 2^32 threads)
   NOF_ARG(scan_aligned(value, value_sb, 0, size, v) && scan_aligned(h, 0, 0, size, v));
   NOF_ARG(G != D || scan_aligned(gate, gate_sb, 0, (int)learn_type_size(gate_type), v));
   NOF_ARG(scan_aligned(state, 0, 0, 4, v) && scan_aligned(new_state, 0, 0, 4, v));

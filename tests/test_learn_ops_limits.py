@@ -88,3 +88,10 @@ def test_scans_of_more_threads_than_a_launch_holds():
         assert size(B - 1, T, D, G, t) >= 0
     assert refuses(bwd(1, 1 << 17, 1, 1024, 512)) and so.nof_gated_scan_workspace_bytes(1 << 17, 1, 1024, 512, 1) == 0      # (the forward's)
     assert so.nof_gated_scan_workspace_bytes((1 << 24) - 1, 100000, 1, 1, 0) >= 0                # 256 threads for every B x D: the most
+
+
+def test_step_of_more_threads_than_a_launch_holds():
+    so = lib.load()
+    for t, B, D in ((0, 1 << 22, 1024), (0, 1 << 23, 257), (1, 1 << 22, 2048), (2, 1 << 23, 514), (1, 1 << 23, 511), (0, (1 << 24) - 1, 1 << 20)):
+        rc = so.nof_gated_scan_step(PTR, D, t, PTR, D, t, PTR, PTR, PTR, B, D, D, None)
+        assert refuses(rc) and b'24' in so.nof_last_error(), (t, B, D)
