@@ -574,7 +574,7 @@ static void emb_launch_fwd(const void* table, int64_t stride, const void* ids, i
   const int64_t nv = nof_div_up(D, EmbVec<T>::V);
   const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
   const int64_t want = nof_div_up(N, EMB_T >> ls), most = (int64_t)1 << 20;
-  hipLaunchKernelGGL(k_embed_fwd<T>, dim3((unsigned)(want < most ? want : most), (unsigned)nof_div_up(nv, (int64_t)1 << ls)), dim3(EMB_T), 0, st,
+  LEARN_LAUNCH(k_embed_fwd<T>, dim3((unsigned)(want < most ? want : most), (unsigned)nof_div_up(nv, (int64_t)1 << ls)), dim3(EMB_T), 0, st,
                      (const T*)table, stride, ids, ids64, scale, (T*)out, N, rows, D, ls);
 }
 
@@ -587,12 +587,12 @@ static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* ke
   // dout past the caches from half of the last one (256 MB) on.  65536 x 2048 bf16: the table's rows stay, a lookup behind it takes 60 us
   // instead of 84; 8192 x 1024: the launch takes 30 us so, 20 through the caches, where dout still lies.
   auto reduce = (int64_t)p.s.N * D * (int64_t)sizeof(T) >= (int64_t)128 << 20 ? k_embed_reduce<T, true> : k_embed_reduce<T, false>;
-  hipLaunchKernelGGL(reduce, dim3(p.n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N, (uint32_t)p.s.rows, D, scale,
+  LEARN_LAUNCH(reduce, dim3(p.n_red + n_zero, cols), dim3(EMB_T), 0, st, (const T*)dout, stride, key, pos, p.s.N, (uint32_t)p.s.rows, D, scale,
                      (T*)grad, part, p.ls, p.C, p.n_red, (uint32_t)p.zeroed);
   if (p.chunks > 1) {
     const int64_t jv = nof_div_up(D, 4);
     const int jl = learn_log2_up(jv < 64 ? jv : 64);
-    hipLaunchKernelGGL(k_embed_join<T>, dim3(p.chunks < EMB_MAX_GRID ? p.chunks : EMB_MAX_GRID, (unsigned)nof_div_up(jv, (int64_t)1 << jl)), dim3(EMB_T), 0, st, key, p.s.N,
+    LEARN_LAUNCH(k_embed_join<T>, dim3(p.chunks < EMB_MAX_GRID ? p.chunks : EMB_MAX_GRID, (unsigned)nof_div_up(jv, (int64_t)1 << jl)), dim3(EMB_T), 0, st, key, p.s.N,
                        (uint32_t)p.s.rows, D, scale, (T*)grad, (const float*)part, jl, p.C);
   }
 }
@@ -602,7 +602,7 @@ template <typename T>
 static void emb_launch_few(const void* dout, int64_t stride, const void* ids, int ids64, float scale, void* grad, const EmbPlan& p, int32_t D, hipStream_t st) {
   const int64_t nv = nof_div_up(D, EmbVec<T>::V);
   const int ls = learn_log2_up(nv < 8 ? nv : 8);
-  hipLaunchKernelGGL(k_embed_few<T>, dim3((unsigned)p.s.rows, (unsigned)nof_div_up(nv, (int64_t)1 << ls)), dim3(EMB_T), 0, st, (const T*)dout, stride, ids,
+  LEARN_LAUNCH(k_embed_few<T>, dim3((unsigned)p.s.rows, (unsigned)nof_div_up(nv, (int64_t)1 << ls)), dim3(EMB_T), 0, st, (const T*)dout, stride, ids,
                      ids64, (int)p.s.N, D, scale, (T*)grad, ls);
 }
 
@@ -613,10 +613,11 @@ extern "C" int nof_embed_fwd(const void* table, int64_t table_stride, int32_t ty
   if (N == 0 || D == 0) return 0;
   NOF_ARG(ids && out && (table || V == 0));
   hipStream_t st = (hipStream_t)stream;
+  LEARN_BEGIN();
   if (type == NOF_TYPE_F32) emb_launch_fwd<float>(table, table_stride, ids, ids64, scale, out, N, V, D, st);
   else if (type == NOF_TYPE_BF16) emb_launch_fwd<__bf16>(table, table_stride, ids, ids64, scale, out, N, V, D, st);
   else emb_launch_fwd<_Float16>(table, table_stride, ids, ids64, scale, out, N, V, D, st);
-  NOF_LAUNCH_OK();
+  LEARN_END();
   return 0;
 }
 
@@ -638,11 +639,12 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
   NOF_ARG(N == 0 || workspace_bytes >= p.bytes);
   NOF_ARG(N == 0 || ((uintptr_t)workspace & 255) == 0);
   hipStream_t st = (hipStream_t)stream;
+  LEARN_BEGIN();
   if (p.few) {
     if (type == NOF_TYPE_F32) emb_launch_few<float>(dout, dout_stride, ids, ids64, scale, grad_table, p, D, st);
     else if (type == NOF_TYPE_BF16) emb_launch_few<__bf16>(dout, dout_stride, ids, ids64, scale, grad_table, p, D, st);
     else emb_launch_few<_Float16>(dout, dout_stride, ids, ids64, scale, grad_table, p, D, st);
-    NOF_LAUNCH_OK();
+    LEARN_END();
     return 0;
   }
   char* ws = (char*)workspace;
@@ -668,21 +670,21 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
     };
     if (p.small) {
       const unsigned more = share(left);
-      hipLaunchKernelGGL(k_embed_sort_small, dim3(1 + more), dim3(1024), 0, st, ids, (int)ids64, V, (int)N, p.s.passes, key[0], pos[0], z);
+      LEARN_LAUNCH(k_embed_sort_small, dim3(1 + more), dim3(1024), 0, st, ids, (int)ids64, V, (int)N, p.s.passes, key[0], pos[0], z);
     } else {
       for (int pass = 0; pass < p.s.passes; ++pass, cur ^= 1) {
         unsigned more = share(EMB_ZHIST);
-        hipLaunchKernelGGL(k_embed_hist, dim3(p.s.n_blocks + more), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur], hist, z);
+        LEARN_LAUNCH(k_embed_hist, dim3(p.s.n_blocks + more), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur], hist, z);
         more = share(EMB_ZSCATTER);
-        hipLaunchKernelGGL(k_embed_scatter, dim3(p.s.n_blocks + more), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur],
+        LEARN_LAUNCH(k_embed_scatter, dim3(p.s.n_blocks + more), dim3(EMB_SORT_T), 0, st, p.s, pass, (const uint32_t*)key[cur],
                            (const uint32_t*)pos[cur], key[cur ^ 1], pos[cur ^ 1], (const uint32_t*)hist, z);
       }
     }
-    NOF_LAUNCH_OK();
+    LEARN_END();
   }
   if (type == NOF_TYPE_F32) emb_launch_sums<float>(dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
   else if (type == NOF_TYPE_BF16) emb_launch_sums<__bf16>(dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
   else emb_launch_sums<_Float16>(dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
-  NOF_LAUNCH_OK();
+  LEARN_END();
   return 0;
 }

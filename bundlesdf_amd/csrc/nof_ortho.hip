@@ -907,7 +907,7 @@ static void ort_launch_small(const void* g, void* out, int64_t batch, int64_t m,
   const int rt = (int)nof_div_up(m < n ? m : n, 32);
   constexpr size_t lds = (size_t)2 * 32 * (2 * KT + ort_parts(RT) * RT) * (32 * KT + 8);      // 136 KiB for KT = RT = 4
   if (lds > 64 << 10) (void)hipFuncSetAttribute((const void*)&k_ortho_small<T, KT, RT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  hipLaunchKernelGGL((k_ortho_small<T, KT, RT>), dim3((unsigned)batch), dim3(64 * rt * KT), lds, st, (const T*)g, (T*)out, (int)m, (int)n, steps, c, eps);
+  LEARN_LAUNCH((k_ortho_small<T, KT, RT>), dim3((unsigned)batch), dim3(64 * rt * KT), lds, st, (const T*)g, (T*)out, (int)m, (int)n, steps, c, eps);
 }
 
 template <int MODE, typename S> static int64_t ort_tiles(const OrtArgs& p) {
@@ -918,7 +918,7 @@ template <int MODE, typename T, typename S>
 static void ort_gemm(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
   p.tiles = (int)ort_tiles<MODE, S>(p);
   const int64_t parts = MODE == ORT_GRAM ? p.split : 1;
-  hipLaunchKernelGGL((k_ortho_gemm<MODE, T, S>), dim3((unsigned)(p.tiles * batch * parts)), dim3(S::threads), 0, st, p, out);
+  LEARN_LAUNCH((k_ortho_gemm<MODE, T, S>), dim3((unsigned)(p.tiles * batch * parts)), dim3(S::threads), 0, st, p, out);
 }
 template <int MODE, typename T>
 static void ort_product(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
@@ -943,8 +943,8 @@ static int ort_launch_norm(const void* g, double* part, int64_t batch, int64_t m
   const bool wide = ((uintptr_t)g & 15) == 0 && m * n % V == 0;
   const int64_t want = nof_div_up(m * n, 256 * 8 * (wide ? 4 : 1));
   const int n_part = (int)(want < ORT_NORM_BLOCKS ? want : ORT_NORM_BLOCKS);
-  if (wide) hipLaunchKernelGGL((k_ortho_norm<T, V>), dim3(n_part, (unsigned)batch), dim3(256), 0, st, (const T*)g, m * n, part);
-  else hipLaunchKernelGGL((k_ortho_norm<T, 1>), dim3(n_part, (unsigned)batch), dim3(256), 0, st, (const T*)g, m * n, part);
+  if (wide) LEARN_LAUNCH((k_ortho_norm<T, V>), dim3(n_part, (unsigned)batch), dim3(256), 0, st, (const T*)g, m * n, part);
+  else LEARN_LAUNCH((k_ortho_norm<T, 1>), dim3(n_part, (unsigned)batch), dim3(256), 0, st, (const T*)g, m * n, part);
   return n_part;
 }
 
@@ -953,7 +953,7 @@ static void ort_thin_step(const void* g, void* out, const OrtThin& p, int64_t ba
   constexpr int px = 128 * (32 * RT + 8) > 32 * RT * 136 ? 128 * (32 * RT + 8) : 32 * RT * 136;
   constexpr size_t lds = 2 * (size_t)(2 * px + ort_parts(RT) * 32 * RT * (32 * RT + 8));                              // 136 KiB for RT = 4
   if (lds > 64 << 10) (void)hipFuncSetAttribute((const void*)&k_ortho_thin<T, RT, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  hipLaunchKernelGGL((k_ortho_thin<T, RT, MODE>), dim3((unsigned)(batch * p.blocks)), dim3(256 * RT), lds, st, (const T*)g, (T*)out, p);
+  LEARN_LAUNCH((k_ortho_thin<T, RT, MODE>), dim3((unsigned)(batch * p.blocks)), dim3(256 * RT), lds, st, (const T*)g, (T*)out, p);
 }
 template <typename T, int RT>
 static void ort_launch_thin(const void* g, void* out, void* workspace, int64_t batch, int64_t m, int64_t n, int32_t steps, const float* coef, float eps,
@@ -1009,7 +1009,7 @@ static void ort_launch(const void* g, void* out, void* workspace, int64_t batch,
   p.parts = (float*)(p.ws + batch * p.per);
   const unsigned nb = (unsigned)batch;
   const int n_part = ort_launch_norm<T>(g, part, batch, m, n, st);
-  hipLaunchKernelGGL(k_ortho_split<T>, dim3((p.tall ? p.rp : p.kp) / 64, (p.tall ? p.kp : p.rp) / 64, nb), dim3(256), 0, st, (const T*)g,
+  LEARN_LAUNCH(k_ortho_split<T>, dim3((p.tall ? p.rp : p.kp) / 64, (p.tall ? p.kp : p.rp) / 64, nb), dim3(256), 0, st, (const T*)g,
                      (const double*)part, n_part, p, eps);
   for (int s = 0; s < steps; ++s, p.cur ^= 1) {
     p.ca = coef[3 * s]; p.cb = coef[3 * s + 1]; p.cc = coef[3 * s + 2];
@@ -1069,9 +1069,10 @@ extern "C" int nof_orthogonalize(const void* update, void* out, int32_t type, in
   const int64_t need = nof_orthogonalize_workspace_bytes(batch, m, n);
   NOF_ARG(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need));
   hipStream_t st = (hipStream_t)stream;
+  LEARN_BEGIN();
   if (type == NOF_TYPE_F32) ort_launch<float>(update, out, workspace, batch, m, n, steps, h_coef, eps, st);
   else if (type == NOF_TYPE_BF16) ort_launch<__bf16>(update, out, workspace, batch, m, n, steps, h_coef, eps, st);
   else ort_launch<_Float16>(update, out, workspace, batch, m, n, steps, h_coef, eps, st);
-  NOF_LAUNCH_OK();
+  LEARN_END();
   return 0;
 }

@@ -1,6 +1,9 @@
 """Borders of what the learning operators take (bundlesdf_amd/learn_ops.py, the last section of include/nof_hip.h), on the host: what lies behind them is
 refused before anything is launched.  Never on a GPU: the addresses are none (tests/conftest.py)."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -95,3 +98,51 @@ def test_step_of_more_threads_than_a_launch_holds():
     for t, B, D in ((0, 1 << 22, 1024), (0, 1 << 23, 257), (1, 1 << 22, 2048), (2, 1 << 23, 514), (1, 1 << 23, 511), (0, (1 << 24) - 1, 1 << 20)):
         rc = so.nof_gated_scan_step(PTR, D, t, PTR, D, t, PTR, PTR, PTR, B, D, D, None)
         assert refuses(rc) and b'24' in so.nof_last_error(), (t, B, D)
+
+
+# A library in front of the runtime's: every launch succeeds but the one whose number the environment gives, and the last error is the last call's.
+FAKE = r"""
+#include <cstdlib>
+static int launches, last;
+extern "C" int hipLaunchKernel(const void*, ...) { const char* f = getenv("FAIL"); return last = launches++ == (f ? atoi(f) : -1) ? 9 : 0; }
+extern "C" int hipGetLastError() { const int e = last; last = 0; return e; }
+extern "C" int __hipPushCallConfiguration(...) { return 0; }
+extern "C" int __hipPopCallConfiguration(...) { return 0; }
+extern "C" int hipFuncSetAttribute(const void*, int, int) { return 0; }
+extern "C" int fake_launches() { return launches; }
+"""
+CALLS = """
+import ctypes as C, sys
+fake = C.CDLL(sys.argv[1], mode=C.RTLD_GLOBAL)
+so = C.CDLL(sys.argv[2])
+p, null, i64, f = C.c_void_p(256), C.c_void_p(None), C.c_int64, C.c_float
+quintic = (f * 15)(*[3.4445, -4.7750, 2.0315] * 5)
+ws = i64(1 << 40)
+call = {
+    'gradient': lambda: so.nof_embed_bwd(p, i64(8), 0, p, 0, f(1.0), p, p, ws, i64(9000), i64(70000), 8, null),
+    'small gradient': lambda: so.nof_embed_bwd(p, i64(8), 0, p, 0, f(1.0), p, p, ws, i64(900), i64(70000), 8, null),
+    'scan': lambda: so.nof_gated_scan_fwd(p, i64(9000), i64(1), 0, p, i64(9000 * 4), i64(4), 0, null, null, 0, p, p, null, p, ws, i64(1), i64(9000), 4, 1, null),
+    'scan back': lambda: so.nof_gated_scan_bwd(p, i64(9000), i64(1), 0, p, i64(9000 * 200), i64(200), 0, p, i64(9000 * 200), i64(200), null, p, null, 0, p, p, p,
+                                               p, ws, i64(1), i64(9000), 200, 1, null),
+    'update': lambda: so.nof_orthogonalize(p, p, 0, 5, quintic, f(1e-30), p, ws, i64(1), i64(200), i64(300), null),
+    'cut update': lambda: so.nof_orthogonalize(p, p, 1, 5, quintic, f(1e-30), p, ws, i64(1), i64(200), i64(2000), null),
+    'thin update': lambda: so.nof_orthogonalize(p, p, 2, 5, quintic, f(1e-30), p, ws, i64(1), i64(90), i64(2000), null),
+}[sys.argv[3]]
+print(call(), fake.fake_launches())
+"""
+
+
+@pytest.mark.parametrize('call,launches', [('gradient', 6), ('small gradient', 3), ('scan', 2), ('scan back', 3), ('update', 17), ('cut update', 22), ('thin update', 7)])
+def test_a_launch_that_fails_is_the_last_and_reported(tmp_path, call, launches):
+    fake = tmp_path / 'libfake.so'
+    (tmp_path / 'fake.cpp').write_text(FAKE)
+    subprocess.run(['g++', '-shared', '-fPIC', '-o', str(fake), str(tmp_path / 'fake.cpp')], check=True)
+    lib.load()
+
+    def run(fail):
+        r = subprocess.run([sys.executable, '-c', CALLS, str(fake), lib.LIB_PATH, call], env={**os.environ, 'FAIL': str(fail)}, capture_output=True, text=True, check=True)
+        return tuple(int(x) for x in r.stdout.split())
+
+    assert run(-1) == (0, launches)
+    for k in range(launches):
+        assert run(k) == (9, k + 1), k
