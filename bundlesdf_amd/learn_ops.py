@@ -245,6 +245,8 @@ def gated_scan_grad(gate, value, dh, dlast=None, state=None, marks=None, lengths
     (value, vst), (gate, gst), (dh, dst) = _scan_strided(value, even), _scan_strided(gate, even and G == D), _scan_strided(dh, even)
     dlast, marks = _flat(dlast, even), _flat(marks, even)
     lengths = lengths.contiguous() if lengths is not None else None
+    if D == 0:                                                            # no channel shares the gates
+        return gate.new_zeros((B, T, G)), value.new_empty((B, T, 0)), value.new_empty((B, 0), dtype=torch.float32)
     dgate, dvalue, dstate = gate.new_empty((B, T, G)), value.new_empty((B, T, D)), value.new_empty((B, D), dtype=torch.float32)
     nbytes = _bytes('nof_gated_scan_workspace_bytes', B, T, D, G, ty)
     ws = _scratch(value, nbytes)

@@ -585,7 +585,7 @@ int nof_gated_scan_fwd(const void* gate, int64_t gate_sb, int64_t gate_st, int32
                        float* last, float* marks, void* workspace, int64_t workspace_bytes, int64_t B, int64_t T, int32_t D,
                        int32_t G, void* stream);
 /* dh [B,T,D] and dlast [B,D] (NULL: zeros) = the loss's gradients of h and last; marks as the forward of the same inputs wrote them ->
- * dgate (gate_type; summed over a shared gate's channels), dvalue (type), dstate [B,D] float32 (may be NULL). */
+ * dgate (gate_type; summed over a shared gate's channels; not written where D = 0), dvalue (type), dstate [B,D] float32 (may be NULL). */
 int nof_gated_scan_bwd(const void* gate, int64_t gate_sb, int64_t gate_st, int32_t gate_type, const void* value, int64_t value_sb,
                        int64_t value_st, int32_t type, const void* dh, int64_t dh_sb, int64_t dh_st, const float* dlast,
                        const float* marks, const int32_t* lengths, int32_t reverse, void* dgate, void* dvalue, float* dstate,

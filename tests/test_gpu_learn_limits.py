@@ -46,3 +46,16 @@ def test_gradient_of_more_than_2_30_positions(nof):
     for k in range(-(-N // V)):
         want += torch.where(k * V + v < N, (k + k * V + v) % 7, 0)
     assert torch.equal(grad[:, 0].long(), want)                       # whole numbers below 2^24: exact in any order
+
+
+@pytest.mark.parametrize('gdtype', [torch.float32, torch.bfloat16])
+def test_gates_of_no_channel_have_no_gradient(nof, gdtype):
+    from bundlesdf_amd import learn_ops as L
+    B, T, G = 3, 700, 100
+    gate, value = torch.ones(B, T, G, dtype=gdtype, device='cuda'), torch.ones(B, T, 0, dtype=torch.bfloat16, device='cuda')
+    h, last, marks = L.gated_scan(gate, value, want_marks=True)
+    assert h.shape == (B, T, 0) and last.shape == (B, 0)
+    poisoned(B, T, G, dtype=gdtype)
+    dgate, dvalue, dstate = L.gated_scan_grad(gate, value, value, marks=marks)
+    assert dgate.shape == gate.shape and dgate.dtype == gdtype and (dgate == 0).all()
+    assert dvalue.shape == value.shape and dstate.shape == (B, 0)
