@@ -8,13 +8,14 @@ a field with learnt codes, blended features and matrix-shaped weights trains wit
 
 Like the rest of the framework they are explicit forward and backward calls, launched on torch's current stream of the tensors'
 device, without a host synchronisation: every one can be captured into a graph.  Tensors are float32, bfloat16 or float16; sums, states
-and norms are float32 or wider and a result is rounded to its type once.  They record no autograd history -- a tensor that would need it
-is refused -- and they raise lib.NofError on anything they do not take; there is no fallback.
+and norms are float32 or wider and a result is rounded to its type once.  They record no autograd history and carry no tangents -- a tensor
+that would need either is refused -- and they raise lib.NofError on anything they do not take; there is no fallback.
 """
 import ctypes as C
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import lib
 from .lib import NofError
@@ -40,6 +41,8 @@ def _on_device(what, *tensors):
         if t.requires_grad and torch.is_grad_enabled():
             raise NofError(f'{what} records no autograd history: call it under torch.no_grad() or with detached tensors, '
                            'and its gradient function for the gradients')
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise NofError(f'{what} carries no forward-mode tangents: call it with the primal tensors')
     return dev
 
 

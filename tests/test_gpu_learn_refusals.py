@@ -1,0 +1,34 @@
+"""Tensors that the learning operators (bundlesdf_amd/learn_ops.py) refuse or read as what they stand for."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+pytestmark = pytest.mark.gpu
+R = dict(device='cuda')
+
+
+def calls(L):
+    """(name, function, its float arguments)"""
+    ids = torch.tensor([2, 0, 2, 5], **R)
+    return [('embed_lookup', lambda t: L.embed_lookup(t, ids), [torch.randn(6, 3, **R)]),
+            ('embed_lookup_grad', lambda d: L.embed_lookup_grad(d, ids, 6), [torch.randn(4, 3, **R)]),
+            ('gated_scan', lambda g, v, s: L.gated_scan(g, v, s), [torch.rand(2, 9, 1, **R), torch.randn(2, 9, 4, **R), torch.randn(2, 4, **R)]),
+            ('gated_scan_grad', lambda g, v, d, dl, s: L.gated_scan_grad(g, v, d, dl, s),
+             [torch.rand(2, 9, 1, **R), torch.randn(2, 9, 4, **R), torch.randn(2, 9, 4, **R), torch.randn(2, 4, **R), torch.randn(2, 4, **R)]),
+            ('gated_scan_step', lambda g, v, s: L.gated_scan_step(g, v, s), [torch.rand(2, 4, **R), torch.randn(2, 4, **R), torch.randn(2, 4, **R)]),
+            ('orthogonalize', lambda u: L.orthogonalize(u), [torch.randn(5, 7, **R)])]
+
+
+def test_tangents_are_refused(nof):
+    from bundlesdf_amd import learn_ops as L
+    for name, f, args in calls(L):
+        want = f(*args)
+        with forward_ad.dual_level():
+            for k in range(len(args)):
+                dual = list(args)
+                dual[k] = forward_ad.make_dual(args[k], torch.ones_like(args[k]))
+                with pytest.raises(nof.NofError, match=f'{name} carries no forward-mode tangents'):
+                    f(*dual)
+            got = f(*args)                                            # without one: as ever
+        for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+            assert torch.equal(a, b)
