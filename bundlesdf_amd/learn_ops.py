@@ -78,6 +78,7 @@ def _apart(a, b):
 
 def _rows(x):
     """x [N, D] with its elements side by side in a row: (tensor, elements between rows)"""
+    x = x.resolve_neg()                                                  # (a view like z.conj().imag holds the other sign)
     if x.shape[1] > 1 and x.stride(1) != 1:
         x = x.contiguous()
     return x, x.stride(0) if x.shape[0] > 1 else x.shape[1]
@@ -146,6 +147,7 @@ def _scan_even(dtype, D, G):
 
 def _scan_strided(x, even):
     """x [B, T, C] (or [B, C]) as the kernels take it -- channels side by side, two-channel loads on their border -- and its strides"""
+    x = x.resolve_neg()
     if x.is_contiguous():
         n = x.shape
         st = (n[1],) if len(n) == 2 else (n[1] * n[2], n[2])
@@ -167,8 +169,7 @@ def _flat(x, even):
     """a [B, D] float32 argument as the kernels take it, or None"""
     if x is None:
         return None
-    if not x.is_contiguous():
-        x = x.contiguous()
+    x = x.resolve_neg().contiguous()
     return x.clone() if even and x.data_ptr() % 8 else x
 
 
@@ -268,8 +269,8 @@ def gated_scan_step(gate, value, state, new_state=None):
     _state_ok('gated_scan_step', 'state', state, B, D)
     _state_ok('gated_scan_step', 'new_state', new_state, B, D)
     dev = _on_device('gated_scan_step', gate, value, state, new_state)
-    if not (new_state is None or new_state.is_contiguous()):
-        raise NofError('gated_scan_step: new_state must be contiguous')
+    if not (new_state is None or (new_state.is_contiguous() and not new_state.is_neg())):
+        raise NofError('gated_scan_step: new_state must be contiguous and no negated view')
     dt = value.dtype
     even = _scan_even(dt, D, G)
     (value, vst), (gate, gst), state = _scan_strided(value, even), _scan_strided(gate, even and G == D), _flat(state, even)
@@ -315,10 +316,10 @@ def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-30, out=None):
     if not (batch < 65536):
         raise NofError('orthogonalize: at most 65535 matrices')
     coef = _coefficients(int(steps), tuple(tuple(c) if isinstance(c, (tuple, list)) else c for c in coefficients))
-    if not (out is None or (out.shape == update.shape and out.dtype == update.dtype and out.is_contiguous())):
-        raise NofError("orthogonalize: out must be contiguous, of update's shape and type")
+    if not (out is None or (out.shape == update.shape and out.dtype == update.dtype and out.is_contiguous() and not out.is_neg())):
+        raise NofError("orthogonalize: out must be contiguous, of update's shape and type and no negated view")
     dev = _on_device('orthogonalize', update, out)
-    update = update.contiguous()
+    update = update.resolve_neg().contiguous()
     if out is None:
         out = update.new_empty(update.shape)
     elif not _apart(out, update):

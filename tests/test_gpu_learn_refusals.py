@@ -32,3 +32,37 @@ def test_tangents_are_refused(nof):
             got = f(*args)                                            # without one: as ever
         for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
             assert torch.equal(a, b)
+
+
+def negated(x, **k):
+    """x as a view of memory that holds -x"""
+    y = torch.complex(torch.zeros_like(x), -x).conj().imag
+    assert y.is_neg() and torch.equal(y, x)
+    return y
+
+
+@pytest.mark.parametrize('as_view', [negated, lambda x: torch._neg_view(-x)], ids=['conj', 'neg_view'])
+def test_negated_views_are_read_as_what_they_stand_for(nof, as_view):
+    """one channel, one element, one row: where nothing else makes a copy of them"""
+    from bundlesdf_amd import learn_ops as L
+    ids = torch.tensor([1, 0, 1], **R)
+    more = calls(L) + [('lookup', lambda t: L.embed_lookup(t, ids), [torch.randn(2, 1, **R)]), ('grad', lambda d: L.embed_lookup_grad(d, ids, 2), [torch.randn(3, 1, **R)]),
+                       ('scan', lambda g, v, s: L.gated_scan(g, v, s), [torch.rand(2, 9, 1, **R), torch.randn(2, 9, 1, **R), torch.randn(2, 1, **R)]),
+                       ('scan grad', lambda g, v, d, dl, s: L.gated_scan_grad(g, v, d, dl, s),
+                        [torch.rand(2, 9, 1, **R), torch.randn(2, 9, 1, **R), torch.randn(2, 9, 1, **R), torch.randn(2, 1, **R), torch.randn(2, 1, **R)]),
+                       ('step', lambda g, v, s: L.gated_scan_step(g, v, s), [torch.rand(2, 1, **R), torch.randn(2, 1, **R), torch.randn(2, 1, **R)]),
+                       ('update', lambda u: L.orthogonalize(u), [torch.randn(1, 1, **R)])]
+    for name, f, args in more:
+        want = f(*args)
+        for k in range(len(args)):
+            view = list(args)
+            view[k] = as_view(args[k])
+            assert view[k].is_neg() and torch.equal(view[k], args[k])
+            got = f(*view)
+            for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+                assert torch.equal(a, b), (name, k)
+    u, s = torch.randn(4, 4, **R), torch.randn(2, 4, **R)
+    with pytest.raises(nof.NofError, match='negated'):
+        L.orthogonalize(u, out=torch._neg_view(u.clone()))
+    with pytest.raises(nof.NofError, match='negated'):
+        L.gated_scan_step(torch.rand(2, 4, **R), torch.randn(2, 4, **R), s, torch._neg_view(s.clone()))
