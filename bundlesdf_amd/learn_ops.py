@@ -76,6 +76,16 @@ def _apart(a, b):
     return x + n <= y or y + m <= x or (x == y and n == m) or n == 0 or m == 0
 
 
+def _clear_of(a, x, strides):
+    """whether what is written to the contiguous `a` cannot be read from x by another lane: x lies apart, or each element of it is a's own"""
+    if x.dtype == a.dtype and x.data_ptr() == a.data_ptr() and x.shape == a.shape and x.is_contiguous():
+        return True
+    size = x.element_size()
+    last = sum([(n - 1) * st for n, st in zip(x.shape, strides)]) + x.shape[-1]                 # (`strides`: all but the last, whose step is 1)
+    lo, at = a.data_ptr(), x.data_ptr()
+    return lo + a.numel() * a.element_size() <= at or at + last * size <= lo or a.numel() == 0 or x.numel() == 0
+
+
 def _rows(x):
     """x [N, D] with its elements side by side in a row: (tensor, elements between rows)"""
     x = x.resolve_neg()                                                  # (a view like z.conj().imag holds the other sign)
@@ -261,7 +271,7 @@ def gated_scan_grad(gate, value, dh, dlast=None, state=None, marks=None, lengths
 
 def gated_scan_step(gate, value, state, new_state=None):
     """One position of gated_scan: gate [B, G], value [B, D], state [B, D] float32 -> (h [B, D] in value's type, the new state).
-    new_state: where the new state goes (`state` itself for an update in place); None allocates it."""
+    new_state: where the new state goes (`state` itself for an update in place, apart from gate and value); None allocates it."""
     D, G = _scan_args('gated_scan_step', gate, value, None, 2)
     B = value.shape[0]
     if not (state is not None):
@@ -281,6 +291,8 @@ def gated_scan_step(gate, value, state, new_state=None):
             raise NofError('gated_scan_step: new_state must start on an 8-byte border')
         if not _apart(new_state, state):
             raise NofError('gated_scan_step: new_state must be state itself or lie apart from it')
+        if not (_clear_of(new_state, value, vst) and _clear_of(new_state, gate, gst)):
+            raise NofError('gated_scan_step: new_state must lie apart from gate and value')
     h = value.new_empty((B, D))
     _call(dev, 'nof_gated_scan_step', gate.data_ptr(), *gst, _TYPE[gate.dtype], value.data_ptr(), *vst, _TYPE[dt], state.data_ptr(),
           new_state.data_ptr(), h.data_ptr(), B, D, G)

@@ -66,3 +66,28 @@ def test_negated_views_are_read_as_what_they_stand_for(nof, as_view):
         L.orthogonalize(u, out=torch._neg_view(u.clone()))
     with pytest.raises(nof.NofError, match='negated'):
         L.gated_scan_step(torch.rand(2, 4, **R), torch.randn(2, 4, **R), s, torch._neg_view(s.clone()))
+
+
+def test_a_new_state_that_another_lane_reads_is_refused(nof):
+    from bundlesdf_amd import learn_ops as L
+    line, state = torch.zeros(400, **R), torch.randn(4, 8, **R)
+    gate, value = torch.rand(4, 8, **R), torch.randn(4, 8, **R)
+    for shift in (1, 8, 31):
+        at = line[shift:shift + 32].view(4, 8)
+        with pytest.raises(nof.NofError, match='apart from gate and value'):
+            L.gated_scan_step(gate, line[:32].view(4, 8), state, at)
+        with pytest.raises(nof.NofError, match='apart from gate and value'):
+            L.gated_scan_step(line[:32].view(4, 8), value, state, at)
+        with pytest.raises(nof.NofError, match='apart from gate and value'):
+            L.gated_scan_step(line[:4].view(4, 1) if shift < 4 else line[shift + 3:shift + 7].view(4, 1), value, state, at)
+    with pytest.raises(nof.NofError, match='apart from gate and value'):                  # rows of a wider tensor
+        L.gated_scan_step(gate, line[:400].view(4, 100)[:, 90:98], state, line[100:132].view(4, 8))
+    with pytest.raises(nof.NofError, match='apart from gate and value'):                  # of another type
+        L.gated_scan_step(gate, line[:16].view(torch.bfloat16).view(4, 8), state, line[:32].view(4, 8))
+    want = L.gated_scan_step(gate, value, state)
+    for which in (0, 1):                                                                  # in the very place of one of them: each lane its own element
+        g, v = gate.clone(), value.clone()
+        h, new = L.gated_scan_step(g, v, state, (g, v)[which])
+        assert new.data_ptr() == (g, v)[which].data_ptr() and torch.equal(new, want[1]) and torch.equal(h, want[0])
+    h, new = L.gated_scan_step(gate, line[:32].view(4, 8).copy_(value), state, line[32:64].view(4, 8))       # side by side
+    assert torch.equal(new, want[1]) and torch.equal(h, want[0])
