@@ -305,9 +305,9 @@ QUINTIC = (3.4445, -4.7750, 2.0315)     # steep at 0 (a small singular value gro
 
 @functools.lru_cache(maxsize=64)
 def _coefficients(steps, coefficients):
-    flat = coefficients if isinstance(coefficients[0], (tuple, list)) else (coefficients,) * steps
     if not (1 <= steps <= 32):
         raise NofError('orthogonalize: steps must be in [1, 32]')
+    flat = coefficients if len(coefficients) > 0 and isinstance(coefficients[0], (tuple, list)) else (coefficients,) * steps
     if not (len(flat) == steps and all(len(c) == 3 for c in flat)):
         raise NofError('orthogonalize: coefficients must be (a, b, c) or one such triple per step')
     return (C.c_float * (3 * steps))(*[float(x) for c in flat for x in c])

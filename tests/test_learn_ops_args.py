@@ -1,7 +1,9 @@
 """Checks of the learning operators' arguments (bundlesdf_amd/learn_ops.py) that need no GPU."""
+import pytest
 import torch
 
 from bundlesdf_amd import learn_ops as L
+from bundlesdf_amd import lib
 
 
 def test_what_a_new_state_overlaps():
@@ -18,3 +20,11 @@ def test_what_a_new_state_overlaps():
     assert clear(line[34:35].view(1, 1)) and clear(line[9:10].view(1, 1))
     assert not clear(line.view(4, 25)[:, :2]) and not clear(line[8:9].view(1, 1).expand(4, 1).as_strided((4, 1), (1, 1)))
     assert clear(line[8:9].view(1, 1).expand(4, 6)[:, :1])                                # one element for every row
+
+
+def test_steps_are_judged_before_anything_is_made_of_them():
+    for steps in (0, -1, 33, 10 ** 12):
+        with pytest.raises(lib.NofError, match='steps'):
+            L.orthogonalize(torch.zeros(4, 6), steps=steps)
+    with pytest.raises(lib.NofError, match='triple'):
+        L.orthogonalize(torch.zeros(4, 6), coefficients=())
