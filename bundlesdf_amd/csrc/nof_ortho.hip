@@ -129,9 +129,9 @@ __device__ __forceinline__ void ort_mma6(const _Float16* L, const _Float16* R, i
 // times as long.
 struct OrtCoef { float c[3 * ORT_MAX_STEPS]; };
 
-// RT: rows of tiles at most
+// RT: rows of tiles at most; `out` may be `g`
 template <typename T, int KT, int RT>
-__global__ __launch_bounds__(64 * KT * RT) void k_ortho_small(const T* __restrict__ g, T* __restrict__ out, int m, int n, int steps, OrtCoef coef, float eps) {
+__global__ __launch_bounds__(64 * KT * RT) void k_ortho_small(const T* g, T* out, int m, int n, int steps, OrtCoef coef, float eps) {
   extern __shared__ __attribute__((aligned(16))) char ort_lds[];
   constexpr int square = ort_square(RT);
   __shared__ double red[16], a64[square == ORT_WIDE ? 32 * ORT_WIDE_ROW : 1];
@@ -290,7 +290,7 @@ __device__ __forceinline__ void ort_tile_product(const _Float16* L, int dl, cons
 }
 
 template <typename T, int RT, int MODE>
-__global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* __restrict__ g, T* __restrict__ out, OrtThin p) {
+__global__ __launch_bounds__(256 * RT) void k_ortho_thin(const T* g, T* out, OrtThin p) {
   extern __shared__ __attribute__((aligned(16))) char ort_lds[];
   constexpr int square = ort_square(RT);
   __shared__ double red[4 * RT], a64[square == ORT_WIDE ? 32 * ORT_WIDE_ROW : 1];

@@ -485,10 +485,10 @@ __global__ __launch_bounds__(256) void k_scan_gate_sum(const float* __restrict__
   }
 }
 
+// (new_state may be what a lane has read: its own elements of state, or of a float32 gate or value)
 template <typename TG, typename T, int V>
-__global__ __launch_bounds__(256) void k_scan_step(const TG* __restrict__ gate, int64_t gate_st, const T* __restrict__ value, int64_t value_st,
-                                                   const float* __restrict__ state, float* __restrict__ new_state, T* __restrict__ h, int B,
-                                                   int D, int G, int blocks_per_row) {
+__global__ __launch_bounds__(256) void k_scan_step(const TG* gate, int64_t gate_st, const T* value, int64_t value_st, const float* state,
+                                                   float* new_state, T* __restrict__ h, int B, int D, int G, int blocks_per_row) {
   const int b = blockIdx.x / blocks_per_row, ch = ((blockIdx.x % blocks_per_row) * 256 + threadIdx.x) * V;
   if (ch >= D) return;
   float a[V], x[V], s[V];

@@ -590,7 +590,7 @@ int nof_gated_scan_bwd(const void* gate, int64_t gate_sb, int64_t gate_st, int32
                        int64_t value_st, int32_t type, const void* dh, int64_t dh_sb, int64_t dh_st, const float* dlast,
                        const float* marks, const int32_t* lengths, int32_t reverse, void* dgate, void* dvalue, float* dstate,
                        void* workspace, int64_t workspace_bytes, int64_t B, int64_t T, int32_t D, int32_t G, void* stream);
-/* one position: gate [B,G], value [B,D], state [B,D] -> new_state [B,D] (may be `state`), h [B,D] = new_state in `type`.  B times D up to a
+/* one position: gate [B,G], value [B,D], state [B,D] -> new_state [B,D] (may be `state`, but overlap nothing else), h [B,D] = new_state in `type`.  B times D up to a
  * multiple of 256: below 2^32. */
 int nof_gated_scan_step(const void* gate, int64_t gate_sb, int32_t gate_type, const void* value, int64_t value_sb, int32_t type,
                         const float* state, float* new_state, void* h, int64_t B, int32_t D, int32_t G, void* stream);
