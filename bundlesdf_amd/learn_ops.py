@@ -214,7 +214,8 @@ def gated_scan(gate, value, state=None, lengths=None, reverse=False, want_marks=
     gate [B, T, G] (value's type or float32), value [B, T, D]; G divides D: channel d uses gate d // (D // G) -- G = D is a gate per
     channel, G = 1 one for all.  lengths [B] int32: rows from lengths[b] on do not exist (not read; zeros in h).  reverse: from the last
     existing row to the first -- with gate = 1 - opacity and value = opacity * feature, h[:, 0] is the ray's blend, back to front.
-    Gates compose over positions in float32: their products must stay in its range (|gate| <= 1 always does)."""
+    Gates compose over positions in float32: their products must stay in its range (|gate| <= 1 always does).  Behind an infinity a channel
+    is infinite or NaN (a product of gates that has become zero meets it)."""
     D, G = _scan_args('gated_scan', gate, value, lengths, 3)
     B, T = value.shape[:2]
     _state_ok('gated_scan', 'state', state, B, D)

@@ -574,7 +574,8 @@ int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type, const voi
  * *_st: elements between batches / positions (channels are side by side); h, dgate, dvalue are contiguous.  state, last [B,D] float32
  * (state NULL: zeros; last, h and marks may be NULL).  lengths [B] int32 or NULL: only the first lengths[b] rows (clamped to [0, T]) exist;
  * the others are not read, their rows of h, dgate, dvalue are zeros.  reverse = 1: the recurrence runs from row lengths[b] - 1 down to 0.
- * Positions compose in parallel, so products of gates over a run of positions must stay within binary32 (|gate| <= 1 always does).
+ * Positions compose in parallel, so products of gates over a run of positions must stay within binary32 (|gate| <= 1 always does); behind an
+ * infinity a channel is infinite or NaN (where such a product has become zero).
  * 16-bit types with an even number of channels per group: pointers and strides (a shared gate's aside) are multiples of two elements.
  * B < 2^24, T < 2^31, D <= 2^20.  A launch holds less than 2^32 threads: B D < 2^24 always fits (and far more where rows are wide), what does
  * not is refused; the workspace query answers for the forward where only the backward does not. */
@@ -590,8 +591,8 @@ int nof_gated_scan_bwd(const void* gate, int64_t gate_sb, int64_t gate_st, int32
                        int64_t value_st, int32_t type, const void* dh, int64_t dh_sb, int64_t dh_st, const float* dlast,
                        const float* marks, const int32_t* lengths, int32_t reverse, void* dgate, void* dvalue, float* dstate,
                        void* workspace, int64_t workspace_bytes, int64_t B, int64_t T, int32_t D, int32_t G, void* stream);
-/* one position: gate [B,G], value [B,D], state [B,D] -> new_state [B,D] (may be `state`, but overlap nothing else), h [B,D] = new_state in `type`.  B times D up to a
- * multiple of 256: below 2^32. */
+/* one position: gate [B,G], value [B,D], state [B,D] -> new_state [B,D] (may be `state`, but overlap nothing else), h [B,D] = new_state in
+ * `type`.  B times D up to a multiple of 256: below 2^32. */
 int nof_gated_scan_step(const void* gate, int64_t gate_sb, int32_t gate_type, const void* value, int64_t value_sb, int32_t type,
                         const float* state, float* new_state, void* h, int64_t B, int32_t D, int32_t G, void* stream);
 /* The orthogonalised update of `batch` weight matrices [m,n]: X = update / max(|update|_F, eps) (a zero matrix: zeros), then for each of

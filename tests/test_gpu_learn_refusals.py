@@ -91,3 +91,15 @@ def test_a_new_state_that_another_lane_reads_is_refused(nof):
         assert new.data_ptr() == (g, v)[which].data_ptr() and torch.equal(new, want[1]) and torch.equal(h, want[0])
     h, new = L.gated_scan_step(gate, line[:32].view(4, 8).copy_(value), state, line[32:64].view(4, 8))       # side by side
     assert torch.equal(new, want[1]) and torch.equal(h, want[0])
+
+
+def test_behind_an_infinity_its_channel_is_not_finite(nof):
+    from bundlesdf_amd import learn_ops as L
+    gate, value, state = torch.full((2, 4000, 1), 0.5, **R), torch.randn(2, 4000, 3, **R), torch.zeros(2, 3, **R)
+    want, last = L.gated_scan(gate, value, state)
+    for at, sign in ((0, 1.0), (17, -1.0), (1500, -1.0)):
+        bad = value.clone()
+        bad[1, at, 2] = sign * float('inf')
+        h, end = L.gated_scan(gate, bad, state)
+        assert not h[1, at:, 2].isfinite().any() and not end[1, 2].isfinite() and h[1, at, 2] == sign * float('inf')
+        assert torch.equal(h[0], want[0]) and torch.equal(h[1, :, :2], want[1, :, :2]) and torch.equal(h[1, :at], want[1, :at])
