@@ -57,11 +57,10 @@ __device__ __forceinline__ double ort_factor(double sumsq, float eps) {
 }
 
 // Few rows leave little to average: an error of A A is one of all of X, and up to four steps amplify it.  So in matrices of at most 64 rows
-// the sums of the large parts and of what the small ones add are kept apart (the many small terms then cost the large sum no rounding), and
 // A A is more exact than pairs would give it: of 33 to 64 rows as products of three fp16 parts (33 bits), of at most 32 on the binary64 matrix
-// cores.  Relative error against 64 bits, 24 random matrices each: 9 x 287 2.8e-7 (as pairs 8.5e-7, a binary32 computation 5.9e-7), 32 x 500
-// 6e-7 (2.2e-6, 2.7e-6), 33 x 128 1.3e-6 (2.0e-6, 1.4e-6), 64 x 500 1.2e-6 (1.8e-6, 1.6e-6); from 65 rows on pairs are no worse than
-// binary32 (128 x 1000: 7e-7 and 1.7e-6).  64 x 64 on the binary64 cores: 33 us, as three parts 20, as pairs 18.
+// cores.  Relative error against 64 bits, 24 random matrices each: 9 x 287 2.7e-7 (as pairs 8.0e-7, a binary32 computation 6.0e-7), 32 x 500
+// 7.9e-7 (2.2e-6, 2.7e-6), 33 x 128 1.3e-6 (1.8e-6, 1.3e-6), 64 x 500 1.2e-6 (1.7e-6, 1.6e-6); from 65 rows on pairs are no worse than
+// binary32 (128 x 1000: 5.7e-7 and 1.7e-6).  64 x 64 as three parts 21.7 us, as pairs 19.8; 16 x 16 on the binary64 cores 13.1, as pairs 14.4.
 enum { ORT_PAIRS, ORT_THREE, ORT_WIDE };
 __host__ __device__ constexpr int ort_square(int rt) { return rt == 1 ? ORT_WIDE : rt == 2 ? ORT_THREE : ORT_PAIRS; }
 __host__ __device__ constexpr int ort_parts(int rt) { return ort_square(rt) == ORT_THREE ? 3 : 2; }        // planes of A's image
@@ -124,8 +123,8 @@ __device__ __forceinline__ void ort_mma6(const _Float16* L, const _Float16* R, i
 // One wave per 32 x 32 tile of X (r <= k after the turn; tiles rt x KT).  LDS: images of hi and lo, rows of 32 KT + 8 halves (the pad
 // spreads a column's 16-byte reads over all banks; known at compile time, or sixteen row offsets per store stay live and spill).  The first
 // pair holds X for the Gram product and X^T for the last one, the second A, then P: symmetric, so their tiles are stored turned, four
-// halves at a time.  Bound by the chain of products, barriers and LDS round trips: 1.7 us a step for 16 x 16, 3.2 for 64 x 64,
-// 8 for 128 x 128 (half of it the matrix cores); four waves of 2 x 2 tiles instead of sixteen of one read half as much LDS and take 1.4
+// halves at a time.  Bound by the chain of products, barriers and LDS round trips: 1.8 us a step for 16 x 16, 3.4 for 64 x 64,
+// 8.2 for 128 x 128 (half of it the matrix cores); four waves of 2 x 2 tiles instead of sixteen of one read half as much LDS and take 1.4
 // times as long.
 struct OrtCoef { float c[3 * ORT_MAX_STEPS]; };
 
@@ -258,8 +257,8 @@ __global__ __launch_bounds__(64 * KT * RT) void k_ortho_small(const T* g, T* out
 // At most 128 on the shorter side, more on the longer: a launch a step instead of three.  A workgroup owns a stretch of X's columns, 128 at a
 // time through LDS, and knows the Gram matrix as the sum of all workgroups' parts of it, which the launch before left behind: it forms A and
 // P for itself, then X <- P X of its columns and the new part.  X stays in memory as the accumulators hold it.  Parts are added in the order
-// of the workgroups.  64 x 1000 fp32: 50 us (109 as tiles of the larger matrices, whose Gram product is one tile's chain over the long side),
-// 64 x 16384: 119 us (599), 128 x 4096: 141 us (222).
+// of the workgroups.  64 x 1000 fp32: 52 us (as tiles of the larger matrices, whose Gram product is one tile's chain over the long side, twice that),
+// 64 x 16384: 122 us (five times), 128 x 4096: 145 us (1.6 times).
 struct OrtThin {
   const double* part; int n_part;
   float* x; const float* gram_in; float* gram_out;
@@ -866,9 +865,9 @@ typedef OrtShape<2, 2, 1, 1, 2, 2> OrtNarrow;
 typedef OrtShape<2, 2, 1, 1, 2, 4> OrtNarrowDeep;
 typedef OrtShape<2, 2, 1, 1, 2, 1> OrtSingle;                          // the join's
 // The Gram product of few tiles over a long axis is cut along it: at most two workgroups a compute unit, and eight stages a part at least.
-// Five steps of 200 x 4096: 255 us uncut, 153 cut; 600 x 2900: 282 and 241; 333 x 1001, 3 of them: 174 and 170.  Below 1024 the join costs
-// more than the parts save (512 x 512: 146 and 154), and so it does with many tiles of a middling length (1024 x 1024: 209 and 221;
-// 1024 x 2048: 285 either way; 1024 x 4096: 435 and 424).  Parts of four stages gain nothing (200 x 4096: 171).
+// Five steps of 200 x 4096: 251 us uncut, 147 cut; 600 x 2900: 273 and 221; 333 x 1001, 3 of them: 170 and 166.  Below 1024 the join costs
+// more than the parts save (512 x 512: 142 and 149), and so it does with many tiles of a middling length (1024 x 1024: 210 and 219;
+// 1024 x 2048: 288 and 284; 1024 x 4096: 415 and 389).  Parts of four stages gained nothing (200 x 4096: 153 and 171).
 static int ort_cuts(int64_t batch, int64_t rp, int64_t kp) {
   const int64_t n = rp / 64, tiles = batch * n * (n + 1) / 2, most = kp / 256, want = 512 / tiles;
   if (kp < 1024 || want < 2 || kp * want < 6144) return 1;

@@ -7,8 +7,8 @@
 // Bound by memory: the forward reads a, x and writes h once, the backward reads a, x, dh and writes da, dx.  Composition of two steps
 // (a, b) then (a', b') is (a a', a' b + b'), so time is cut: a workgroup of up to four waves takes a CHUNK of positions at a time, each of its
 // slots SCAN_U consecutive positions of one lane's channels in registers (as loaded; converted where used); slots compose their (a, b) by
-// shuffles within a wave and through LDS between waves -- one barrier a chunk --, the state between chunks stays in registers.  Four such
-// workgroups a compute unit hide each other's loads.  Where batch x channels give too few workgroups, time is also cut into segments: a first
+// shuffles within a wave and through LDS between waves -- one barrier a chunk --, the state between chunks stays in registers.  Three such
+// workgroups a compute unit (two in the backward of a shared gate's pairs) hide each other's loads.  Where batch x channels give too few workgroups, time is also cut into segments: a first
 // launch composes each segment (its slots walk their share without a barrier), and every workgroup of the second folds the segments before
 // its own.
 //
@@ -509,8 +509,8 @@ __global__ __launch_bounds__(256) void k_scan_step(const TG* gate, int64_t gate_
 // ---- host -------------------------------------------------------------------------------------------------------------------------
 // Everything here depends on the sizes alone, so that the forward's marks fit the backward.
 // Segments: from one wave per SIMD (1024 waves) on, a workgroup's own look-ahead keeps the memory busy and a second pass over the inputs
-// would cost more than it gives; below, two waves per SIMD, of two chunks at least.  4 x 16384 x 1024 bf16, forward + backward: 111 + 177 us
-// so, 123 + 192 with four waves per SIMD, 154 + 209 with one.
+// would cost more than it gives; below, two waves per SIMD, of two chunks at least.  4 x 16384 x 1024 bf16, forward + backward: 118 + 177 us
+// so, 128 + 198 with four waves per SIMD, 159 + 209 with one.
 // Tiles narrower than a wave where that leaves a fifth fewer lanes without a channel: 65 channels a group (24 x 1777 x 520, eight gates)
 // backward 84 us, 115 as 64 + 1.
 static void scan_layout(ScanArgs& p, int span, int v) {
