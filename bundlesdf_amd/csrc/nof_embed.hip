@@ -570,7 +570,7 @@ static bool emb_sizes_ok(int64_t N, int64_t V, int32_t D) {
 
 template <typename T>
 static void emb_launch_fwd(const void* table, int64_t stride, const void* ids, int ids64, float scale, void* out, int64_t N, int64_t rows,
-                           int32_t D, hipStream_t st) {
+                           int32_t D, LearnStream& st) {
   const int64_t nv = nof_div_up(D, EmbVec<T>::V);
   const int ls = learn_log2_up(nv < EMB_T ? nv : EMB_T);
   const int64_t want = nof_div_up(N, EMB_T >> ls), most = (int64_t)1 << 20;
@@ -580,7 +580,7 @@ static void emb_launch_fwd(const void* table, int64_t stride, const void* ids, i
 
 template <typename T>
 static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* key, const uint32_t* pos, float scale, void* grad, float* part,
-                            const EmbPlan& p, int32_t D, hipStream_t st) {
+                            const EmbPlan& p, int32_t D, LearnStream& st) {
   const unsigned cols = (unsigned)nof_div_up(nof_div_up(D, EmbVec<T>::V), (int64_t)1 << p.ls);
   const int64_t zeros = nof_div_up(p.s.rows - p.zeroed, EMB_ZROWS);
   const unsigned n_zero = (unsigned)(zeros < EMB_MAX_GRID ? zeros : EMB_MAX_GRID);
@@ -599,7 +599,7 @@ static void emb_launch_sums(const void* dout, int64_t stride, const uint32_t* ke
 
 // at most eight lanes a row, so that a frequent id is many groups' work
 template <typename T>
-static void emb_launch_few(const void* dout, int64_t stride, const void* ids, int ids64, float scale, void* grad, const EmbPlan& p, int32_t D, hipStream_t st) {
+static void emb_launch_few(const void* dout, int64_t stride, const void* ids, int ids64, float scale, void* grad, const EmbPlan& p, int32_t D, LearnStream& st) {
   const int64_t nv = nof_div_up(D, EmbVec<T>::V);
   const int ls = learn_log2_up(nv < 8 ? nv : 8);
   LEARN_LAUNCH(k_embed_few<T>, dim3((unsigned)p.s.rows, (unsigned)nof_div_up(nv, (int64_t)1 << ls)), dim3(EMB_T), 0, st, (const T*)dout, stride, ids,
@@ -612,12 +612,11 @@ extern "C" int nof_embed_fwd(const void* table, int64_t table_stride, int32_t ty
   NOF_ARG(emb_sizes_ok(N, V, D) && table_stride >= 0);
   if (N == 0 || D == 0) return 0;
   NOF_ARG(ids && out && (table || V == 0));
-  hipStream_t st = (hipStream_t)stream;
-  LEARN_BEGIN();
+  LearnStream st = {(hipStream_t)stream, hipSuccess};
   if (type == NOF_TYPE_F32) emb_launch_fwd<float>(table, table_stride, ids, ids64, scale, out, N, V, D, st);
   else if (type == NOF_TYPE_BF16) emb_launch_fwd<__bf16>(table, table_stride, ids, ids64, scale, out, N, V, D, st);
   else emb_launch_fwd<_Float16>(table, table_stride, ids, ids64, scale, out, N, V, D, st);
-  LEARN_END();
+  LEARN_END(st);
   return 0;
 }
 
@@ -638,13 +637,12 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
   NOF_ARG(emb_launches(p));
   NOF_ARG(N == 0 || workspace_bytes >= p.bytes);
   NOF_ARG(N == 0 || ((uintptr_t)workspace & 255) == 0);
-  hipStream_t st = (hipStream_t)stream;
-  LEARN_BEGIN();
+  LearnStream st = {(hipStream_t)stream, hipSuccess};
   if (p.few) {
     if (type == NOF_TYPE_F32) emb_launch_few<float>(dout, dout_stride, ids, ids64, scale, grad_table, p, D, st);
     else if (type == NOF_TYPE_BF16) emb_launch_few<__bf16>(dout, dout_stride, ids, ids64, scale, grad_table, p, D, st);
     else emb_launch_few<_Float16>(dout, dout_stride, ids, ids64, scale, grad_table, p, D, st);
-    LEARN_END();
+    LEARN_END(st);
     return 0;
   }
   char* ws = (char*)workspace;
@@ -680,11 +678,11 @@ extern "C" int nof_embed_bwd(const void* dout, int64_t dout_stride, int32_t type
                            (const uint32_t*)pos[cur], key[cur ^ 1], pos[cur ^ 1], (const uint32_t*)hist, z);
       }
     }
-    LEARN_END();
+    LEARN_END(st);
   }
   if (type == NOF_TYPE_F32) emb_launch_sums<float>(dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
   else if (type == NOF_TYPE_BF16) emb_launch_sums<__bf16>(dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
   else emb_launch_sums<_Float16>(dout, dout_stride, key[cur], pos[cur], scale, grad_table, part, p, D, st);
-  LEARN_END();
+  LEARN_END(st);
   return 0;
 }

@@ -26,11 +26,13 @@ static inline bool learn_type_ok(int32_t t) { return t == NOF_TYPE_F32 || t == N
 static inline int learn_log2_up(int64_t n) { int b = 0; while (((int64_t)1 << b) < n) ++b; return b; }
 static inline int64_t learn_align(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
 
-// A call of several launches ends with the first that fails, and says so: the runtime's last error is the last launch's, one that succeeds clears
-// it, and what later launches read would not be there.  LEARN_BEGIN, LEARN_LAUNCH for each, LEARN_END before the return.
-static thread_local hipError_t learn_status;
-#define LEARN_BEGIN() (learn_status = hipSuccess)
-#define LEARN_LAUNCH(...)                                                                   \
-  do { if (learn_status == hipSuccess) { hipLaunchKernelGGL(__VA_ARGS__); learn_status = hipGetLastError(); } } while (0)
-#define LEARN_END()                                                                         \
-  do { if (learn_status != hipSuccess) return nof_set_error((int)learn_status, "%s: %s", __func__, hipGetErrorString(learn_status)); } while (0)
+// A call's stream and the status of its launches.  A call of several ends with the first that fails, and says so: the runtime's last error is the
+// last launch's, one that succeeds clears it, and what later launches read would not be there.
+struct LearnStream { hipStream_t stream; hipError_t status; };
+#define LEARN_LAUNCH(kernel, grid, block, lds, st, ...)                                     \
+  do { if ((st).status == hipSuccess) {                                                     \
+         hipLaunchKernelGGL(kernel, grid, block, lds, (st).stream, __VA_ARGS__);            \
+         (st).status = hipGetLastError();                                                   \
+       } } while (0)
+#define LEARN_END(st)                                                                       \
+  do { if ((st).status != hipSuccess) return nof_set_error((int)(st).status, "%s: %s", __func__, hipGetErrorString((st).status)); } while (0)

@@ -900,7 +900,7 @@ extern "C" int64_t nof_orthogonalize_workspace_bytes(int64_t batch, int64_t m, i
 }
 
 template <typename T, int KT, int RT>
-static void ort_launch_small(const void* g, void* out, int64_t batch, int64_t m, int64_t n, int32_t steps, const float* coef, float eps, hipStream_t st) {
+static void ort_launch_small(const void* g, void* out, int64_t batch, int64_t m, int64_t n, int32_t steps, const float* coef, float eps, LearnStream& st) {
   OrtCoef c = {};
   for (int i = 0; i < 3 * steps; ++i) c.c[i] = coef[i];
   const int rt = (int)nof_div_up(m < n ? m : n, 32);
@@ -914,13 +914,13 @@ template <int MODE, typename S> static int64_t ort_tiles(const OrtArgs& p) {
   return MODE == ORT_GRAM || MODE == ORT_POLY || MODE == ORT_JOIN ? ni * (ni + 1) / 2 : ni * nj;
 }
 template <int MODE, typename T, typename S>
-static void ort_gemm(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
+static void ort_gemm(OrtArgs& p, T* out, int64_t batch, LearnStream& st) {
   p.tiles = (int)ort_tiles<MODE, S>(p);
   const int64_t parts = MODE == ORT_GRAM ? p.split : 1;
   LEARN_LAUNCH((k_ortho_gemm<MODE, T, S>), dim3((unsigned)(p.tiles * batch * parts)), dim3(S::threads), 0, st, p, out);
 }
 template <int MODE, typename T>
-static void ort_product(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
+static void ort_product(OrtArgs& p, T* out, int64_t batch, LearnStream& st) {
   const int64_t wide = p.rp % 128 == 0 && p.kp % 128 == 0 ? batch * ort_tiles<MODE, OrtWide>(p) : 0;
   if constexpr (MODE == ORT_GRAM) {
     if (p.split > 1) {
@@ -937,7 +937,7 @@ static void ort_product(OrtArgs& p, T* out, int64_t batch, hipStream_t st) {
 
 // the sums of squares, as many as it says
 template <typename T>
-static int ort_launch_norm(const void* g, double* part, int64_t batch, int64_t m, int64_t n, hipStream_t st) {
+static int ort_launch_norm(const void* g, double* part, int64_t batch, int64_t m, int64_t n, LearnStream& st) {
   constexpr int V = 16 / (int)sizeof(T);
   const bool wide = ((uintptr_t)g & 15) == 0 && m * n % V == 0;
   const int64_t want = nof_div_up(m * n, 256 * 8 * (wide ? 4 : 1));
@@ -948,7 +948,7 @@ static int ort_launch_norm(const void* g, double* part, int64_t batch, int64_t m
 }
 
 template <typename T, int RT, int MODE>
-static void ort_thin_step(const void* g, void* out, const OrtThin& p, int64_t batch, hipStream_t st) {
+static void ort_thin_step(const void* g, void* out, const OrtThin& p, int64_t batch, LearnStream& st) {
   constexpr int px = 128 * (32 * RT + 8) > 32 * RT * 136 ? 128 * (32 * RT + 8) : 32 * RT * 136;
   constexpr size_t lds = 2 * (size_t)(2 * px + ort_parts(RT) * 32 * RT * (32 * RT + 8));                              // 136 KiB for RT = 4
   if (lds > 64 << 10) (void)hipFuncSetAttribute((const void*)&k_ortho_thin<T, RT, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -956,7 +956,7 @@ static void ort_thin_step(const void* g, void* out, const OrtThin& p, int64_t ba
 }
 template <typename T, int RT>
 static void ort_launch_thin(const void* g, void* out, void* workspace, int64_t batch, int64_t m, int64_t n, int32_t steps, const float* coef, float eps,
-                            hipStream_t st) {
+                            LearnStream& st) {
   OrtThin p = {};
   p.m = (int)m; p.n = (int)n; p.tall = m > n; p.r = (int)(m < n ? m : n); p.k = (int)(m < n ? n : m); p.eps = eps;
   ort_thin_plan(p.r, p.k, p.blocks, p.chunks);
@@ -979,7 +979,7 @@ static void ort_launch_thin(const void* g, void* out, void* workspace, int64_t b
 
 template <typename T>
 static void ort_launch(const void* g, void* out, void* workspace, int64_t batch, int64_t m, int64_t n, int32_t steps, const float* coef, float eps,
-                       hipStream_t st) {
+                       LearnStream& st) {
   const int64_t r = m < n ? m : n, k = m < n ? n : m;
   if (ort_is_small(m, n)) {
     const int kt = (int)nof_div_up(k, 32);
@@ -1067,11 +1067,10 @@ extern "C" int nof_orthogonalize(const void* update, void* out, int32_t type, in
   NOF_ARG(update && out);
   const int64_t need = nof_orthogonalize_workspace_bytes(batch, m, n);
   NOF_ARG(need == 0 || (workspace && ((uintptr_t)workspace & 255) == 0 && workspace_bytes >= need));
-  hipStream_t st = (hipStream_t)stream;
-  LEARN_BEGIN();
+  LearnStream st = {(hipStream_t)stream, hipSuccess};
   if (type == NOF_TYPE_F32) ort_launch<float>(update, out, workspace, batch, m, n, steps, h_coef, eps, st);
   else if (type == NOF_TYPE_BF16) ort_launch<__bf16>(update, out, workspace, batch, m, n, steps, h_coef, eps, st);
   else ort_launch<_Float16>(update, out, workspace, batch, m, n, steps, h_coef, eps, st);
-  LEARN_END();
+  LEARN_END(st);
   return 0;
 }

@@ -624,12 +624,11 @@ extern "C" int nof_gated_scan_fwd(const void* gate, int64_t gate_sb, int64_t gat
   p.state = state; p.lengths = lengths; p.reverse = reverse;
   p.h = h; p.last = last; p.marks = marks;
   p.seg = (float*)workspace;
-  hipStream_t st = (hipStream_t)stream;
-  LEARN_BEGIN();
+  LearnStream st = {(hipStream_t)stream, hipSuccess};
   const unsigned x = (unsigned)(B * p.tiles);
   if (p.segs > 1) SCAN_PICK(k_scan_segments, dim3(x, p.segs - 1), dim3(64 * p.waves), false);
   SCAN_PICK(k_scan_fwd, dim3(x, p.segs), dim3(64 * p.waves));
-  LEARN_END();
+  LEARN_END(st);
   return 0;
 }
 
@@ -656,8 +655,7 @@ extern "C" int nof_gated_scan_bwd(const void* gate, int64_t gate_sb, int64_t gat
   p.dgate = dgate; p.dvalue = dvalue; p.dstate = dstate;
   p.seg = (float*)workspace;
   p.gpart = (float*)((char*)workspace + seg);
-  hipStream_t st = (hipStream_t)stream;
-  LEARN_BEGIN();
+  LearnStream st = {(hipStream_t)stream, hipSuccess};
   const unsigned x = (unsigned)(B * p.tiles);
   if (p.segs > 1) SCAN_PICK(k_scan_segments, dim3(x, p.segs - 1), dim3(64 * p.waves), true);
   SCAN_PICK(k_scan_bwd, dim3(x, p.segs), dim3(64 * p.waves));
@@ -668,13 +666,13 @@ extern "C" int nof_gated_scan_bwd(const void* gate, int64_t gate_sb, int64_t gat
     else if (gate_type == NOF_TYPE_BF16) LEARN_LAUNCH(k_scan_gate_sum<__bf16>, grid, dim3(256), 0, st, (const float*)p.gpart, (__bf16*)dgate, n, p.tiles_per_span);
     else LEARN_LAUNCH(k_scan_gate_sum<_Float16>, grid, dim3(256), 0, st, (const float*)p.gpart, (_Float16*)dgate, n, p.tiles_per_span);
   }
-  LEARN_END();
+  LEARN_END(st);
   return 0;
 }
 
 template <typename TG, typename T, int V>
 static void scan_launch_step(const void* gate, int64_t gate_sb, const void* value, int64_t value_sb, const float* state, float* new_state,
-                             void* h, int64_t B, int32_t D, int32_t G, hipStream_t st) {
+                             void* h, int64_t B, int32_t D, int32_t G, LearnStream& st) {
   const int per_row = (int)nof_div_up(D, 256 * V);
   LEARN_LAUNCH((k_scan_step<TG, T, V>), dim3((unsigned)(B * per_row)), dim3(256), 0, st, (const TG*)gate, gate_sb, (const T*)value,
                      value_sb, state, new_state, (T*)h, (int)B, D, G, per_row);
@@ -691,8 +689,7 @@ extern "C" int nof_gated_scan_step(const void* gate, int64_t gate_sb, int32_t ga
   NOF_ARG(scan_aligned(value, value_sb, 0, size, v) && scan_aligned(h, 0, 0, size, v));
   NOF_ARG(G != D || scan_aligned(gate, gate_sb, 0, (int)learn_type_size(gate_type), v));
   NOF_ARG(scan_aligned(state, 0, 0, 4, v) && scan_aligned(new_state, 0, 0, 4, v));
-  hipStream_t st = (hipStream_t)stream;
-  LEARN_BEGIN();
+  LearnStream st = {(hipStream_t)stream, hipSuccess};
 #define SCAN_STEP(TG, T, V) scan_launch_step<TG, T, V>(gate, gate_sb, value, value_sb, state, new_state, h, B, D, G, st)
   if (type == NOF_TYPE_F32) SCAN_STEP(float, float, 1);
   else if (type == NOF_TYPE_BF16 && gate_type == type) { if (v == 2) SCAN_STEP(__bf16, __bf16, 2); else SCAN_STEP(__bf16, __bf16, 1); }
@@ -700,6 +697,6 @@ extern "C" int nof_gated_scan_step(const void* gate, int64_t gate_sb, int32_t ga
   else if (gate_type == type) { if (v == 2) SCAN_STEP(_Float16, _Float16, 2); else SCAN_STEP(_Float16, _Float16, 1); }
   else { if (v == 2) SCAN_STEP(float, _Float16, 2); else SCAN_STEP(float, _Float16, 1); }
 #undef SCAN_STEP
-  LEARN_END();
+  LEARN_END(st);
   return 0;
 }
