@@ -8,9 +8,10 @@
 // Operands are fp16 pairs hi + lo / 2048 of 4096 times the value: off by 2^-23 of the value, or by 2^-48 where that is more (hi is subnormal
 // below 2^-26 and lo takes what it leaves; with lo as it is, it would be subnormal below 2^-15 already: rows of 1e-5 of the largest were off by
 // 1e-4 so, and steps that lift them made them most of the result).  Products hi hi + (hi lo + lo hi) / 2048 accumulate in binary32, large and
-// small apart: as exact as a binary32 product at a third of the fp16 rate, which on this card is some three times the binary32 rate.  One fp16
-// product instead would be off by 2^-12 per step, which small singular values amplify by up to a^steps: 4 % for a matrix of rank 4 plus noise of 1e-4.  The norm is summed in 64 bits: an error of it is common to all
-// values and the polynomial amplifies it.  Of at most 64 rows, A A is formed more exactly (ort_square).
+// small apart: a product is off by 5 * 2^-24 at most where binary32 rounds it by 2^-24, at a third of the fp16 rate, which on this card is some
+// three times the binary32 rate.  One fp16 product instead would be off by 2^-12 per step, which small singular values amplify by up to a^steps:
+// 4 % for a matrix of rank 4 plus noise of 1e-4.  The norm is summed in 64 bits: an error of it is common to all values and the polynomial
+// amplifies it.  Of at most 64 rows, A A is formed more exactly (ort_square).
 //
 // Matrices of at most 128 x 128 take one workgroup and one launch (k_ortho_small): X lives in accumulator registers, operands in LDS.
 // Thin ones, of at most 128 on one side, take a launch a step (k_ortho_thin).  Larger ones are three launches a step over images of X, X^T,

@@ -318,8 +318,9 @@ def orthogonalize(update, steps=5, coefficients=QUINTIC, eps=1e-30, out=None):
     """The orthogonalised form of weight updates [..., m, n]: X = update / max(|update|_F, eps), then `steps` times
     X <- (a + b A + c A A) X, A = X X^T (over the shorter side), with coefficients (a, b, c) -- one triple, or a tuple of `steps` of them.
     The singular vectors stay, the singular values go to the quintic's fixed band around 1.  Result in the update's type, in `out` (which
-    may be `update`) where given.  As exact as binary32 products for what is larger than 2^-25 of the norm, to 2^-48 of the norm below.  Equal
-    calls give equal bits; how many matrices share a call may change a matrix's last bits.  Coefficients that let a singular value leave [0, 2] are refused."""
+    may be `update`) where given.  Products hold their operands to 2^-23 of themselves or 2^-48 of the norm and add in
+    binary32.  Equal calls give equal bits; how many matrices share a call may change a matrix's last bits.  Coefficients that let a singular
+    value leave [0, 2] are refused."""
     if not (update.dim() >= 2 and update.dtype in _TYPE):
         raise NofError('orthogonalize: update must be [..., m, n] float32, bfloat16 or float16')
     m, n = update.shape[-2:]

@@ -598,9 +598,9 @@ int nof_gated_scan_step(const void* gate, int64_t gate_sb, int32_t gate_type, co
 /* The orthogonalised update of `batch` weight matrices [m,n]: X = update / max(|update|_F, eps) (a zero matrix: zeros), then for each of
  * `steps` <= 32 triples (a, b, c) of h_coef: X <- (a I + b A + c A A) X with A = X X^T (X^T X for m > n) -> out [batch,m,n] in the update's
  * type (may be `update` itself).  A singular value s becomes a s + b s^3 + c s^5; triples that take a start in [0, 1] beyond 2, or the
- * bracket beyond 15, are refused.  Products are as exact as binary32's (fp16 operand pairs, binary32 sums) for what is larger than 2^-25 of
- * max(|update|_F, eps), and exact to 2^-48 of that below: rows or columns of a millionth of the others keep their precision, those of 1e-9 some
- * five digits.  The norm is summed in 64 bits.  m, n <= 16384, batch < 65536. */
+ * bracket beyond 15, are refused.  Products hold their operands (fp16 pairs) to 2^-23 of themselves, or to 2^-48 of max(|update|_F, eps) where that is
+ * more, and add in binary32: a product is off by at most five times what a binary32 one is, and rows or columns of a millionth of the others keep
+ * their precision, those of 1e-9 some five digits.  The norm is summed in 64 bits.  m, n <= 16384, batch < 65536. */
 int64_t nof_orthogonalize_workspace_bytes(int64_t batch, int64_t m, int64_t n);
 int nof_orthogonalize(const void* update, void* out, int32_t type, int32_t steps, const float* h_coef, float eps, void* workspace,
                       int64_t workspace_bytes, int64_t batch, int64_t m, int64_t n, void* stream);
