@@ -76,19 +76,21 @@ def _apart(a, b):
     return x + n <= y or y + m <= x or (x == y and n == m) or n == 0 or m == 0
 
 
-def _clear_of(a, x, strides):
-    """whether what is written to the contiguous `a` cannot be read from x by another lane: x lies apart, or each element of it is a's own"""
-    if x.dtype == a.dtype and x.data_ptr() == a.data_ptr() and x.shape == a.shape and x.is_contiguous():
+def _clear_of(lo, hi, D, x, at, row):
+    """whether what is written to a contiguous [B, D] float32 at the addresses lo to hi cannot be read from x [B, C], `row` elements between rows,
+    by another lane: x lies apart, or each element of it is the written one's own"""
+    if hi <= at or lo == hi:
         return True
-    size = x.element_size()
-    last = sum([(n - 1) * st for n, st in zip(x.shape, strides)]) + x.shape[-1]                 # (`strides`: all but the last, whose step is 1)
-    lo, at = a.data_ptr(), x.data_ptr()
-    return lo + a.numel() * a.element_size() <= at or at + last * size <= lo or a.numel() == 0 or x.numel() == 0
+    rows, cols = x.shape
+    if at + ((rows - 1) * row + cols) * x.element_size() <= lo or cols == 0:
+        return True
+    return at == lo and cols == D and x.dtype == torch.float32 and rows * D * 4 == hi - lo and (row == D or rows == 1)
 
 
 def _rows(x):
     """x [N, D] with its elements side by side in a row: (tensor, elements between rows)"""
-    x = x.resolve_neg()                                                  # (a view like z.conj().imag holds the other sign)
+    if x.is_neg():                                                       # (a view like z.conj().imag holds the other sign)
+        x = x.resolve_neg()
     if x.shape[1] > 1 and x.stride(1) != 1:
         x = x.contiguous()
     return x, x.stride(0) if x.shape[0] > 1 else x.shape[1]
@@ -157,7 +159,8 @@ def _scan_even(dtype, D, G):
 
 def _scan_strided(x, even):
     """x [B, T, C] (or [B, C]) as the kernels take it -- channels side by side, two-channel loads on their border -- and its strides"""
-    x = x.resolve_neg()
+    if x.is_neg():
+        x = x.resolve_neg()
     if x.is_contiguous():
         n = x.shape
         st = (n[1],) if len(n) == 2 else (n[1] * n[2], n[2])
@@ -179,7 +182,10 @@ def _flat(x, even):
     """a [B, D] float32 argument as the kernels take it, or None"""
     if x is None:
         return None
-    x = x.resolve_neg().contiguous()
+    if x.is_neg():
+        x = x.resolve_neg()
+    if not x.is_contiguous():
+        x = x.contiguous()
     return x.clone() if even and x.data_ptr() % 8 else x
 
 
@@ -285,18 +291,21 @@ def gated_scan_step(gate, value, state, new_state=None):
     dt = value.dtype
     even = _scan_even(dt, D, G)
     (value, vst), (gate, gst), state = _scan_strided(value, even), _scan_strided(gate, even and G == D), _flat(state, even)
+    gate_at, value_at = gate.data_ptr(), value.data_ptr()
     if new_state is None:
         new_state = state.new_empty((B, D))
+        lo = new_state.data_ptr()
     else:
-        if even and new_state.data_ptr() % 8:
+        lo = new_state.data_ptr()
+        hi = lo + 4 * B * D
+        if even and lo % 8:
             raise NofError('gated_scan_step: new_state must start on an 8-byte border')
-        if not _apart(new_state, state):
+        if state is not new_state and not _apart(new_state, state):
             raise NofError('gated_scan_step: new_state must be state itself or lie apart from it')
-        if not (_clear_of(new_state, value, vst) and _clear_of(new_state, gate, gst)):
+        if not (_clear_of(lo, hi, D, value, value_at, vst[0]) and _clear_of(lo, hi, D, gate, gate_at, gst[0])):
             raise NofError('gated_scan_step: new_state must lie apart from gate and value')
     h = value.new_empty((B, D))
-    _call(dev, 'nof_gated_scan_step', gate.data_ptr(), *gst, _TYPE[gate.dtype], value.data_ptr(), *vst, _TYPE[dt], state.data_ptr(),
-          new_state.data_ptr(), h.data_ptr(), B, D, G)
+    _call(dev, 'nof_gated_scan_step', gate_at, *gst, _TYPE[gate.dtype], value_at, *vst, _TYPE[dt], state.data_ptr(), lo, h.data_ptr(), B, D, G)
     return h, new_state
 
 

@@ -11,7 +11,7 @@ def test_what_a_new_state_overlaps():
     a = line[10:34].view(4, 6)
 
     def clear(x):
-        return L._clear_of(a, x, x.stride()[:-1])
+        return L._clear_of(a.data_ptr(), a.data_ptr() + 96, 6, x, x.data_ptr(), x.stride(0))
 
     assert clear(a) and clear(line[34:58].view(4, 6)) and clear(line[0:10].view(2, 5)) and clear(line[:0].view(0, 6))
     for lo in (5, 9, 11, 33):
