@@ -1,4 +1,5 @@
-"""The orthogonalised update on the field's own weight matrices, by the hook that a training step calls between its backward and Adam: matrices move by it, everything else by Adam, and the next step runs on the new weights."""
+"""The orthogonalised update on the field's own weight matrices, by the hook that a training step calls between its backward and Adam: matrices
+move by it, everything else by Adam, and the next step runs on the new weights."""
 import numpy as np
 import pytest
 import torch
